@@ -21,12 +21,15 @@
  *   rspx_qkv_rope_cache q_norm/k_norm + RoPE + KV write of one decoder layer
  *                       (rmsnorm.py:25, HF apply_rotary_pos_emb, kv_buffer.py:32-36 update)
  *   rspx_trie_mask      respect/decoding/verify.py:22-41 mask + dispatch.py:94-115 padding
- *   rspx_kv_compact     respect/decoding/kv_buffer.py:93 compact(cache, prompt_len, base, slots)
  *   rspx_argmax_rows    respect/decoding/acceptance.py:20 greedy_token(logits, offset, size)
  *   rspx_square         respect/system/fused.py:126 _sq_k (the squares of rmsnorm, fused.py:176)
  *   rspx_add_sq         respect/system/fused.py:185 add_sq(r, h)
  *   rspx_norm_apply     respect/system/fused.py:148 _norm_apply_k (norm_from, fused.py:165)
  *   rspx_rope_vision    respect/system/fused.py:97  rope_vision(x, cos, sin)
+ *
+ * No counterpart in the reference, which answers one request at a time: serving several
+ * sequences at once.
+ *   rspx_prompt_attn    causal attention over whole prompts, packed
  */
 #ifndef RESPECT_AMD_H
 #define RESPECT_AMD_H
@@ -67,7 +70,7 @@ const char* rspx_strerror(int code);
 
 /* Library version.  The last number goes up with every change of a signature in this
  * header: code compiled against another one compares it before its first call. */
-#define RSPX_VERSION "respect_amd 0.1.0 gfx950 abi 1"
+#define RSPX_VERSION "respect_amd 0.1.0 gfx950 abi 2"
 const char* rspx_version(void);
 
 /* ---------------------------------------------------------------- attention
@@ -444,6 +447,26 @@ int rspx_norm_apply(const void* x, int64_t sx, const float* var, const void* w, 
                     float eps, void* stream);
 int rspx_rope_vision(const void* x, int64_t sxl, int64_t sxh, const float* cos, const float* sin, int64_t scl,
                      void* y, int L, int NH, int D, void* stream);
+
+/* ---------------------------------------------------------------- prompt attention
+ * Causal attention over whole prompts, packed one after the other.
+ *   q [Tq, H, D], k / v [Tk, HK, D], out [Tq, H, D] bf16; strides in elements, D
+ *   contiguous, bases and strides 16-byte aligned (out: 8), strides of k and v below
+ *   2^24 elements.  Head h reads kv head h / (H / HK), any H / HK.  D in {32, 64, 128, 256}.
+ * tiles: device int32 [n_tiles][4], each (first row of q, rows, first key of its
+ * sequence, keys the first row sees): row first + i attends to keys [key0, key0 +
+ * seen + i).  rows <= rspx_prompt_attn_tile_rows(H, HK); every row of q in one tile
+ * (rows in none are left unwritten); seen may be negative: a row that sees no key gets
+ * zeros.  Tiles with the most keys first keep the device busy to the end.  A tile that
+ * points outside [0, Tq) or [0, Tk) is cut to them.  sm_scale > 0.
+ * fp32 softmax, probabilities rounded to bf16 for the product with v, one rounding of
+ * the result.  A row's bits depend on its own sequence up to the row alone: not on the
+ * other sequences, on the tiles' size or order, or on what later keys and values hold.
+ */
+int rspx_prompt_attn_tile_rows(int H, int HK);
+int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh, const void* v,
+                     int64_t svt, int64_t svh, const int32_t* tiles, int n_tiles, void* out, int64_t sot, int64_t soh,
+                     int H, int HK, int Tq, int Tk, int D, float sm_scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,342 @@
+// Causal attention over whole prompts, packed one after the other, for gfx950.
+//
+//   o[t, h] = sum_j softmax_j(scale q[t, h] . k_j) v_j
+//
+// over the keys j that row t of its sequence sees.  The work is a list of tiles of at most
+// 32 RW rows of one sequence; a workgroup takes one tile for 4 / RW query heads of one kv
+// head, each wave 32 rows of one head.  Keys and values of 64 positions at a time go from
+// memory straight into LDS (two stages) and serve all four waves.
+//
+// A wave computes S^T = K Q^T by v_mfma_f32_32x32x16_bf16, so a lane holds 32 scores of one
+// row: the softmax (fp32, a running maximum that moves only when a score passes it by
+// 2^kTau) needs no lane exchange but the rare move's.  The probabilities, rounded to bf16
+// as the trie attention rounds them (relative error 2^-9 each, against fp32 sums), are used
+// in place as the B operand of O^T += V^T P^T with V read transposed from LDS.
+//
+// Every row is computed from its own column of the MFMA tiles in 64-key steps from the
+// sequence's first key on: its bits depend on its sequence alone, not on the pack, on the
+// tile it falls in or on later rows.
+#include <type_traits>
+
+#include "common.h"
+#include "respect_amd.h"
+
+namespace rspx {
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kKeys = 64;            // keys of a step
+constexpr int kRows = 32;            // rows of a wave
+constexpr float kTau = 8.0f;         // log2 headroom before the reference maximum moves
+constexpr float kNone = -1e30f;      // reference maximum before the first key
+
+struct PromptArgs {
+  const uint16_t *q, *k, *v;
+  const int* tiles;            // [n][4]: first row, rows, first key, keys the first row sees
+  uint16_t* out;
+  int64_t sqt, sqh, skt, skh, svt, svh, sot, soh;
+  int G, Tq, Tk, units;        // units = H / heads per workgroup
+  float c;                     // scale * log2(e)
+};
+
+// Non-template wrappers: the host pass rejects these builtins inside templates.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint32_t nbytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)nbytes, 0x00020000);
+}
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t r, int voff, lds_char* dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, 0, 0, 0);
+}
+__device__ __forceinline__ s16x4 tr_read(const lds_char* __restrict__ p) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+}
+
+// 16-byte unit swizzles of a staged row of U units: eight consecutive keys' units of one
+// column lie in different banks (K), four keys' pairs of units (V).
+template <int D>
+__device__ __forceinline__ int kswizzle(int key) {
+  constexpr int U = D / 8;
+  if constexpr (U >= 8) return key % 8;
+  else return (key / (8 / U)) % U;
+}
+template <int D>
+__device__ __forceinline__ int vswizzle(int key) {
+  constexpr int U = D / 8;
+  if constexpr (U >= 16) return 2 * (key % 8);
+  else return 2 * ((key / (16 / U)) % (U / 2));
+}
+
+// HW heads and RW = 4 / HW row blocks of 32 rows per workgroup.
+template <int D, int HW>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(PromptArgs A) {
+  constexpr int U = D / 8, NS = D / 16, DT = D / 32;
+  constexpr int kBytes = kKeys * D * 2;                    // K or V of one stage
+  constexpr int kLoads = kBytes / 1024 / 4;                // 1 KB loads per wave, K and V each
+  __shared__ __align__(16) char lds[2][2][kBytes];
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int unit = blockIdx.x % A.units, tile = blockIdx.x / A.units;
+  const int head = unit * HW + w % HW;
+  const int kvh = (unit * HW) / A.G;
+  const int* T = A.tiles + 4 * (int64_t)tile;
+  // A tile that points outside the tensors is cut to them.
+  const int q0 = min(max(T[0], 0), A.Tq), k0 = min(max(T[2], 0), A.Tk);
+  const int rows = min(min(max(T[1], 0), kRows * (4 / HW)), A.Tq - q0);
+  const int seen0 = T[3];                                  // row i sees keys [k0, k0 + seen0 + i)
+  const int keys = (int)min(max((int64_t)seen0 + rows - 1, (int64_t)0), (int64_t)(A.Tk - k0));
+
+  const int rb = kRows * (w / HW);                         // this wave's rows in the tile
+  const int row = rb + col;
+  const int seen = min(seen0 + row, keys);                 // keys of this lane's row
+  const bool live = row < rows;
+
+  // B operand of the scores: lane (col, half) holds row col, head_dim 16 i + 8 half .. + 7.
+  bf16x8 qf[NS];
+  const uint16_t* qrow = A.q + (int64_t)(q0 + (live ? row : 0)) * A.sqt + (int64_t)head * A.sqh + 8 * half;
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    u32x4 x = {0, 0, 0, 0};
+    if (live) x = *reinterpret_cast<const u32x4*>(qrow + 16 * i);
+    qf[i] = __builtin_bit_cast(bf16x8, x);
+  }
+
+  // Byte offsets of this lane's units of a step's K and V: load j of wave w fills units
+  // 64 (4 j + w) + lane of the stage.  Rows past the last key read as zeros.
+  const uint16_t* kp = A.k + (int64_t)k0 * A.skt + (int64_t)kvh * A.skh;
+  const uint16_t* vp = A.v + (int64_t)k0 * A.svt + (int64_t)kvh * A.svh;
+  int ko[kLoads], vo[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int u = 64 * (4 * j + w) + lane, key = u / U;
+    ko[j] = (int)(2 * key * A.skt) + 16 * ((u % U) ^ kswizzle<D>(key));
+    vo[j] = (int)(2 * key * A.svt) + 16 * ((u % U) ^ vswizzle<D>(key));
+  }
+  auto issue = [&](int t) {
+    const int left = min(keys - t * kKeys, kKeys);         // > 0
+    const auto rk = rsrc(kp + (int64_t)t * kKeys * A.skt, (uint32_t)(2 * (left - 1) * A.skt + 2 * D));
+    const auto rv = rsrc(vp + (int64_t)t * kKeys * A.svt, (uint32_t)(2 * (left - 1) * A.svt + 2 * D));
+    lds_char* dk = (lds_char*)lds[t & 1][0];
+    lds_char* dv = (lds_char*)lds[t & 1][1];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) to_lds(rk, ko[j], dk + 1024 * (4 * j + w));
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) to_lds(rv, vo[j], dv + 1024 * (4 * j + w));
+  };
+
+  float mref = kNone, lsum = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int j = 0; j < DT; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+
+  const int steps = (keys + kKeys - 1) / kKeys;
+  if (steps > 0) issue(0);
+  // One step of 64 keys.  `edge`: some row of the tile may not see all of them.
+  auto step = [&](int t, auto edge) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of step t
+    __syncthreads();                                       // everyone's; and step t - 1 is read
+    if (t + 1 < steps) issue(t + 1);
+    const lds_char* sk = (const lds_char*)lds[t & 1][0];
+    const lds_char* sv = (const lds_char*)lds[t & 1][1];
+
+    // S^T: two blocks of 32 keys.  Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
+    f32x16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+      const int key = 32 * kb + col;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const u32x4 x = *(const __attribute__((address_space(3))) u32x4*)(
+            sk + 16 * (key * U + ((2 * i + half) ^ kswizzle<D>(key))));
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[i], s[kb], 0, 0, 0);
+      }
+    }
+    if constexpr (edge) {   // keys that a row does not see
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (t * kKeys + 32 * kb + 8 * (e / 4) + 4 * half + e % 4 >= seen) s[kb][e] = kNegInf;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+    if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
+      const float top = fmaxf(mx, shfl_xor(mx, 32)) * A.c;
+      const float mn = top > mref + kTau ? top : mref;     // rows that stay get a factor of exactly 1
+      const float alpha = fexp2(mref - mn);
+      lsum = lsum * alpha;
+      mref = mn;
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
+    }
+    bf16x8 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 8 * i + 2 * e;
+        const float a = fexp2(__builtin_fmaf(s[r / 16][r % 16], A.c, -mref));
+        const float b = fexp2(__builtin_fmaf(s[r / 16][r % 16 + 1], A.c, -mref));
+        lsum = lsum + a;
+        lsum = lsum + b;
+        x[e] = pack_bf16x2(a, b);
+      }
+      p[i] = __builtin_bit_cast(bf16x8, x);
+    }
+    // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
+    // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
+    auto vop = [&](int i, int j) {
+      s16x4 h[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const int l16 = lane & 15;
+        const int key = 16 * i + 8 * z + 4 * half + (l16 >> 2);
+        const int u = 4 * j + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+        h[z] = tr_read(sv + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1));
+      }
+      return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // A key that a row does not see has p = 0, but 0 * inf and 0 * NaN are NaN: such a value
+    // among the step's may not reach the rows before it.
+    bool odd = false;
+    if constexpr (edge) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+          asm volatile("" ::: "memory");                   // one operand at a time: registers
+          const s16x8 x = vop(i, j);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) odd |= (x[e] & 0x7f80) == 0x7f80;
+        }
+      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    }
+    if (edge && odd) {
+      // The values that are not finite go to the rows that see them one by one, and the
+      // product runs without them: every other sum keeps its bits.
+      const int mine = seen - t * kKeys;                   // keys of the step that this lane's row sees
+#pragma unroll 1
+      for (int key = 0; key < kKeys; ++key)
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int d = 32 * j + 8 * (e / 4) + 4 * half + e % 4;
+            const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
+                sv + 16 * (key * U + ((d / 8) ^ vswizzle<D>(key))) + 2 * (d % 8));
+            if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + bf16_to_f32(x);
+          }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+          asm volatile("" ::: "memory");                   // one operand at a time: registers
+          s16x8 x = vop(i, j);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = (x[e] & 0x7f80) == 0x7f80 ? (short)0 : x[e];
+          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), p[i], acc[j], 0, 0, 0);
+        }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vop(i, j)), p[i], acc[j], 0, 0, 0);
+  };
+  const int whole = min(max(seen0, 0), keys) / kKeys;      // steps that every row sees whole
+  int t = 0;
+  for (; t < whole; ++t) step(t, std::false_type());
+  for (; t < steps; ++t) step(t, std::true_type());
+
+  // Lane (col, half): row col, head_dim 32 j + 8 (e / 4) + 4 half + e % 4.
+  if (!live) return;
+  lsum = lsum + shfl_xor(lsum, 32);
+  const float inv = 1.0f / lsum;
+  uint16_t* o = A.out + (int64_t)(q0 + row) * A.sot + (int64_t)head * A.soh + 4 * half;
+#pragma unroll
+  for (int j = 0; j < DT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      u32x2 x;
+#pragma unroll
+      for (int z = 0; z < 2; ++z) x[z] = pack_bf16x2(acc[j][4 * e + 2 * z] * inv, acc[j][4 * e + 2 * z + 1] * inv);
+      if (seen <= 0) x = u32x2{0, 0};                      // a row that sees no key
+      *reinterpret_cast<u32x2*>(o + 32 * j + 8 * e) = x;
+    }
+}
+
+int heads_per_group(int G) { return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1; }
+
+template <int D>
+int launch(const PromptArgs& A, int HW, int n, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)A.units * n));
+  if (HW == 4) hipLaunchKernelGGL((prompt_attn_kernel<D, 4>), grid, dim3(256), 0, s, A);
+  else if (HW == 2) hipLaunchKernelGGL((prompt_attn_kernel<D, 2>), grid, dim3(256), 0, s, A);
+  else hipLaunchKernelGGL((prompt_attn_kernel<D, 1>), grid, dim3(256), 0, s, A);
+  return hipGetLastError() == hipSuccess ? RSPX_OK : RSPX_ELAUNCH;
+}
+
+}  // namespace
+
+}  // namespace rspx
+
+using namespace rspx;
+
+extern "C" int rspx_prompt_attn_tile_rows(int H, int HK) {
+  if (H < 1 || HK < 1 || H % HK) return -1;
+  return kRows * (4 / heads_per_group(H / HK));
+}
+
+extern "C" int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh,
+                                const void* v, int64_t svt, int64_t svh, const int32_t* tiles, int n_tiles, void* out,
+                                int64_t sot, int64_t soh, int H, int HK, int Tq, int Tk, int D, float sm_scale,
+                                void* stream) {
+  if (H < 1 || HK < 1 || H % HK || Tq < 0 || Tk < 0 || n_tiles < 0) return RSPX_EINVAL;
+  if (!(sm_scale > 0.f) || sm_scale > 3e38f) return RSPX_EINVAL;
+  if (D != 32 && D != 64 && D != 128 && D != 256) return RSPX_EUNSUPPORTED;
+  // Byte offsets inside a 64-key step are 32-bit.
+  constexpr int64_t kMaxStride = 1 << 24;
+  if (sqt < 0 || sqh < 0 || skt < 0 || skh < 0 || svt < 0 || svh < 0 || sot < 0 || soh < 0 || skt >= kMaxStride ||
+      svt >= kMaxStride)
+    return RSPX_EINVAL;
+  if (n_tiles == 0 || Tq == 0) return RSPX_OK;
+  if (!q || !tiles || !out || (Tk > 0 && (!k || !v))) return RSPX_EINVAL;
+  auto al = [](const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; };
+  if (!al(q, 16) || !al(k, 16) || !al(v, 16) || !al(out, 8) || sqt % 8 || sqh % 8 || skt % 8 || skh % 8 || svt % 8 ||
+      svh % 8 || sot % 4 || soh % 4)
+    return RSPX_EALIGN;
+  PromptArgs A;
+  A.q = static_cast<const uint16_t*>(q);
+  A.k = static_cast<const uint16_t*>(k);
+  A.v = static_cast<const uint16_t*>(v);
+  A.tiles = tiles;
+  A.out = static_cast<uint16_t*>(out);
+  A.sqt = sqt, A.sqh = sqh, A.skt = skt, A.skh = skh, A.svt = svt, A.svh = svh, A.sot = sot, A.soh = soh;
+  A.G = H / HK, A.Tq = Tq, A.Tk = Tk;
+  const int HW = heads_per_group(A.G);
+  A.units = H / HW;
+  if ((int64_t)A.units * n_tiles > INT32_MAX) return RSPX_EINVAL;
+  A.c = sm_scale * 1.44269504088896340736f;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (D) {
+    case 32: return launch<32>(A, HW, n_tiles, s);
+    case 64: return launch<64>(A, HW, n_tiles, s);
+    case 128: return launch<128>(A, HW, n_tiles, s);
+    default: return launch<256>(A, HW, n_tiles, s);
+  }
+}
