@@ -30,6 +30,7 @@
  * No counterpart in the reference, which answers one request at a time: serving several
  * sequences at once.
  *   rspx_prompt_attn    causal attention over whole prompts, packed
+ *   rspx_paged_attn     attention of one new token per sequence over a paged cache
  */
 #ifndef RESPECT_AMD_H
 #define RESPECT_AMD_H
@@ -467,6 +468,27 @@ int rspx_prompt_attn_tile_rows(int H, int HK);
 int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh, const void* v,
                      int64_t svt, int64_t svh, const int32_t* tiles, int n_tiles, void* out, int64_t sot, int64_t soh,
                      int H, int HK, int Tq, int Tk, int D, float sm_scale, void* stream);
+
+/* ---------------------------------------------------------------- paged attention
+ * Attention of one new token per sequence over a paged KV cache.
+ *   q [B, H, D], out [B, H, D] bf16; kc / vc [HK, pages * page, D] (head and slot
+ *   strides); table [B][width] int32 (row stride stb): key j of sequence b is pool row
+ *   table[b][j / page] * page + j % page; lens [B] int32: the keys of each sequence, the
+ *   new token's own among them.  D contiguous, 16-byte aligned bases and strides (out:
+ *   any).  page a power of two; H / HK <= 16; D in {32, 64, 128, 256}; sm_scale > 0.
+ * lens[b] == 0 gives zeros.  A length that is negative or above width * page, and a
+ * page that is none among those a sequence reads, give NaN rows; nothing outside the
+ * pool is read.  Table entries past a sequence's length are not read.
+ * fp32 softmax, probabilities as two bf16 terms for the product with v, one rounding
+ * of the result.  A sequence's bits depend on its own keys and length alone.
+ * workspace: rspx_paged_attn_workspace_bytes bytes, 16-byte aligned, of any content; not
+ * shared by calls that can run at the same time.
+ */
+int64_t rspx_paged_attn_workspace_bytes(int B, int H, int D, int page, int width);
+int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn, const void* vc,
+                    int64_t svh, int64_t svn, const int32_t* table, int64_t stb, const int32_t* lens, void* out,
+                    int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages, int page, int width,
+                    float sm_scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
