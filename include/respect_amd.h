@@ -21,6 +21,7 @@
  *   rspx_qkv_rope_cache q_norm/k_norm + RoPE + KV write of one decoder layer
  *                       (rmsnorm.py:25, HF apply_rotary_pos_emb, kv_buffer.py:32-36 update)
  *   rspx_trie_mask      respect/decoding/verify.py:22-41 mask + dispatch.py:94-115 padding
+ *   rspx_kv_compact     respect/decoding/kv_buffer.py:93 compact(cache, prompt_len, base, slots)
  *   rspx_argmax_rows    respect/decoding/acceptance.py:20 greedy_token(logits, offset, size)
  *   rspx_square         respect/system/fused.py:126 _sq_k (the squares of rmsnorm, fused.py:176)
  *   rspx_add_sq         respect/system/fused.py:185 add_sq(r, h)
@@ -31,6 +32,7 @@
  * sequences at once.
  *   rspx_prompt_attn    causal attention over whole prompts, packed
  *   rspx_paged_attn     attention of one new token per sequence over a paged cache
+ *   rspx_kv_move, rspx_kv_write   rows of a paged cache moved and written
  */
 #ifndef RESPECT_AMD_H
 #define RESPECT_AMD_H
@@ -489,6 +491,23 @@ int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int
                     int64_t svh, int64_t svn, const int32_t* table, int64_t stb, const int32_t* lens, void* out,
                     int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages, int page, int width,
                     float sm_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- rows of a paged cache
+ * rspx_kv_move: for each of n_tensors pools (device array `bases` of base addresses,
+ * each [HK][cap][D] bf16, head stride sh, slot stride sn) and each head, the moves
+ * (src slot, dst slot) of device int32 moves[n_moves][2].  groups [n_groups + 1] cuts
+ * them into groups: those of one group take effect in order, provided no destination
+ * is the source of a later move of the group (rows moved down in increasing order are
+ * that); different groups must not touch each other's destinations.  A move with a
+ * slot outside [0, cap) is skipped.  D % 8 == 0.
+ * rspx_kv_write: rows k / v [T, HK, D] of one layer to slots[t] of its pools; a slot
+ * outside [0, cap) is skipped; slots differ.
+ */
+int rspx_kv_move(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh, int64_t sn, int cap,
+                 const int32_t* groups, int n_groups, const int32_t* moves, int n_moves, void* stream);
+int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh,
+                  const int32_t* slots, int T, int cap, void* cache_k, int64_t sckh, int64_t sckn, void* cache_v,
+                  int64_t scvh, int64_t scvn, int HK, int D, void* stream);
 
 #ifdef __cplusplus
 }
