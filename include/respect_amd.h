@@ -33,6 +33,7 @@
  *   rspx_prompt_attn    causal attention over whole prompts, packed
  *   rspx_paged_attn     attention of one new token per sequence over a paged cache
  *   rspx_kv_move, rspx_kv_write   rows of a paged cache moved and written
+ *   rspx_token_logprobs log probabilities, entropy and best alternatives per row
  */
 #ifndef RESPECT_AMD_H
 #define RESPECT_AMD_H
@@ -508,6 +509,21 @@ int rspx_kv_move(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh
 int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh,
                   const int32_t* slots, int T, int cap, void* cache_k, int64_t sckh, int64_t sckn, void* cache_v,
                   int64_t scvh, int64_t scvn, int HK, int D, void* stream);
+
+/* ---------------------------------------------------------------- scores of given tokens
+ * Per row of logits [M, V] (fp32, row stride sl, 16-byte aligned rows), with columns
+ * [off, off + size) counted as -inf: given[m] = log p of tokens[m], entropy[m] (nats),
+ * and the `top` largest scores' log p (values [M, top], best first) and columns (ids
+ * [M, top]).  Ties go to the lowest index, NaN is the largest value; a row that holds a
+ * NaN or +inf has NaN results.  A token outside [0, V): given NaN.  A row with every
+ * score -inf: -inf, entropy 0.  top <= 64 and <= V; 0: values / ids unused.
+ * A row's bits do not depend on M.  workspace: rspx_token_logprobs_workspace_bytes
+ * bytes, 8-byte aligned, of any content.
+ */
+int64_t rspx_token_logprobs_workspace_bytes(int M, int V, int top);
+int rspx_token_logprobs(const float* logits, int64_t sl, int M, int V, int off, int size, const int64_t* tokens,
+                        int top, float* given, float* entropy, float* values, int64_t* ids, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

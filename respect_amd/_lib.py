@@ -96,6 +96,9 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_kv_move": (_i32, [_c_p, _i32, _i32, _i32, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
     "rspx_kv_write": (_i32, [_c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i32, _i32, _c_p, _i64, _i64, _c_p, _i64, _i64,
                              _i32, _i32, _c_p]),
+    "rspx_token_logprobs_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "rspx_token_logprobs": (_i32, [_c_p, _i64, _i32, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _i64,
+                                   _c_p]),
 }
 
 _lib = None
