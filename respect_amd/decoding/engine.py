@@ -33,6 +33,9 @@ rows the call carries, and attention folds a row's node slots in slot order,
 so a token verified inside a trie gets the same logits and KV bits as when it
 is decoded alone -- the property the reference's verification relies on
 (respect/decoding/verify.py:12-46, respect/decoding/sequential.py:17-42).
+
+``prefill_batch`` and ``step_batch`` run the same layers for several sequences at once
+over a PagedKVCache, with rspx_prompt_attn and rspx_paged_attn as the attention.
 """
 from __future__ import annotations
 
@@ -44,6 +47,8 @@ import torch
 from .. import _lib
 from ..kernels.attention import raise_if_gave_up, status_word, trie_attn
 from ..kernels.gemm import TiledWeight, tile_weight
+from ..kernels.paged_attention import paged_attn
+from ..kernels.prompt_attention import PackedPrompts, prompt_attn
 from ..system.fused import rope_tables
 from .acceptance import greedy_token
 
@@ -69,6 +74,12 @@ class DecoderConfig:
         H, F, V = self.hidden, self.ffn, self.vocab
         per_layer = self.qkv_rows * H + H * self.heads * self.head_dim + 2 * F * H + H * F + 2 * H + 2 * self.head_dim
         return 2 * (self.layers * per_layer + V * H + H)
+
+
+def _reach(n: int) -> int:
+    """Positions the rotary tables hold for a sequence of n tokens: a power of two, so that they
+    seldom grow as it does."""
+    return 1 << max(10, (n - 1).bit_length())
 
 
 class Layer:
@@ -220,12 +231,33 @@ class Decoder:
         ``kv_only``: only the K/V of the tokens is wanted; the last layer stops
         once it has written them, and None is returned."""
         cfg = self.cfg
+        T = int(ids.shape[0])
+        if P < 0 or NN < 0 or P + NN > cache.cap:
+            raise ValueError(f"forward: prompt {P} + node segment {NN} exceeds the cache's {cache.cap} slots")
+        HQ, HK, D = cfg.heads, cfg.kv_heads, cfg.head_dim
+        att = torch.empty(-(-T // 64) * 64 * HQ * D, dtype=torch.bfloat16, device=self.device)   # [T, HQ D], tiled
+        ws_attn = self._workspace("attn", _lib.lib().rspx_trie_attn_workspace_bytes(HQ, HK, T, P, D))
+        self.attn_ws_used = ws_attn   # its first word flags a wait that gave up (kernels.attention.status_word)
+
+        def attend(li, qo):
+            ck, cv = cache.k[li], cache.v[li]
+            trie_attn(qo.permute(1, 0, 2), ck[:, :P], cv[:, :P], ck[:, P:P + NN], cv[:, P:P + NN], msk,
+                      self.sm_scale, out=att, workspace=ws_attn, out_tiled=True)
+            return att.data_ptr(), _lib.RSPX_TILED
+
+        return self._stack(ids, slots.to(torch.int32), positions, cache.cap,
+                           lambda li: (cache.k[li], cache.v[li], cache.cap), attend, kv_only)
+
+    def _stack(self, ids, slots32, positions, reach: int, kv, attend, kv_only: bool = False) -> torch.Tensor | None:
+        """Every layer over the tokens ``ids``, whose positions lie below ``reach``.  ``kv(layer)``:
+        (K [HK, cap, D], V, cap), where a token's K/V go to slots32 of it; ``attend(layer, q
+        [T, HQ, D])``, once they are written: the attention's result as the o projection's x
+        (device pointer, row stride)."""
+        cfg = self.cfg
         L = _lib.lib()
         dev = self.device
         s = _lib.stream_ptr(dev)
         T = int(ids.shape[0])
-        if P < 0 or NN < 0 or P + NN > cache.cap:
-            raise ValueError(f"forward: prompt {P} + node segment {NN} exceeds the cache's {cache.cap} slots")
         Hd, HQ, HK, D = cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim
         bf = torch.bfloat16
         TILED = _lib.RSPX_TILED
@@ -234,25 +266,20 @@ class Decoder:
         y = torch.empty(rows * Hd, dtype=bf, device=dev)          # normalised rows [T, H], tiled
         _lib.check("rspx_rmsnorm", L.rspx_rmsnorm(x.data_ptr(), Hd, self.layers[0].in_norm.data_ptr(), y.data_ptr(),
                                                   TILED, T, Hd, cfg.eps, s))
-        cos, sin = self._rope_rows(positions, cache.cap)
-        slots32 = slots.to(torch.int32)
+        cos, sin = self._rope_rows(positions, reach)
         qo = torch.empty((T, HQ, D), dtype=bf, device=dev)
-        att = torch.empty(rows * HQ * D, dtype=bf, device=dev)   # attention output [T, HQ D], tiled
         mlp = torch.empty(rows * cfg.ffn, dtype=bf, device=dev)  # SwiGLU output [T, F], tiled when fused
-        ws_attn = self._workspace("attn", L.rspx_trie_attn_workspace_bytes(HQ, HK, T, P, D))
-        self.attn_ws_used = ws_attn   # its first word flags a wait that gave up (kernels.attention.status_word)
         for li, lay in enumerate(self.layers):
-            ck, cv = cache.k[li], cache.v[li]
+            ck, cv, cap = kv(li)
             qkvp, S = self._partials(y.data_ptr(), TILED, T, lay.tqkv)
             _lib.check("rspx_qkv_rope_cache_partials", L.rspx_qkv_rope_cache_partials(
                 qkvp, S, lay.q_norm.data_ptr(), lay.k_norm.data_ptr(), cos.data_ptr(),
-                sin.data_ptr(), cos.stride(0), slots32.data_ptr(), cache.cap, ck.data_ptr(), ck.stride(0), ck.stride(1),
+                sin.data_ptr(), cos.stride(0), slots32.data_ptr(), cap, ck.data_ptr(), ck.stride(0), ck.stride(1),
                 cv.data_ptr(), cv.stride(0), cv.stride(1), qo.data_ptr(), T, HQ, HK, D, cfg.eps, s))
             if kv_only and li + 1 == len(self.layers):
                 return None
-            trie_attn(qo.permute(1, 0, 2), ck[:, :P], cv[:, :P], ck[:, P:P + NN], cv[:, P:P + NN], msk,
-                      self.sm_scale, out=att, workspace=ws_attn, out_tiled=True)
-            hp, S = self._partials(att.data_ptr(), TILED, T, lay.tout)
+            ax, sax = attend(li, qo)
+            hp, S = self._partials(ax, sax, T, lay.tout)
             _lib.check("rspx_add_rmsnorm_partials", L.rspx_add_rmsnorm_partials(
                 x.data_ptr(), Hd, hp, S, lay.post_norm.data_ptr(), x.data_ptr(), Hd, y.data_ptr(), TILED,
                 T, Hd, cfg.eps, s))
@@ -298,6 +325,72 @@ class Decoder:
                 m = T - 1
                 last = y.view(-1, self.cfg.hidden // 32, 4, 4, 16, 8)[m // 64, :, m % 64 // 16, :, m % 16].reshape(1, -1)
         return self._linear(last.data_ptr(), last.stride(0), 1, self.t_lm_head, out_dtype=torch.float32)
+
+    # ------------------------------------------------------------------ several sequences
+    @torch.no_grad()
+    def prefill_batch(self, prompts, cache) -> tuple[list[int], torch.Tensor]:
+        """New sequences of the PagedKVCache ``cache`` holding ``prompts`` (1-D token tensors on the
+        GPU, none empty), all in one pass.  Returns (sequences, logits [B, V] of each prompt's
+        last token).  A prompt's results do not depend on the others; its attention runs in
+        ``prompt_attn``'s order, so its bits are not those of ``prefill``."""
+        self._check_paged(cache)
+        rows = [int(p.shape[0]) for p in prompts]
+        if not rows or min(rows) < 1:
+            raise ValueError("prefill_batch: prompts must be one or more, none empty")
+        cfg, dev, T = self.cfg, self.device, sum(rows)
+        plan = PackedPrompts(rows, device=dev)
+        ids = torch.cat(list(prompts))
+        positions = torch.cat([torch.arange(n, device=dev) for n in rows])
+        seqs = cache.add(rows)
+        try:
+            slots = cache.slots(seqs, 0, rows)
+            k, v = torch.empty((2, cfg.kv_heads, T, cfg.head_dim), dtype=torch.bfloat16, device=dev)
+            kt, vt = k.transpose(0, 1), v.transpose(0, 1)
+            att = torch.empty((T, cfg.heads, cfg.head_dim), dtype=torch.bfloat16, device=dev)
+
+            def attend(li, qo):
+                cache.write(li, kt, vt, slots)
+                prompt_attn(qo, kt, vt, plan, self.sm_scale, out=att)
+                return att.data_ptr(), cfg.heads * cfg.head_dim
+
+            y = self._stack(ids, torch.arange(T, dtype=torch.int32, device=dev), positions, _reach(max(rows)),
+                            lambda li: (k, v, T), attend)
+            # the last rows of the tiled rows (RSPX_TILED): elements 32 b + 8 g + e at [b, g, e]
+            m = torch.tensor(rows, device=dev).cumsum(0) - 1
+            last = y.view(-1, cfg.hidden // 32, 4, 4, 16, 8)[m // 64, :, m % 64 // 16, :, m % 16].reshape(len(rows), -1)
+            return seqs, self._linear(last.data_ptr(), last.stride(0), len(rows), self.t_lm_head, out_dtype=torch.float32)
+        except BaseException:
+            cache.free(seqs)
+            raise
+
+    @torch.no_grad()
+    def step_batch(self, ids: torch.Tensor, cache, seqs) -> torch.Tensor:
+        """One token (``ids`` [B] on the GPU) of each of the sequences ``seqs`` of the PagedKVCache
+        ``cache``, appended to them.  Returns fp32 logits [B, V].  A sequence's results do not
+        depend on the others."""
+        self._check_paged(cache)
+        seqs = list(seqs)
+        if tuple(ids.shape) != (len(seqs),) or not seqs:
+            raise ValueError("step_batch: one token per sequence, at least one")
+        cfg, B = self.cfg, len(seqs)
+        cache.extend(seqs, 1)
+        n = [cache.length(s) for s in seqs]
+        slots = cache.slots(seqs, [m - 1 for m in n], 1)
+        table, lens = cache.tables(seqs)
+        att = torch.empty((B, cfg.heads, cfg.head_dim), dtype=torch.bfloat16, device=self.device)
+
+        def attend(li, qo):
+            paged_attn(qo, cache.k[li], cache.v[li], table, lens, cache.page, self.sm_scale, out=att)
+            return att.data_ptr(), cfg.heads * cfg.head_dim
+
+        y = self._stack(ids, slots, lens - 1, _reach(max(n)), lambda li: (cache.k[li], cache.v[li], cache.pages * cache.page),
+                        attend)
+        return self._linear(y.data_ptr(), _lib.RSPX_TILED, B, self.t_lm_head, out_dtype=torch.float32)
+
+    def _check_paged(self, cache) -> None:
+        c = self.cfg
+        if (cache.layers, cache.HK, cache.D) != (c.layers, c.kv_heads, c.head_dim) or cache.k[0].device != self.embed.device:
+            raise ValueError("the cache's layers, kv heads, head_dim or GPU are not the decoder's")
 
     # ------------------------------------------------------------------ graphs
     def graphed(self, cache, P: int, T: int, NN: int) -> "GraphedForward":

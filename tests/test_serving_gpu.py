@@ -1,0 +1,123 @@
+"""Several sequences at once through the decoder: packed prefill into a paged cache, token steps
+over it, scores of the tokens, forks, rejected tokens taken back -- against the CPU reference
+decoder, and a sequence's bits against the same sequence alone."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+CFG = dict(layers=2, hidden=512, heads=4, kv_heads=2, head_dim=128, ffn=1024, vocab=4096)
+LENS = [100, 1, 37, 260]
+
+
+@pytest.fixture(scope="module")
+def model():
+    from respect_amd.decoding.engine import Decoder, DecoderConfig
+    return Decoder(DecoderConfig(**CFG), seed=1, std=0.05)
+
+
+def _cache(pages=64, page=16, **kw):
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    return PagedKVCache(CFG["layers"], CFG["kv_heads"], CFG["head_dim"], pages, page=page, **kw)
+
+
+def _prompts(lens=LENS, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, CFG["vocab"], (n,), generator=g).cuda() for n in lens]
+
+
+def test_against_the_reference_decoder(model):
+    """Prefill and two greedy steps: logits within the bound of the decoder's other forwards, the
+    scores of the chosen tokens those of the logits."""
+    from oracle.decoder import RefDecoder
+    from respect_amd.decoding.acceptance import greedy_token
+    from respect_amd.decoding.logprobs import token_logprobs
+    ref, cache, prompts = RefDecoder(model), _cache(), _prompts()
+    seqs, logits = model.prefill_batch(prompts, cache)
+    kv, got = [None] * len(seqs), [p.tolist() for p in prompts]
+    new = [list(p) for p in got]
+    for step in range(3):
+        print(f"[serving] step {step}", flush=True)
+        for i, s in enumerate(seqs):
+            n, a = len(got[i]), len(got[i]) - len(new[i])
+            allow = torch.tril(torch.ones(n, 300, dtype=torch.bool))[a:]
+            want, kv[i] = ref.forward(new[i], list(range(a, n)), list(range(a, n)), allow, kv[i])
+            assert (logits[i].cpu() - want[-1]).abs().max() <= 0.05 * want.abs().max()
+        choice = greedy_token(logits)
+        given, entropy, values, ids = token_logprobs(logits, choice, top=3)
+        lp = torch.log_softmax(logits.double(), -1)
+        assert torch.equal(ids[:, 0], choice) and torch.equal(values[:, 0], given)
+        assert torch.allclose(given.double(), lp.gather(1, choice[:, None])[:, 0], rtol=0, atol=1e-5)
+        assert torch.allclose(entropy.double(), -(lp.exp() * lp).sum(-1), rtol=0, atol=1e-4)
+        new = [[t] for t in choice.tolist()]
+        for i, t in enumerate(new):
+            got[i] += t
+        logits = model.step_batch(choice, cache, seqs)
+    assert [cache.length(s) for s in seqs] == [n + 3 for n in LENS]
+
+
+def test_a_sequence_does_not_depend_on_the_batch(model):
+    cache, prompts = _cache(), _prompts()
+    seqs, logits = model.prefill_batch(prompts, cache)
+    tokens = torch.tensor([5, 6, 7, 8], device="cuda")
+    after = model.step_batch(tokens, cache, seqs)
+    for i in (0, 1, 3):
+        other = _cache(page=64, pages=8)
+        (s,), one = model.prefill_batch(prompts[i:i + 1], other)
+        assert torch.equal(one[0], logits[i])
+        assert torch.equal(model.step_batch(tokens[i:i + 1], other, [s])[0], after[i])
+        n = LENS[i] + 1
+        a, b = cache.slots([seqs[i]], 0, n).long(), other.slots([s], 0, n).long()
+        for x, y in zip(cache.k + cache.v, other.k + other.v):
+            assert torch.equal(x[:, a], y[:, b])
+
+
+def test_forks_rejected_tokens_and_pages(model):
+    """Forks continue as their origin would, each on its own; tokens taken back leave no trace; a
+    full cache refuses and keeps what it holds; in the end every page is free."""
+    cache, prompts = _cache(pages=80), _prompts()
+    seqs, _ = model.prefill_batch(prompts, cache)
+    tok = lambda *t: torch.tensor(t, device="cuda")
+    forks = cache.fork(seqs[:2], 2)
+    a = model.step_batch(tok(1, 2, 3, 4, 5, 6), cache, forks + [seqs[0], seqs[1]])
+    b = model.step_batch(tok(1, 2, 3, 4), cache, [seqs[2]] + cache.fork([seqs[3]]) + forks[:2])
+    assert not torch.equal(a[0], a[1])
+    # the same from fresh caches
+    c2 = _cache()
+    s2, _ = model.prefill_batch(prompts, c2)
+    assert torch.equal(model.step_batch(tok(1, 3), c2, s2[:2]), a[[0, 2]])
+    assert torch.equal(model.step_batch(tok(3), c2, s2[:1])[0], b[2])
+    # three tokens fed, the first kept, then another way on
+    n = cache.length(seqs[2])
+    for t in (11, 12, 13):
+        model.step_batch(tok(t), cache, [seqs[2]])
+    cache.compact([seqs[2]], n, [[0]])
+    x = model.step_batch(tok(14), cache, [seqs[2]])
+    model.step_batch(tok(1), c2, s2[2:3])
+    model.step_batch(tok(11), c2, s2[2:3])
+    assert torch.equal(model.step_batch(tok(14), c2, s2[2:3]), x)
+    free = cache.free_pages
+    with pytest.raises(RuntimeError):
+        model.prefill_batch(_prompts([free * 16 + 1]), cache)
+    assert cache.free_pages == free
+    cache.free(range(9))
+    assert cache.free_pages == 80
+
+
+def test_refusals(model):
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    cache = _cache()
+    seqs, _ = model.prefill_batch(_prompts([3]), cache)
+    with pytest.raises(ValueError):
+        model.prefill_batch([], cache)
+    with pytest.raises(ValueError):
+        model.prefill_batch(_prompts([3, 0]), cache)
+    with pytest.raises(ValueError):
+        model.prefill_batch(_prompts([3]), PagedKVCache(1, 2, 128, 8))
+    with pytest.raises(ValueError):
+        model.step_batch(torch.tensor([1, 2], device="cuda"), cache, seqs)
+    with pytest.raises(ValueError):
+        model.step_batch(torch.tensor([1], device="cuda"), cache, [seqs[0] + 1])
+    with pytest.raises(ValueError):
+        model.step_batch(torch.tensor([1, 2], device="cuda"), cache, seqs * 2)
+    assert cache.length(seqs[0]) == 3
