@@ -30,8 +30,9 @@ def _cache(lens, page, HK, D, seed=0, spare=3, width=None):
 
 
 def _exact(q, rows, scale=None):
-    """(result, bound) in float64.  p enters the product as two bf16 terms (2^-16 of it is lost
-    at most); sums and scores as in fp32, the result rounded to bf16 once."""
+    """(result, bound) in float64.  p enters the product as two bf16 terms: cut to 8 bits, which
+    leaves a rest below 2^-7 p, and that rest rounded, off by half a step, 2^-8 of it at most:
+    2^-15 p.  Sums and scores as in fp32, the result rounded to bf16 once."""
     B, H, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     out, bound = torch.zeros(B, H, D, dtype=torch.float64), torch.zeros(B, H, D, dtype=torch.float64)
@@ -43,7 +44,7 @@ def _exact(q, rows, scale=None):
             o, a = p @ vd, p @ vd.abs()
             es = 2.0 ** -24 * ((D + 8) * float((kd.abs() @ qd.abs()).max()) * scale + 8)
             out[b, h] = o
-            bound[b, h] = (a * (2.0 ** -16 + 2 * es + 2 * (n + 64) * 2.0 ** -24) + o.abs() * 2.0 ** -8) * 1.02
+            bound[b, h] = (a * (2.0 ** -15 + 2 * es + 2 * (n + 64) * 2.0 ** -24) + o.abs() * 2.0 ** -8) * 1.02
     return out, bound
 
 
