@@ -10,10 +10,12 @@
 // status of the C ABI comes back as an int.  Nothing is kept between calls.
 #include <Python.h>
 
+#include <algorithm>
 #include <cmath>
 #include <vector>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -382,10 +384,119 @@ PyObject* trie_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool integer(PyObject* o, int64_t& v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  v = PyLong_AsLongLongAndOverflow(o, &overflow);
+  return overflow == 0;
+}
+
+// None or a number: the softmax scale, D ** -0.5 by default.
+bool softmax_scale(PyObject* o, int64_t D, double& v) {
+  if (o != Py_None) return number(o, v);
+  v = std::pow((double)D, -0.5);
+  return true;
+}
+
+// prompt_attn(q, k, v, Tq, Tk, tiles32, tiles64, tiles128, sm_scale)
+PyObject* prompt_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9) NOT_TAKEN;
+  const Tensor *q = input(a[0]), *k = input(a[1]), *v = input(a[2]);
+  if (!q || !k || !v || q->dim() != 3 || k->dim() != 3 || k->sizes() != v->sizes() || k->size(2) != q->size(2) ||
+      k->device() != q->device() || v->device() != q->device())
+    NOT_TAKEN;
+  const int64_t T = q->size(0), H = q->size(1), D = q->size(2), Tk = k->size(0), HK = k->size(1);
+  int64_t tq, tk;
+  double scale;
+  if (!integer(a[3], tq) || !integer(a[4], tk) || tq != T || tk != Tk || !softmax_scale(a[8], D, scale)) NOT_TAKEN;
+  for (int64_t x : {T, H, D, Tk, HK})
+    if (!fits_int(x)) NOT_TAKEN;
+  const int rows = rspx_prompt_attn_tile_rows((int)H, (int)HK);
+  if (rows < 0) NOT_TAKEN;
+  const Tensor* t = plain(a[rows == 32 ? 5 : rows == 64 ? 6 : 7], at::kInt);
+  if (!t || t->dim() != 2 || t->size(1) != 4 || !t->is_contiguous() || !fits_int(t->size(0)) || t->device() != q->device())
+    NOT_TAKEN;
+  const c10::DeviceGuard guard(q->device());
+  Tensor y = empty_like_of(*q, {T, H, D});
+  const int rc = call([&] {
+    return rspx_prompt_attn(ptr(*q), q->stride(0), q->stride(1), ptr(*k), k->stride(0), k->stride(1), ptr(*v),
+                            v->stride(0), v->stride(1), t->const_data_ptr<int>(), (int)t->size(0), y.data_ptr(), H * D, D,
+                            (int)H, (int)HK, (int)T, (int)Tk, (int)D, (float)scale, stream_of(*q));
+  });
+  STATUS(rc);
+  return wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attn(q, kc, vc, table, lens, page, sm_scale)
+PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) NOT_TAKEN;
+  const Tensor *q = input(a[0]), *k = input(a[1]), *v = input(a[2]), *t = plain(a[3], at::kInt), *l = plain(a[4], at::kInt);
+  if (!q || !k || !v || !t || !l || q->dim() != 3 || k->dim() != 3 || k->sizes() != v->sizes() || k->size(2) != q->size(2) ||
+      t->dim() != 2 || l->dim() != 1 || !l->is_contiguous())
+    NOT_TAKEN;
+  for (const Tensor* x : {k, v, t, l})
+    if (x->device() != q->device()) NOT_TAKEN;
+  const int64_t B = q->size(0), H = q->size(1), D = q->size(2), HK = k->size(0), slots = k->size(1), width = t->size(1);
+  int64_t page;
+  double scale;
+  if (!integer(a[5], page) || page < 1 || slots % page || t->size(0) != B || l->size(0) != B ||
+      (width > 1 && t->stride(1) != 1) || !softmax_scale(a[6], D, scale))
+    NOT_TAKEN;
+  for (int64_t x : {B, H, D, HK, slots, width, page})
+    if (!fits_int(x)) NOT_TAKEN;
+  const int64_t need = std::max<int64_t>(0, rspx_paged_attn_workspace_bytes((int)B, (int)H, (int)D, (int)page, (int)width));
+  const c10::DeviceGuard guard(q->device());
+  Tensor y = empty_like_of(*q, {B, H, D}), ws;
+  if (need) ws = empty_like_of(*q, {need}, at::kByte);
+  const int rc = call([&] {
+    return rspx_paged_attn(ptr(*q), q->stride(0), q->stride(1), ptr(*k), k->stride(0), k->stride(1), ptr(*v), v->stride(0),
+                           v->stride(1), t->const_data_ptr<int>(), t->stride(0), l->const_data_ptr<int>(), y.data_ptr(),
+                           H * D, D, (int)B, (int)H, (int)HK, (int)D, (int)(slots / page), (int)page, (int)width,
+                           (float)scale, need ? ws.data_ptr() : nullptr, need, stream_of(*q));
+  });
+  STATUS(rc);
+  return wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs(logits, tokens, top, offset, size)
+PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) NOT_TAKEN;
+  const Tensor *x = plain(a[0], at::kFloat), *t = plain(a[1], at::kLong);
+  int64_t top, off, size;
+  if (!x || !t || x->dim() != 2 || x->stride(1) != 1 || t->dim() != 1 || !t->is_contiguous() || t->size(0) != x->size(0) ||
+      t->device() != x->device() || !integer(a[2], top) || !integer(a[3], off) || !integer(a[4], size))
+    NOT_TAKEN;
+  const int64_t M = x->size(0), V = x->size(1), s = x->stride(0);
+  if (top < 0 || V < 1 || s < V || s % 4 || reinterpret_cast<uintptr_t>(x->const_data_ptr()) % 16 || !fits_int(M) || !fits_int(V) ||
+      !fits_int(off) || !fits_int(size))
+    NOT_TAKEN;
+  const int k = (int)std::min(top, V);
+  const int64_t need = rspx_token_logprobs_workspace_bytes((int)M, (int)V, k);
+  if (need < 0) NOT_TAKEN;
+  const c10::DeviceGuard guard(x->device());
+  Tensor given = empty_like_of(*x, {M}, at::kFloat), entropy = empty_like_of(*x, {M}, at::kFloat);
+  Tensor values = empty_like_of(*x, {M, k}, at::kFloat), ids = empty_like_of(*x, {M, k}, at::kLong);
+  Tensor ws = empty_like_of(*x, {need}, at::kByte);
+  const int rc = call([&] {
+    return rspx_token_logprobs(x->const_data_ptr<float>(), s, (int)M, (int)V, (int)off, (int)size, t->const_data_ptr<int64_t>(),
+                               k, given.data_ptr<float>(), entropy.data_ptr<float>(), values.data_ptr<float>(),
+                               ids.data_ptr<int64_t>(), ws.data_ptr(), need, stream_of(*x));
+  });
+  STATUS(rc);
+  return Py_BuildValue("(NNNN)", wrap(std::move(given)), wrap(std::move(entropy)), wrap(std::move(values)), wrap(std::move(ids)));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(silu_mul), FAST(rmsnorm), FAST(qk_norm_rope), FAST(rmsnorm_qk_norm_rope),
                          FAST(rope),     FAST(add_sq),  FAST(norm_apply),   FAST(rope_vision),
-                         FAST(linear),   FAST(trie_attn), {nullptr, nullptr, 0, nullptr}};
+                         FAST(linear),   FAST(trie_attn), FAST(prompt_attn), FAST(paged_attn),
+                         FAST(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -17,6 +17,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
     Columns [offset, offset + size) count as -inf, as for ``greedy_token``.  A token outside
     the vocabulary gets NaN; a row with NaN or +inf scores has NaN results, NaN first among
     the ids; a row with nothing left has -inf and entropy 0.  ``top`` <= 64."""
+    y = _lib.calls().token_logprobs(logits, tokens, top, offset, size)
+    if y is not None:
+        return _lib.result("rspx_token_logprobs", y)
     if logits.dtype != torch.float32 or not logits.is_cuda or logits.dim() != 2 or logits.stride(1) != 1:
         raise TypeError("token_logprobs: fp32 [M, V] GPU logits with contiguous rows are required")
     M, V = logits.shape

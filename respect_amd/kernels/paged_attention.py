@@ -20,6 +20,10 @@ def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None):
     All on one GPU; table and lens are read there, so that a captured call follows them.
     A sequence of length 0 gets zeros; one whose length is negative or beyond its table, or
     that reads a page outside the pool, gets NaN.  ``page``: a power of two."""
+    if out is None:
+        y = _lib.calls().paged_attn(q, kc, vc, table, lens, page, sm_scale)
+        if y is not None:
+            return _lib.result("rspx_paged_attn", y)
     if q.dim() != 3 or kc.dim() != 3 or kc.shape != vc.shape or kc.shape[2] != q.shape[2]:
         raise ValueError("paged_attn: q must be [B, H, D], kc and vc [HK, slots, D]")
     B, H, D = q.shape

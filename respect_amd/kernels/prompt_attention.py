@@ -44,17 +44,21 @@ class PackedPrompts:
             # The longest first: the device is then busy to the end.
             parts.append(t[np.argsort(-(t[:, 1] + t[:, 3]), kind="stable")].astype(np.int32))
         flat = torch.from_numpy(np.concatenate(parts)).to(self.device)
-        self._tiles = dict(zip(TILE_ROWS, flat.split([len(t) for t in parts])))
+        self._lists = flat.split([len(t) for t in parts])
 
     def tiles(self, H: int, HK: int) -> torch.Tensor:
         """Device int32 [n, 4]: the tiles rspx_prompt_attn takes for these heads."""
-        return self._tiles[_lib.lib().rspx_prompt_attn_tile_rows(H, HK)]
+        return self._lists[TILE_ROWS.index(_lib.lib().rspx_prompt_attn_tile_rows(H, HK))]
 
 
 def prompt_attn(q, k, v, plan: PackedPrompts, sm_scale=None, out=None):
     """q [Tq, H, D], k / v [Tk, HK, D] bf16, packed as ``plan`` says -> [Tq, H, D] bf16.
     ``sm_scale``: default D ** -0.5.  ``out``: written in place if given (any strides with
     D contiguous, multiples of 8 elements)."""
+    if out is None and isinstance(plan, PackedPrompts):
+        y = _lib.calls().prompt_attn(q, k, v, plan.Tq, plan.Tk, *plan._lists, sm_scale)
+        if y is not None:
+            return _lib.result("rspx_prompt_attn", y)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
         raise ValueError("prompt_attn: q must be [Tq, H, D], k and v [Tk, HK, D]")
     T, H, D = q.shape

@@ -63,8 +63,8 @@ def test_plan_tiles_cover_every_row_once():
     rows, keys = [0, 5, 64, 1, 131, 300], [7, 5, 10, 1, 200, 300]
     plan = PackedPrompts(rows, keys, device="cpu")
     assert (plan.Tq, plan.Tk, plan.rows, plan.keys) == (sum(rows), sum(keys), rows, keys)
-    for size in TILE_ROWS:
-        t = plan._tiles[size].numpy().astype(np.int64)
+    for size, tiles in zip(TILE_ROWS, plan._lists):
+        t = tiles.numpy().astype(np.int64)
         sees = np.full(plan.Tq, -10 ** 9)
         first = np.full(plan.Tq, -1)
         for q0, n, k0, seen in t:

@@ -1,0 +1,77 @@
+"""The native form of the serving operators' common case (respect_amd/_calls): what it leaves to
+the Python wrappers, and that both give the same results."""
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+def test_calls_leaves_what_it_does_not_take():
+    from respect_amd import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    c = _lib.calls()
+    x, i = torch.zeros(4, 2, 64, dtype=BF), torch.zeros(1, 4, dtype=torch.int32)
+    assert c.prompt_attn(x, x, x, 4, 4, i, i, i, None) is None and c.prompt_attn(x) is None
+    assert c.paged_attn(x, x, x, i, i[0], 16, None) is None and c.paged_attn() is None
+    f = torch.zeros(2, 8)
+    assert c.token_logprobs(f, torch.zeros(2, dtype=torch.int64), 1, 0, 0) is None
+    assert c.token_logprobs(f, f, 1.5, None, "a") is None
+
+
+@pytest.mark.gpu
+def test_calls_equal_the_wrappers_own_path(monkeypatch):
+    from respect_amd import _lib
+    from respect_amd.decoding.logprobs import token_logprobs
+    from respect_amd.kernels.paged_attention import paged_attn
+    from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
+
+    class Leave:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+
+    def r(*s, dtype=BF):
+        return torch.randn(*s, generator=g, device="cuda").to(dtype)
+
+    q, k, v, plan = r(70, 8, 64), r(90, 2, 64), r(90, 2, 64), PackedPrompts([60, 10], [60, 30])
+    kc = r(2, 640, 64)
+    table = torch.randperm(40, generator=g, device="cuda").to(torch.int32).view(2, 20)
+    lens = torch.tensor([311, 7], dtype=torch.int32, device="cuda")
+    x, t = r(3, 5000, dtype=torch.float32), torch.tensor([1, 2, 3], device="cuda")
+    wide = r(4, 70, 8, 64)
+    calls = [
+        (True, lambda: prompt_attn(q, k, v, plan)),
+        (True, lambda: prompt_attn(wide[2], k, v, plan, sm_scale=0.3)),
+        (False, lambda: prompt_attn(r(70, 8, 72)[:, :, 3:67], k, v, plan)),
+        (True, lambda: paged_attn(q[:2], kc, kc, table, lens, 16)),
+        (True, lambda: paged_attn(q[:2], kc, kc, table, lens, 16, sm_scale=1)),
+        (False, lambda: paged_attn(q[:2], kc, kc, table.t().contiguous().t(), lens, 16)),
+        (True, lambda: token_logprobs(x, t)),
+        (True, lambda: token_logprobs(x, t, top=9, offset=3, size=40)),
+        (False, lambda: token_logprobs(x[:, 1:], t, top=9)),
+    ]
+    native = _lib.calls()
+    for taken, call in calls:
+        got = []
+
+        class Watch:
+            def __getattr__(self, name):
+                def f(*a):
+                    y = getattr(native, name)(*a)
+                    got.append(y is not None)
+                    return y
+                return f
+        state = g.get_state()
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "_calls", Watch())
+            a = call()
+        assert got == [taken]
+        g.set_state(state)
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "_calls", Leave())
+            b = call()
+        for y, z in zip(*(((a,), (b,)) if isinstance(a, torch.Tensor) else (a, b))):
+            assert y.shape == z.shape and y.dtype == z.dtype and torch.equal(y, z)
