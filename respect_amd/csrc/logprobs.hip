@@ -4,15 +4,17 @@
 //   p_j = exp(x_j - lse),  lse = m + log z,  z = sum_j exp(x_j - m),  m = max_j x_j
 //   given = x_t - lse,  entropy = -sum_j p_j log p_j = log z - sum_j e_j (x_j - m) / z
 //
-// over the columns outside an excluded range.  One read of the scores: a workgroup takes a
-// chunk of kChunk columns of one row into registers, leaves the chunk's (m, z, u = sum e (x - m))
-// and its best `top` (value, index) pairs, and a second launch joins a row's chunks in
-// order, in 64 bits.  A row's result depends on its own scores and on V alone.
+// over the columns outside an excluded range.  One read of the scores: a wave takes 1024
+// columns of one row at a time into registers and leaves (m, z, u = sum e (x - m)) of each
+// such step; a second launch joins a row's steps in 64 bits, in an order that V alone sets.
+// How many steps a workgroup takes depends on the number of rows, no result does.
 //
 // The best pairs are a set under a total order (value, lowest index first, NaN the
-// largest), so their selection may take any order: the top-th best of 64 groups' maxima is a
-// lower bound of the top-th best element, what passes it (at most 64 per group that does, in
-// practice a few more than `top`) is gathered and ranked by counting.
+// largest), so their selection may take any order.  Each wave keeps a list of candidates in
+// LDS and the bound that a pair must pass to enter it, the top-th best found so far: most
+// steps add few or none.  Where a step would add too many (the first one, rising scores, ties) the
+// top-th best of the lanes' best pairs bounds them first: at most 16 of each of `top` lanes pass.
+// Lists are cut to their best by counting.
 //
 // What bounds it: the read of the scores.
 #include "common.h"
@@ -23,20 +25,12 @@ namespace rspx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;                       // elements per thread
-constexpr int kChunk = kThreads * kPer;        // columns of a workgroup
+constexpr int kPer = 16;                       // elements per lane
+constexpr int kSub = 64 * kPer;                // columns of a wave's step: the unit of the sums
+constexpr int kChunk = 4 * kSub;               // columns of a workgroup's step
 constexpr int kMaxTop = 64;
 constexpr int kGroups = 64;                    // groups of four threads
-
-// exp(x) for x <= 0 (or NaN): x log2(e) in two pieces, so that the product's rounding does
-// not grow with |x|.
-__device__ __forceinline__ float exp_neg(float x) {
-  constexpr float kL = 1.44269504088896340736f, kLlo = 1.92596299e-8f, kLn2 = 0.69314718055994530942f;
-  const float h = x * kL;
-  const float l = __builtin_fmaf(x, kLlo, __builtin_fmaf(x, kL, -h));
-  const float e = fexp2(h);
-  return x < -100.f ? e : __builtin_fmaf(e, l * kLn2, e);   // -inf: no inf - inf in l
-}
+constexpr float kL2E = 1.44269504088896340736f;
 
 // The order of the pairs as one unsigned number: larger is better.
 __device__ __forceinline__ uint64_t pair_key(float v, int j) {
@@ -80,6 +74,7 @@ __device__ __forceinline__ void select_top(const uint64_t (&key)[kPer], int top,
   if (threadIdx.x < kGroups) {
     const uint64_t mine = S.group[threadIdx.x];
     int r = 0;
+#pragma unroll 16
     for (int i = 0; i < kGroups; ++i) r += S.group[i] > mine;
     if (r == top - 1 && mine != 0) S.bound = mine;         // keys differ: one thread at most
   }
@@ -93,6 +88,7 @@ __device__ __forceinline__ void select_top(const uint64_t (&key)[kPer], int top,
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = S.cand[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) r += S.cand[j] > mine;
     if (r < top) out(r, mine);
   }
@@ -105,138 +101,278 @@ struct LogArgs {
   const int64_t* tokens;
   float *given, *entropy, *values;
   int64_t* ids;
-  float* stat;                 // [rows][chunks][3]: m, z, u
-  uint64_t* best;              // [rows][chunks][top]
+  float* stat;                 // [rows][4 chunks][3]: m, z, u of each kSub columns
+  uint64_t* best;              // [rows][parts][top]
   int64_t sx;
-  int V, chunks, off, end, top, row0;
+  int V, chunks, parts, off, end, top, row0;   // parts: workgroups of a row
 };
 
-__device__ __forceinline__ bool excluded(const LogArgs& A, int j) { return j >= A.off && j < A.end; }
+// Entries a wave's list has room for: its best, the at most kPer of each of `top` lanes that a
+// tightened bound lets through, and a copy of the best.
+__host__ __device__ __forceinline__ int list_room(int top) { return (kPer + 2) * top; }
 
-__device__ __forceinline__ float block_max(float v, float* s) {
-  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+// The wave's list of n <= (kPer + 1) top pairs cut to its `top` best, best first; returns the
+// last one, the bound of what may still enter (0: fewer than `top`).  The LDS operations of
+// a wave keep their order.
+__device__ __forceinline__ uint64_t prune(uint64_t* list, int& n, int top) {
+  const int lane = __lane_id();
+  uint64_t* best = list + (kPer + 1) * top;
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t mine = list[i];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) r += list[j] > mine;
+    if (r < top) best[r] = mine;
+  }
+  __builtin_amdgcn_wave_barrier();
+  n = min(n, top);
+  if (lane < n) list[lane] = best[lane];
+  __builtin_amdgcn_wave_barrier();
+  return n < top ? 0 : best[top - 1];
 }
 
-template <bool TOP>
-__global__ __launch_bounds__(kThreads) void logprobs_chunk_kernel(LogArgs A) {
-  __shared__ float sm[4], sz[4], su[4];
-  __shared__ Select S;
-  const int c = blockIdx.x;
-  const int64_t row = (int64_t)A.row0 + blockIdx.y;
-  const float* xr = A.x + row * A.sx;
-  float x[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer / 4; ++i) {
-    const int j = c * kChunk + 4 * (threadIdx.x + kThreads * i);
-    f32x4 v = {kNegInf, kNegInf, kNegInf, kNegInf};
-    if (j + 3 < A.V) v = *reinterpret_cast<const f32x4*>(xr + j);
-    else
-      for (int e = 0; e < 4; ++e)
-        if (j + e < A.V) v[e] = xr[j + e];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[4 * i + e] = excluded(A, j + e) ? kNegInf : v[e];
-  }
-  float m = x[0];
-#pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
-  m = block_max(m, sm);
-  float z = 0.f, u = 0.f;
+// Adds the wave's step x (columns j0 + 256 (i / 4) + i % 4, j0 the lane's own) to its list.
+__device__ __forceinline__ void enlist(const float (&x)[kPer], int j0, int V, int top, uint64_t* list, int& n,
+                                       uint64_t& bound) {
+  uint64_t key[kPer];
+  int count = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const float d = m == kNegInf ? x[i] : x[i] - m;        // a chunk of -inf adds nothing
-    const float e = exp_neg(d);
-    z = z + e;
-    u = u + (d == kNegInf ? 0.f : e * d);
+    const int j = j0 + 256 * (i / 4) + i % 4;
+    key[i] = j < V ? pair_key(x[i], j) : 0;
+    count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] > bound));
   }
-  for (int k = 32; k >= 1; k >>= 1) {
-    z = z + __shfl_xor(z, k);
-    u = u + __shfl_xor(u, k);
-  }
-  if ((threadIdx.x & 63) == 0) {
-    sz[threadIdx.x >> 6] = z;
-    su[threadIdx.x >> 6] = u;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float* st = A.stat + (row * A.chunks + c) * 3;
-    st[0] = m;
-    st[1] = (sz[0] + sz[1]) + (sz[2] + sz[3]);
-    st[2] = (su[0] + su[1]) + (su[2] + su[3]);
-  }
-  if constexpr (TOP) {
-    uint64_t key[kPer];
+  if (n + count > 3 * top) {   // many: the top-th best of the lanes' best bounds them
+    if (n > top) bound = prune(list, n, top);
+    uint64_t best = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int j = c * kChunk + 4 * (threadIdx.x + kThreads * (i / 4)) + i % 4;
-      key[i] = j < A.V ? pair_key(x[i], j) : 0;
+    for (int i = 0; i < kPer; ++i) best = key[i] > best ? key[i] : best;
+    int r = 0;
+#pragma unroll 16
+    for (int l = 0; l < 64; ++l) {
+      const uint64_t o = (uint64_t)__builtin_amdgcn_readlane((int)(best >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)best, l);
+      r += o > best;
     }
-    uint64_t* b = A.best + (row * A.chunks + c) * A.top;
-    select_top(key, A.top, S, [&](int r, uint64_t k) { b[r] = k; });
+    const uint64_t at = __builtin_amdgcn_ballot_w64(r == top - 1 && best != 0);   // keys differ: one lane at most
+    if (at) {
+      const int l = __builtin_ctzll(at);
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(best >> 32), l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)best, l);
+      if (o - 1 > bound) bound = o - 1;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint64_t in = __builtin_amdgcn_ballot_w64(key[i] > bound);
+    if (in) {
+      if (key[i] > bound)
+        list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = key[i];
+      n += __builtin_popcountll(in);
+    }
+  }
+  if (n > 2 * top || bound == 0) {
+    const uint64_t last = prune(list, n, top);
+    if (last > bound) bound = last;
   }
 }
 
-// One workgroup per row.
+// Workgroup (part, row): the part's chunks in order, wave w the w-th quarter of each.
+template <bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogArgs A) {
+  extern __shared__ __align__(16) uint64_t lists[];        // [4][list_room(top)]
+  __shared__ int counts[4];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)A.row0 + blockIdx.y;
+  const float* xr = A.x + row * A.sx;
+  const int c0 = (int)((int64_t)blockIdx.x * A.chunks / A.parts), c1 = (int)((int64_t)(blockIdx.x + 1) * A.chunks / A.parts);
+  uint64_t* list = lists + w * list_room(A.top);
+  int n = 0;
+  uint64_t bound = 0;
+  float least = kNegInf;                                   // the bound's value
+  f32x4 next[kPer / 4];
+  auto load = [&](int c) {
+    const int j0 = c * kChunk + w * kSub + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < kPer / 4; ++i) {
+      const int j = j0 + 256 * i;
+      f32x4 v = {kNegInf, kNegInf, kNegInf, kNegInf};
+      if (j + 3 < A.V) v = *reinterpret_cast<const f32x4*>(xr + j);
+      else
+        for (int e = 0; e < 4; ++e)
+          if (j + e < A.V) v[e] = xr[j + e];
+      next[i] = v;
+    }
+  };
+  load(c0);
+  for (int c = c0; c < c1; ++c) {
+    const int s0 = c * kChunk + w * kSub, j0 = s0 + 4 * lane;
+    float x[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = next[i / 4][i % 4];
+    if (c + 1 < c1) load(c + 1);
+    if (s0 < A.end && s0 + kSub > A.off) {                 // excluded columns among them
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int j = j0 + 256 * (i / 4) + i % 4;
+        if (j >= A.off && j < A.end) x[i] = kNegInf;
+      }
+    }
+    float mine = x[0];
+    bool nan = x[0] != x[0];
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) {
+      mine = fmaxf(mine, x[i]);
+      nan |= x[i] != x[i];
+    }
+    nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    float m = mine;
+    for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    // e^d by 2^(d log2 e).  A -inf counts as e^-200 = 0, so that it adds no inf * 0; a step
+    // of -inf only (m itself) adds nothing.
+    float z = 0.f, u = 0.f;
+    const float from = m == kNegInf ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float d = fmaxf(x[i] - from, -200.f);
+      const float e = fexp2(d * kL2E);
+      z = z + e;
+      u = __builtin_fmaf(e, d, u);
+    }
+    for (int k = 32; k >= 1; k >>= 1) {
+      z = z + __shfl_xor(z, k);
+      u = u + __shfl_xor(u, k);
+    }
+    if (lane < 3) {
+      const bool odd = nan || m == __builtin_huge_valf();  // NaN, or inf - inf
+      const float v = lane == 0 ? m : lane == 1 ? z : u;
+      A.stat[((row * A.chunks + c) * 4 + w) * 3 + lane] = odd && lane > 0 ? __builtin_nanf("") : v;
+    }
+    if constexpr (TOP) {
+      if (__builtin_amdgcn_ballot_w64(mine >= least) != 0 || nan) {
+        enlist(x, j0, A.V, A.top, list, n, bound);
+        least = bound == 0 ? kNegInf : key_value(bound);
+      }
+    }
+  }
+  if constexpr (TOP) {
+    if (n > A.top) prune(list, n, A.top);
+    if (lane == 0) counts[w] = n;
+    __syncthreads();
+    // The best of the four waves' lists, ranked by counting.
+    uint64_t* out = A.best + (row * A.parts + blockIdx.x) * A.top;
+    int all = 0;
+    for (int k = 0; k < 4; ++k) all += counts[k];
+    for (int i = threadIdx.x; i < 4 * A.top; i += kThreads) {
+      const int from = i / A.top, at = i % A.top;
+      if (at < counts[from]) {
+        const uint64_t key = lists[from * list_room(A.top) + at];
+        int r = 0;
+        for (int k = 0; k < 4; ++k)
+#pragma unroll 8
+          for (int j = 0; j < counts[k]; ++j) r += lists[k * list_room(A.top) + j] > key;
+        if (r < A.top) out[r] = key;
+      }
+    }
+    for (int i = all + threadIdx.x; i < A.top; i += kThreads) out[i] = 0;
+  }
+}
+
+// One workgroup per row: the sums of its steps in 64 bits, each thread every 256th and the
+// threads in a fixed tree, and the best of its parts' lists.
 template <bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogArgs A) {
-  __shared__ double slz;
-  __shared__ float smax;
+  __shared__ float sm[4];
+  __shared__ double sz[4], su[4];
   __shared__ Select S;
   __shared__ uint64_t kept[kMaxTop];
   const int64_t row = (int64_t)A.row0 + blockIdx.x;
+  const float* st = A.stat + row * A.chunks * 12;
+  const int steps = 4 * A.chunks, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint64_t* b = A.best + row * A.parts * A.top;
+  const int n = TOP ? A.parts * A.top : 0;
+  const uint64_t own = n <= kThreads && (int)threadIdx.x < n ? b[threadIdx.x] : 0;
+  const int64_t t = A.tokens[row];
+  const bool there = t >= 0 && t < A.V;
+  const float xt = there && !(t >= A.off && t < A.end) ? A.x[row * A.sx + t] : kNegInf;
+
+  float m = kNegInf;
+  for (int i = threadIdx.x; i < steps; i += kThreads) m = fmaxf(m, st[3 * i]);
+  for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+  if (lane == 0) sm[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  double z = 0, u = 0;
+  for (int i = threadIdx.x; i < steps; i += kThreads) {
+    const float mi = st[3 * i], zi = st[3 * i + 1], ui = st[3 * i + 2];
+    if (zi != zi) z = zi;                                  // and stays
+    if (mi == kNegInf) continue;                           // nothing in it
+    const double d = (double)mi - (double)m, a = exp(d);
+    z += a * zi;
+    u += a * (ui + d * zi);
+  }
+  for (int k = 32; k >= 1; k >>= 1) {
+    z += __shfl_xor(z, k);
+    u += __shfl_xor(u, k);
+  }
+  if (lane == 0) {
+    sz[w] = z;
+    su[w] = u;
+  }
+  __syncthreads();
+  z = (sz[0] + sz[1]) + (sz[2] + sz[3]);
+  u = (su[0] + su[1]) + (su[2] + su[3]);
+  // log p = (x - m) - log z: m + log z is never formed, scores of 1e38 would swallow log z.
+  const double lz = log(z);
+  auto logp = [&](float v) { return v == kNegInf && z == z ? kNegInf : (float)(((double)v - (double)m) - lz); };
   if (threadIdx.x == 0) {
-    const float* st = A.stat + row * A.chunks * 3;
-    float m = kNegInf;
-    for (int c = 0; c < A.chunks; ++c) m = fmaxf(m, st[3 * c]);
-    double z = 0, u = 0;
-    for (int c = 0; c < A.chunks; ++c) {
-      const double d = (double)st[3 * c] - (double)m;
-      if (st[3 * c] == kNegInf && !(st[3 * c + 1] != st[3 * c + 1])) continue;   // nothing in it, no NaN either
-      const double a = exp(d);
-      z += a * st[3 * c + 1];
-      u += a * (st[3 * c + 2] + d * st[3 * c + 1]);
-    }
-    const double lz = log(z);
     // A row with nothing left: every probability is 0, and so is the entropy.
     A.entropy[row] = m == kNegInf && z == 0 ? 0.f : (float)(lz - u / z);
-    const int64_t t = A.tokens[row];
-    float given = __builtin_nanf("");                      // no such token
-    if (t >= 0 && t < A.V) {
-      const float x = excluded(A, (int)t) ? kNegInf : A.x[row * A.sx + t];
-      given = x == kNegInf && z == z ? kNegInf : (float)(((double)x - (double)m) - lz);
-    }
-    A.given[row] = given;
-    slz = lz;   // lse = m + lz is never formed: scores of 1e38 would swallow lz
-    smax = m;
+    A.given[row] = there ? logp(xt) : __builtin_nanf("");
   }
   if constexpr (TOP) {
-    // The chunks' best in rounds of kChunk keys, the best so far carried along.
-    const uint64_t* b = A.best + row * A.chunks * A.top;
-    const int n = A.chunks * A.top;
-    int at = 0;
-    bool first = true;
-    while (first || at < n) {
-      uint64_t key[kPer];
-      const int room = first ? kChunk : kChunk - kMaxTop;
+    if (n <= kThreads) {                                   // few: ranked by counting
+      if ((int)threadIdx.x < n) S.cand[threadIdx.x] = own;
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int p = threadIdx.x + kThreads * i;
-        key[i] = p < room ? (at + p < n ? b[at + p] : 0) : (!first && p - room < A.top ? kept[p - room] : 0);
+      if (own != 0) {
+        int r = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) r += S.cand[i] > own;
+        if (r < A.top) kept[r] = own;
       }
       __syncthreads();
-      select_top(key, A.top, S, [&](int r, uint64_t k) { kept[r] = k; });
-      at += room;
-      first = false;
+    } else {                                               // in rounds of kChunk, the best so far carried along
+      bool begun = false;
+      for (int at = 0; at < n;) {
+        uint64_t key[kPer];
+        const int room = begun ? kChunk - kMaxTop : kChunk;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int p = threadIdx.x + kThreads * i;
+          key[i] = p < room ? (at + p < n ? b[at + p] : 0) : (begun && p - room < A.top ? kept[p - room] : 0);
+        }
+        __syncthreads();
+        select_top(key, A.top, S, [&](int r, uint64_t k) { kept[r] = k; });
+        at += room;
+        begun = true;
+      }
     }
     for (int i = threadIdx.x; i < A.top; i += kThreads) {
-      const float v = key_value(kept[i]);
-      A.values[row * A.top + i] = v == kNegInf && slz == slz ? kNegInf : (float)(((double)v - (double)smax) - slz);
+      A.values[row * A.top + i] = logp(key_value(kept[i]));
       A.ids[row * A.top + i] = key_index(kept[i]);
     }
   }
+}
+
+// Workgroups per row: about 4096 in all, 2048 where the lists are long, at most one per chunk.
+// A workgroup that takes more steps has its lists filled once for all of them (1000 rows, top
+// 50: 324 us with 8192 workgroups, 256 with 4096, 220 with 2048; 1500 rows, top 5: 215, 195,
+// 198), fewer of them fill the device less evenly (64 rows, top 20: 34, 34, 39).
+int parts_of(int M, int chunks, int top) {
+  const int total = top > 24 ? 2048 : 4096;
+  const int want = (total + M - 1) / M;
+  return want < chunks ? want : chunks;
 }
 
 constexpr int kRowsPerLaunch = 65535;
@@ -250,7 +386,7 @@ using namespace rspx;
 extern "C" int64_t rspx_token_logprobs_workspace_bytes(int M, int V, int top) {
   if (M < 0 || V <= 0 || top < 0 || top > kMaxTop) return -1;
   const int64_t chunks = ((int64_t)V + kChunk - 1) / kChunk;
-  return (int64_t)M * chunks * (8 * (int64_t)top + 12) + 8;
+  return (int64_t)M * (8 * (int64_t)top * (M ? parts_of(M, (int)chunks, top) : 0) + 48 * chunks) + 8;
 }
 
 extern "C" int rspx_token_logprobs(const float* logits, int64_t sl, int M, int V, int off, int size, const int64_t* tokens,
@@ -271,16 +407,18 @@ extern "C" int rspx_token_logprobs(const float* logits, int64_t sl, int M, int V
   A.V = V, A.off = off, A.top = top;
   A.end = (int)((int64_t)off + size < V ? off + size : V);
   A.chunks = (int)(((int64_t)V + kChunk - 1) / kChunk);
+  A.parts = parts_of(M, A.chunks, top);
   A.best = static_cast<uint64_t*>(workspace);
-  A.stat = reinterpret_cast<float*>(A.best + (int64_t)M * A.chunks * top);
+  A.stat = reinterpret_cast<float*>(A.best + (int64_t)M * A.parts * top);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const unsigned bytes = 4 * 8 * (unsigned)list_room(top);
   for (A.row0 = 0; A.row0 < M;) {
     const int n = M - A.row0 < kRowsPerLaunch ? M - A.row0 : kRowsPerLaunch;
     if (top) {
-      hipLaunchKernelGGL(logprobs_chunk_kernel<true>, dim3(A.chunks, n), dim3(kThreads), 0, s, A);
+      hipLaunchKernelGGL(logprobs_part_kernel<true>, dim3(A.parts, n), dim3(kThreads), bytes, s, A);
       hipLaunchKernelGGL(logprobs_join_kernel<true>, dim3(n), dim3(kThreads), 0, s, A);
     } else {
-      hipLaunchKernelGGL(logprobs_chunk_kernel<false>, dim3(A.chunks, n), dim3(kThreads), 0, s, A);
+      hipLaunchKernelGGL(logprobs_part_kernel<false>, dim3(A.parts, n), dim3(kThreads), 0, s, A);
       hipLaunchKernelGGL(logprobs_join_kernel<false>, dim3(n), dim3(kThreads), 0, s, A);
     }
     if (M - A.row0 <= kRowsPerLaunch) break;

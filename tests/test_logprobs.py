@@ -17,10 +17,11 @@ def _logits(M, V, seed=0, scale=2.5):
 
 
 def _exact(x, t, top, off=0, size=0):
-    """Results in float64 and bounds.  With d_j = x_j - m: d is rounded once and e^d computed to a few
-    units, so an element of z is off by (|d| + 8) 2^-24 relative, its sums over 16 elements, 6
-    steps of a wave and 2 of a workgroup by 24 * 2^-24; chunks are joined in 64 bits and every
-    result is rounded once.  u = sum e d carries the same error on each term, and one more product."""
+    """Results in float64 and bounds.  With d_j = x_j - m: d is rounded once, so is d log2 e, whose
+    constant is off by 0.22 of 2^-24; each moves e^d by |d| 2^-24 relative, and 2^x itself is off by
+    a unit: (2.25 |d| + 8) 2^-24 for an element of z.  Its sums over 16 elements and the 6 steps
+    of a wave add 22 * 2^-24; the waves' steps are joined in 64 bits and every result is rounded once.
+    u = sum e d carries the same error on each term, one more d and one more product."""
     x = x.double().clone()
     x[:, off:off + size] = -math.inf
     lp = torch.log_softmax(x, -1)
@@ -28,10 +29,10 @@ def _exact(x, t, top, off=0, size=0):
     m = x.max(-1, keepdim=True).values
     d = torch.where(p > 0, m - x, torch.zeros_like(x))
     eps = 2.0 ** -24
-    ez = eps * (40 + 2 * (p * d).sum(-1))
+    ez = eps * (40 + 2.25 * (p * d).sum(-1))
     given = lp.gather(1, t[:, None])[:, 0]
     entropy = -torch.where(p > 0, p * lp, torch.zeros_like(p)).sum(-1)
-    eh = ez + eps * ((p * d * (42 + 2 * d)).sum(-1) + (p * d).sum(-1) * (40 + 2 * (p * d).sum(-1)))
+    eh = ez + eps * ((p * d * (42 + 2.25 * d)).sum(-1) + (p * d).sum(-1) * (40 + 2.25 * (p * d).sum(-1)))
     ids = torch.argsort(x, dim=-1, descending=True, stable=True)[:, :top]
     values = lp.gather(1, ids)
     return (given, ez + eps * given.abs()), (entropy, eh + eps * entropy.abs()), (values, ez[:, None] + eps * values.abs()), ids
