@@ -57,19 +57,22 @@ __device__ __forceinline__ s16x4 tr_read(const lds_char* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
 }
 
-// 16-byte unit swizzles of a staged row of U units: eight consecutive keys' units of one
-// column lie in different banks (K), four keys' pairs of units (V).
+// 16-byte unit swizzles of a staged row of U units, 256 bytes of banks: sixteen consecutive
+// keys' units of one column lie in different banks (K); so do four keys' four units, and
+// eight keys' two (V).
 template <int D>
 __device__ __forceinline__ int kswizzle(int key) {
   constexpr int U = D / 8;
-  if constexpr (U >= 8) return key % 8;
-  else return (key / (8 / U)) % U;
+  if constexpr (U >= 16) return key % 16;
+  else return (key / (16 / U)) % U;
 }
 template <int D>
 __device__ __forceinline__ int vswizzle(int key) {
   constexpr int U = D / 8;
-  if constexpr (U >= 16) return 2 * (key % 8);
-  else return 2 * ((key / (16 / U)) % (U / 2));
+  const int odd = 2 * ((key >> 2) & 1);
+  if constexpr (U >= 16) return 4 * (key % 4) + odd;
+  else if constexpr (U == 8) return 4 * ((key >> 1) & 1) + odd;
+  else return odd;
 }
 
 // HW heads and RW = 4 / HW row blocks of 32 rows per workgroup.
