@@ -36,6 +36,10 @@ constexpr int kRows = 32;            // rows of a wave
 constexpr float kTau = 8.0f;         // log2 headroom before the reference maximum moves
 constexpr float kNone = -1e30f;      // reference maximum before the first key
 
+constexpr int kEdges = 8;            // more than the steps that some row of a tile sees in part
+// Waves per SIMD, that is workgroups per CU, that the registers and the LDS allow.
+constexpr int waves_per_simd(int D) { return D >= 256 ? 1 : D >= 128 ? 2 : D >= 64 ? 3 : 4; }
+
 struct PromptArgs {
   const uint16_t *q, *k, *v;
   const int* tiles;            // [n][4]: first row, rows, first key, keys the first row sees
@@ -55,6 +59,21 @@ __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t r, int voff, lds_c
 __device__ __forceinline__ s16x4 tr_read(const lds_char* __restrict__ p) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+}
+
+// LDS reads of what is in place (its loads waited for, the barrier passed).  __restrict__:
+// without alias information the compiler waits for every load to LDS in flight, the next
+// steps' included, ahead of the first read.
+__device__ __forceinline__ u32x4 read16(const lds_char* __restrict__ p) {
+  return *(const __attribute__((address_space(3))) u32x4*)p;
+}
+
+// A barrier that does not wait for the loads in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // 16-byte unit swizzles of a staged row of U units, 256 bytes of banks: sixteen consecutive
@@ -77,11 +96,14 @@ __device__ __forceinline__ int vswizzle(int key) {
 
 // HW heads and RW = 4 / HW row blocks of 32 rows per workgroup.
 template <int D, int HW>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(PromptArgs A) {
+__global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(PromptArgs A) {
   constexpr int U = D / 8, NS = D / 16, DT = D / 32;
-  constexpr int kBytes = kKeys * D * 2;                    // K or V of one stage
+  constexpr int kBytes = kKeys * D * 2;                    // K or V of one step
   constexpr int kLoads = kBytes / 1024 / 4;                // 1 KB loads per wave, K and V each
-  __shared__ __align__(16) char lds[2][2][kBytes];
+  // One object: beside a second one the compiler waits for the loads to LDS in flight, the
+  // next step's too, ahead of a step's first read.
+  __shared__ __align__(16) char lds[4 * kBytes + 4 * kEdges];
+  int* flags = reinterpret_cast<int*>(lds + 4 * kBytes);
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -94,10 +116,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(Prom
   const int rows = min(min(max(T[1], 0), kRows * (4 / HW)), A.Tq - q0);
   const int seen0 = T[3];                                  // row i sees keys [k0, k0 + seen0 + i)
   const int keys = (int)min(max((int64_t)seen0 + rows - 1, (int64_t)0), (int64_t)(A.Tk - k0));
+  const int steps = (keys + kKeys - 1) / kKeys;
+  const int whole = min(max(seen0, 0), keys) / kKeys;      // steps that every row sees whole
+  if (threadIdx.x < kEdges) flags[threadIdx.x] = 0;
 
   const int rb = kRows * (w / HW);                         // this wave's rows in the tile
   const int row = rb + col;
-  const int seen = min(seen0 + row, keys);                 // keys of this lane's row
+  const int seen = (int)min((int64_t)seen0 + row, (int64_t)keys);   // keys of this lane's row
   const bool live = row < rows;
 
   // B operand of the scores: lane (col, half) holds row col, head_dim 16 i + 8 half .. + 7.
@@ -122,16 +147,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(Prom
     vo[j] = (int)(2 * key * A.svt) + 16 * ((u % U) ^ vswizzle<D>(key));
   }
   auto issue = [&](int t) {
-    const int left = min(keys - t * kKeys, kKeys);         // > 0
+    if (t >= steps) return;
+    const int left = min(keys - t * kKeys, kKeys);
     const auto rk = rsrc(kp + (int64_t)t * kKeys * A.skt, (uint32_t)(2 * (left - 1) * A.skt + 2 * D));
     const auto rv = rsrc(vp + (int64_t)t * kKeys * A.svt, (uint32_t)(2 * (left - 1) * A.svt + 2 * D));
-    lds_char* dk = (lds_char*)lds[t & 1][0];
-    lds_char* dv = (lds_char*)lds[t & 1][1];
+    lds_char* dk = (lds_char*)lds + 2 * kBytes * (t & 1);
+    lds_char* dv = (lds_char*)lds + 2 * kBytes * (t & 1) + kBytes;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) to_lds(rk, ko[j], dk + 1024 * (4 * j + w));
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) to_lds(rv, vo[j], dv + 1024 * (4 * j + w));
   };
+  issue(0);
 
   float mref = kNone, lsum = 0.f;
   f32x16 acc[DT];
@@ -140,16 +167,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(Prom
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
 
-  const int steps = (keys + kKeys - 1) / kKeys;
-  if (steps > 0) issue(0);
-  // One step of 64 keys.  `edge`: some row of the tile may not see all of them.
+  // One step of 64 keys.  `edge`: some row may not see all of them.
   auto step = [&](int t, auto edge) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of step t
-    __syncthreads();                                       // everyone's; and step t - 1 is read
-    if (t + 1 < steps) issue(t + 1);
-    const lds_char* sk = (const lds_char*)lds[t & 1][0];
-    const lds_char* sv = (const lds_char*)lds[t & 1][1];
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of the step
+    lds_barrier();                                         // everyone's; and the step before is read
+    issue(t + 1);
+    const lds_char* sk = (const lds_char*)lds + 2 * kBytes * (t & 1);
+    lds_char* sv = (lds_char*)lds + 2 * kBytes * (t & 1) + kBytes;
+    // A key that a row does not see has p = 0, but 0 * inf and 0 * NaN are NaN: such a value
+    // among the step's may not reach the rows before it.  Each wave looks a quarter of V over.
+    bool odd = false;
+    if constexpr (edge) {
+      uint32_t found = 0;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const u32x4 x = read16(sv + 1024 * (4 * j + w) + 16 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) found |= (x[e] & 0x7f807f80u) + 0x00800080u;   // an exponent of ones carries
+      }
+      if (__builtin_amdgcn_ballot_w64((found & 0x80008000u) != 0) != 0 && lane == 0) flags[t - whole] = 1;
+      lds_barrier();
+      odd = __builtin_amdgcn_readfirstlane(flags[t - whole]) != 0;
+    }
 
+    bf16x8 p[4];
     // S^T: two blocks of 32 keys.  Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
     f32x16 s[2];
 #pragma unroll
@@ -159,24 +200,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(Prom
       const int key = 32 * kb + col;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const u32x4 x = *(const __attribute__((address_space(3))) u32x4*)(
-            sk + 16 * (key * U + ((2 * i + half) ^ kswizzle<D>(key))));
+        const u32x4 x = read16(sk + 16 * (key * U + ((2 * i + half) ^ kswizzle<D>(key))));
         s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[i], s[kb], 0, 0, 0);
       }
     }
     if constexpr (edge) {   // keys that a row does not see
+      const int mine = seen - t * kKeys - 4 * half;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (t * kKeys + 32 * kb + 8 * (e / 4) + 4 * half + e % 4 >= seen) s[kb][e] = kNegInf;
+          if (32 * kb + 8 * (e / 4) + e % 4 >= mine) s[kb][e] = kNegInf;
     }
     float mx = s[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
     if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
       const float top = fmaxf(mx, shfl_xor(mx, 32)) * A.c;
-      const float mn = top > mref + kTau ? top : mref;     // rows that stay get a factor of exactly 1
+      const float mn = top > mref + kTau ? top : mref;   // rows that stay get a factor of exactly 1
       const float alpha = fexp2(mref - mn);
       lsum = lsum * alpha;
       mref = mn;
@@ -185,7 +226,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(Prom
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
     }
-    bf16x8 p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 x;
@@ -200,68 +240,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prompt_attn_kernel(Prom
       }
       p[i] = __builtin_bit_cast(bf16x8, x);
     }
+    if constexpr (edge) {
+      if (odd) {
+        // The values that are not finite go to the rows that see them one by one, and the
+        // product runs without them: every other sum keeps its bits.
+        const int mine = seen - t * kKeys;               // keys of the step that this lane's row sees
+#pragma unroll 1
+        for (int key = 0; key < kKeys; ++key)
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int d = 32 * j + 8 * (e / 4) + 4 * half + e % 4;
+              const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
+                  sv + 16 * (key * U + ((d / 8) ^ vswizzle<D>(key))) + 2 * (d % 8));
+              if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + bf16_to_f32(x);
+            }
+        lds_barrier();
+#pragma unroll 1
+        for (int j = 0; j < kLoads; ++j) {
+          auto* at = (__attribute__((address_space(3))) u32x4*)(sv + 1024 * (4 * j + w) + 16 * lane);
+          u32x4 x = *at;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u;
+            if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
+          }
+          *at = x;
+        }
+        lds_barrier();
+      }
+    }
     // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
     // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
-    auto vop = [&](int i, int j) {
-      s16x4 h[2];
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const int l16 = lane & 15;
-        const int key = 16 * i + 8 * z + 4 * half + (l16 >> 2);
-        const int u = 4 * j + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-        h[z] = tr_read(sv + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1));
-      }
-      return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    // A key that a row does not see has p = 0, but 0 * inf and 0 * NaN are NaN: such a value
-    // among the step's may not reach the rows before it.
-    bool odd = false;
-    if constexpr (edge) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < DT; ++j) {
-          asm volatile("" ::: "memory");                   // one operand at a time: registers
-          const s16x8 x = vop(i, j);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) odd |= (x[e] & 0x7f80) == 0x7f80;
-        }
-      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-    }
-    if (edge && odd) {
-      // The values that are not finite go to the rows that see them one by one, and the
-      // product runs without them: every other sum keeps its bits.
-      const int mine = seen - t * kKeys;                   // keys of the step that this lane's row sees
-#pragma unroll 1
-      for (int key = 0; key < kKeys; ++key)
-#pragma unroll
-        for (int j = 0; j < DT; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int d = 32 * j + 8 * (e / 4) + 4 * half + e % 4;
-            const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
-                sv + 16 * (key * U + ((d / 8) ^ vswizzle<D>(key))) + 2 * (d % 8));
-            if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + bf16_to_f32(x);
-          }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < DT; ++j) {
-          asm volatile("" ::: "memory");                   // one operand at a time: registers
-          s16x8 x = vop(i, j);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = (x[e] & 0x7f80) == 0x7f80 ? (short)0 : x[e];
-          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), p[i], acc[j], 0, 0, 0);
-        }
-      return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < DT; ++j)
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vop(i, j)), p[i], acc[j], 0, 0, 0);
+      for (int j = 0; j < DT; ++j) {
+        s16x4 h[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int l16 = lane & 15;
+          const int key = 16 * i + 8 * z + 4 * half + (l16 >> 2);
+          const int u = 4 * j + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+          h[z] = tr_read(sv + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1));
+        }
+        const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, p[i], acc[j], 0, 0, 0);
+      }
   };
-  const int whole = min(max(seen0, 0), keys) / kKeys;      // steps that every row sees whole
   int t = 0;
   for (; t < whole; ++t) step(t, std::false_type());
   for (; t < steps; ++t) step(t, std::true_type());
