@@ -5,17 +5,27 @@
 // over the keys j that row t of its sequence sees.  The work is a list of tiles of at most
 // 32 RW rows of one sequence; a workgroup takes one tile for 4 / RW query heads of one kv
 // head, each wave 32 rows of one head.  Keys and values of 64 positions at a time go from
-// memory straight into LDS (two stages) and serve all four waves.
+// memory straight into LDS (two slots of each) and serve all four waves.
 //
 // A wave computes S^T = K Q^T by v_mfma_f32_32x32x16_bf16, so a lane holds 32 scores of one
 // row: the softmax (fp32, a running maximum that moves only when a score passes it by
 // 2^kTau) needs no lane exchange but the rare move's.  The probabilities, rounded to bf16
-// as the trie attention rounds them (relative error 2^-9 each, against fp32 sums), are used
-// in place as the B operand of O^T += V^T P^T with V read transposed from LDS.
+// as the trie attention rounds them (half a step each, against fp32 sums), are used in place
+// as the B operand of O^T += V^T P^T with V read transposed from LDS.  The products of the
+// next step's scores run beside a step's exponentials.
 //
 // Every row is computed from its own column of the MFMA tiles in 64-key steps from the
 // sequence's first key on: its bits depend on its sequence alone, not on the pack, on the
 // tile it falls in or on later rows.
+//
+// What bounds it: in long prompts the power budget (16384 tokens, 32 / 8 heads of 128: 1.98 ms,
+// 1.11 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.8 GHz, the
+// MFMAs are busy 58 % of it, VALU half; LDS reads 29 %, no bank conflicts); in short ones and
+// few heads the serial chain of a step at one wave per SIMD (1.0 us at D = 128).  Measured and
+// not kept: eight waves per tile that take the steps in turn and are joined (three quarters of
+// the time with few workgroups, but 337 us instead of 289 for 24 packed prompts, and the
+// choice may not depend on the pack), three and four steps in LDS (no gain), MFMAs and
+// exponentials interleaved by scheduling barriers (5 to 30 % slower), wave priorities (2 %).
 #include <type_traits>
 
 #include "common.h"
@@ -146,19 +156,47 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
     ko[j] = (int)(2 * key * A.skt) + 16 * ((u % U) ^ kswizzle<D>(key));
     vo[j] = (int)(2 * key * A.svt) + 16 * ((u % U) ^ vswizzle<D>(key));
   }
-  auto issue = [&](int t) {
+  auto issue_k = [&](int t) {
     if (t >= steps) return;
     const int left = min(keys - t * kKeys, kKeys);
-    const auto rk = rsrc(kp + (int64_t)t * kKeys * A.skt, (uint32_t)(2 * (left - 1) * A.skt + 2 * D));
-    const auto rv = rsrc(vp + (int64_t)t * kKeys * A.svt, (uint32_t)(2 * (left - 1) * A.svt + 2 * D));
-    lds_char* dk = (lds_char*)lds + 2 * kBytes * (t & 1);
-    lds_char* dv = (lds_char*)lds + 2 * kBytes * (t & 1) + kBytes;
+    const auto r = rsrc(kp + (int64_t)t * kKeys * A.skt, (uint32_t)(2 * (left - 1) * A.skt + 2 * D));
+    lds_char* dst = (lds_char*)lds + kBytes * (t & 1);
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) to_lds(rk, ko[j], dk + 1024 * (4 * j + w));
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) to_lds(rv, vo[j], dv + 1024 * (4 * j + w));
+    for (int j = 0; j < kLoads; ++j) to_lds(r, ko[j], dst + 1024 * (4 * j + w));
   };
-  issue(0);
+  auto issue_v = [&](int t) {
+    if (t >= steps) return;
+    const int left = min(keys - t * kKeys, kKeys);
+    const auto r = rsrc(vp + (int64_t)t * kKeys * A.svt, (uint32_t)(2 * (left - 1) * A.svt + 2 * D));
+    lds_char* dst = (lds_char*)lds + kBytes * (2 + (t & 1));
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) to_lds(r, vo[j], dst + 1024 * (4 * j + w));
+  };
+  // S^T of a step: two blocks of 32 keys.  Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
+  auto scores = [&](int t, f32x16 (&o)[2]) __attribute__((always_inline)) {
+    const lds_char* sk = (const lds_char*)lds + kBytes * (t & 1);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[kb][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int key = 32 * kb + col;
+        const u32x4 x = read16(sk + 16 * (key * U + ((2 * i + half) ^ kswizzle<D>(key))));
+        o[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[i], o[kb], 0, 0, 0);
+      }
+  };
+  f32x16 s[2];
+  if (steps > 0) {
+    issue_k(0);
+    issue_v(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kLoads);           // vmcnt(kLoads): this wave's part of K
+    lds_barrier();
+    issue_k(1);
+    scores(0, s);
+  }
 
   float mref = kNone, lsum = 0.f;
   f32x16 acc[DT];
@@ -167,13 +205,15 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
 
-  // One step of 64 keys.  `edge`: some row may not see all of them.
+  const int first_edge = min(whole, steps - 1);            // the last step has no scores to run ahead
+  // One step of 64 keys, whose scores are in s; the next ones' products run beside its softmax.
+  // `edge`: some row may not see all of its keys.
   auto step = [&](int t, auto edge) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of the step
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of V and the next K
     lds_barrier();                                         // everyone's; and the step before is read
-    issue(t + 1);
-    const lds_char* sk = (const lds_char*)lds + 2 * kBytes * (t & 1);
-    lds_char* sv = (lds_char*)lds + 2 * kBytes * (t & 1) + kBytes;
+    issue_k(t + 2);
+    issue_v(t + 1);
+    lds_char* sv = (lds_char*)lds + kBytes * (2 + (t & 1));
     // A key that a row does not see has p = 0, but 0 * inf and 0 * NaN are NaN: such a value
     // among the step's may not reach the rows before it.  Each wave looks a quarter of V over.
     bool odd = false;
@@ -185,25 +225,12 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
         for (int e = 0; e < 4; ++e) found |= (x[e] & 0x7f807f80u) + 0x00800080u;   // an exponent of ones carries
       }
-      if (__builtin_amdgcn_ballot_w64((found & 0x80008000u) != 0) != 0 && lane == 0) flags[t - whole] = 1;
+      if (__builtin_amdgcn_ballot_w64((found & 0x80008000u) != 0) != 0 && lane == 0) flags[t - first_edge] = 1;
       lds_barrier();
-      odd = __builtin_amdgcn_readfirstlane(flags[t - whole]) != 0;
+      odd = __builtin_amdgcn_readfirstlane(flags[t - first_edge]) != 0;
     }
 
     bf16x8 p[4];
-    // S^T: two blocks of 32 keys.  Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
-    f32x16 s[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-      const int key = 32 * kb + col;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const u32x4 x = read16(sk + 16 * (key * U + ((2 * i + half) ^ kswizzle<D>(key))));
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[i], s[kb], 0, 0, 0);
-      }
-    }
     if constexpr (edge) {   // keys that a row does not see
       const int mine = seen - t * kKeys - 4 * half;
 #pragma unroll
@@ -226,6 +253,8 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
     }
+    f32x16 ahead[2];
+    if constexpr (!edge) scores(t + 1, ahead);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 x;
@@ -288,9 +317,11 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
         const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
         acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, p[i], acc[j], 0, 0, 0);
       }
+    if constexpr (!edge) s[0] = ahead[0], s[1] = ahead[1];
+    else if (t + 1 < steps) scores(t + 1, s);
   };
   int t = 0;
-  for (; t < whole; ++t) step(t, std::false_type());
+  for (; t < first_edge; ++t) step(t, std::false_type());
   for (; t < steps; ++t) step(t, std::true_type());
 
   // Lane (col, half): row col, head_dim 32 j + 8 (e / 4) + 4 half + e % 4.
