@@ -33,6 +33,7 @@
  *   rspx_prompt_attn    causal attention over whole prompts, packed
  *   rspx_paged_attn     attention of one new token per sequence over a paged cache
  *   rspx_kv_move, rspx_kv_write   rows of a paged cache moved and written
+ *   rspx_pages_*        who holds which page of it (host code)
  *   rspx_token_logprobs log probabilities, entropy and best alternatives per row
  */
 #ifndef RESPECT_AMD_H
@@ -51,6 +52,8 @@ extern "C" {
 #define RSPX_EWORKSPACE (-3)   /* workspace missing or too small */
 #define RSPX_EALIGN (-4)       /* pointer or stride not 16-byte aligned */
 #define RSPX_ELAUNCH (-5)      /* HIP launch error */
+#define RSPX_EFULL (-6)        /* not enough free pages or sequences */
+#define RSPX_ENOMEM (-7)       /* no host memory */
 
 /* Tiled activation layout.  Passed as the row stride of a bf16 activation
  * matrix A[M, K] with K % 32 == 0 -- x of rspx_linear, rspx_linear_silu and
@@ -509,6 +512,44 @@ int rspx_kv_move(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh
 int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh,
                   const int32_t* slots, int T, int cap, void* cache_k, int64_t sckh, int64_t sckn, void* cache_v,
                   int64_t scvh, int64_t scvn, int HK, int D, void* stream);
+
+/* ---------------------------------------------------------------- pages of a paged cache
+ * Who holds which page: host code, nothing is enqueued.  `pages` pages of `page` rows (a
+ * power of two), up to `sequences` sequences at a time, named by small numbers.  Pages are
+ * taken lowest first and counted: those that sequences share are free once none holds them.
+ * A call that fails (RSPX_EINVAL: no such sequence, one named twice, a bad count;
+ * RSPX_EFULL; RSPX_ENOMEM) has changed nothing.  One thread at a time.
+ *   add      n new sequences of lengths[i] rows -> ids
+ *   extend   room for counts[i] further rows; a begun page that is shared becomes its own
+ *   fork     `copies` sequences with the content of each of ids -> out [n * copies], those
+ *            of the first one first: full pages shared, the begun one copied
+ *   compact  row starts[i] + path[k] becomes row starts[i] + k, and the sequence ends after
+ *            them; its pages stay with it.  Path i is paths[ends[i - 1] .. ends[i]), increasing
+ *   trim     the pages past the end are given back;  free: the sequences are forgotten
+ * The rows that a call makes move on the device are its moves: rspx_pages_moves gives their
+ * number and that of their groups, rspx_pages_copy_moves writes groups [n_groups + 1] and
+ * then moves [n_moves][2], as rspx_kv_move takes them (nothing at all for no group).
+ *   width    the most pages that one of ids holds;  table: [n][width] page numbers, -1 past
+ *            a sequence's pages, and lens [n], as rspx_paged_attn takes them
+ *   slots    pool rows of rows first[i] .. first[i] + counts[i] - 1, one sequence after another
+ */
+typedef struct rspx_pages rspx_pages;
+rspx_pages* rspx_pages_new(int pages, int page, int sequences); /* NULL: bad sizes or no memory */
+void rspx_pages_delete(rspx_pages* p);
+int rspx_pages_available(const rspx_pages* p);
+int64_t rspx_pages_length(const rspx_pages* p, int seq); /* -1: no such sequence */
+int rspx_pages_add(rspx_pages* p, const int64_t* lengths, int n, int32_t* ids);
+int rspx_pages_extend(rspx_pages* p, const int32_t* ids, int n, const int64_t* counts);
+int rspx_pages_fork(rspx_pages* p, const int32_t* ids, int n, int copies, int32_t* out);
+int rspx_pages_compact(rspx_pages* p, const int32_t* ids, int n, const int64_t* starts, const int64_t* paths,
+                       const int64_t* ends);
+int rspx_pages_trim(rspx_pages* p, const int32_t* ids, int n);
+int rspx_pages_free(rspx_pages* p, const int32_t* ids, int n);
+int rspx_pages_moves(const rspx_pages* p, int32_t* n_groups, int32_t* n_moves);
+int rspx_pages_copy_moves(const rspx_pages* p, int32_t* out);
+int rspx_pages_width(rspx_pages* p, const int32_t* ids, int n);
+int rspx_pages_table(rspx_pages* p, const int32_t* ids, int n, int width, int32_t* table, int32_t* lens);
+int rspx_pages_slots(rspx_pages* p, const int32_t* ids, int n, const int64_t* first, const int64_t* counts, int32_t* out);
 
 /* ---------------------------------------------------------------- scores of given tokens
  * Per row of logits [M, V] (fp32, row stride sl, 16-byte aligned rows), with columns

@@ -96,6 +96,21 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_kv_move": (_i32, [_c_p, _i32, _i32, _i32, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
     "rspx_kv_write": (_i32, [_c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i32, _i32, _c_p, _i64, _i64, _c_p, _i64, _i64,
                              _i32, _i32, _c_p]),
+    "rspx_pages_new": (_c_p, [_i32, _i32, _i32]),
+    "rspx_pages_delete": (None, [_c_p]),
+    "rspx_pages_available": (_i32, [_c_p]),
+    "rspx_pages_length": (_i64, [_c_p, _i32]),
+    "rspx_pages_add": (_i32, [_c_p, _c_p, _i32, _c_p]),
+    "rspx_pages_extend": (_i32, [_c_p, _c_p, _i32, _c_p]),
+    "rspx_pages_fork": (_i32, [_c_p, _c_p, _i32, _i32, _c_p]),
+    "rspx_pages_compact": (_i32, [_c_p, _c_p, _i32, _c_p, _c_p, _c_p]),
+    "rspx_pages_trim": (_i32, [_c_p, _c_p, _i32]),
+    "rspx_pages_free": (_i32, [_c_p, _c_p, _i32]),
+    "rspx_pages_moves": (_i32, [_c_p, _c_p, _c_p]),
+    "rspx_pages_copy_moves": (_i32, [_c_p, _c_p]),
+    "rspx_pages_width": (_i32, [_c_p, _c_p, _i32]),
+    "rspx_pages_table": (_i32, [_c_p, _c_p, _i32, _i32, _c_p, _c_p]),
+    "rspx_pages_slots": (_i32, [_c_p, _c_p, _i32, _c_p, _c_p, _c_p]),
     "rspx_token_logprobs_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "rspx_token_logprobs": (_i32, [_c_p, _i64, _i32, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _i64,
                                    _c_p]),

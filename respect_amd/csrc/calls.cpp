@@ -16,6 +16,7 @@
 
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -492,11 +493,183 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------ pages of a paged cache
+// handle: the rspx_pages*; bases, HK, D, sh, sn, cap: the pools as rspx_kv_move takes them.
+
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
+// A list or tuple of ints that fit T.
+template <class T>
+bool integers(PyObject* o, std::vector<T>& v) {
+  if (!PyList_CheckExact(o) && !PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  v.reserve(v.size() + n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    int64_t x;
+    if (!integer(PySequence_Fast_GET_ITEM(o, i), x) || (int64_t)(T)x != x) return false;
+    v.push_back((T)x);
+  }
+  return true;
+}
+
+// One number for each of n, or n of them.
+bool counts_of(PyObject* o, size_t n, std::vector<int64_t>& v) {
+  int64_t x;
+  if (integer(o, x)) {
+    v.assign(n, x);
+    return true;
+  }
+  return integers(o, v) && v.size() == n;
+}
+
+struct Pool {
+  rspx_pages* pages;
+  const Tensor* bases;
+  int64_t HK, D, sh, sn, cap;
+  bool read(PyObject* handle, PyObject* const* a, Py_ssize_t n) {
+    int64_t h;
+    if (n != 6 || !integer(handle, h) || h == 0 || !(bases = plain(a[0], at::kLong))) return false;
+    pages = reinterpret_cast<rspx_pages*>(h);
+    return integer(a[1], HK) && integer(a[2], D) && integer(a[3], sh) && integer(a[4], sn) && integer(a[5], cap);
+  }
+};
+
+// int32 numbers that fill(host pointer) writes, on the device.  torch keeps the pinned
+// memory until the copy is done.
+template <class F>
+Tensor uploaded(const Tensor& like, int64_t n, F&& fill) {
+  Tensor host = at::empty({n}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+  fill(host.data_ptr<int>());
+  return host.to(like.device(), at::kInt, /*non_blocking=*/true);
+}
+
+// Enqueues the moves of the call just made.
+int move_rows(const Pool& p) {
+  int32_t groups = 0, moves = 0;
+  rspx_pages_moves(p.pages, &groups, &moves);
+  if (groups == 0) return RSPX_OK;
+  Tensor t = uploaded(*p.bases, (int64_t)groups + 1 + 2 * (int64_t)moves, [&](int* out) { rspx_pages_copy_moves(p.pages, out); });
+  return call([&] {
+    const int32_t* d = t.const_data_ptr<int>();
+    return rspx_kv_move(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel(), (int)p.HK, (int)p.D, p.sh, p.sn,
+                        (int)p.cap, d, groups, d + groups + 1, moves, stream_of(*p.bases));
+  });
+}
+
+PyObject* list_of(const std::vector<int32_t>& v) {
+  PyObject* l = PyList_New((Py_ssize_t)v.size());
+  if (!l) return nullptr;
+  for (size_t i = 0; i < v.size(); ++i) {
+    PyObject* x = PyLong_FromLong(v[i]);
+    if (!x) {
+      Py_DECREF(l);
+      return nullptr;
+    }
+    PyList_SET_ITEM(l, (Py_ssize_t)i, x);
+  }
+  return l;
+}
+
+// pages_fork(handle, seqs, copies, *pool) -> the new sequences
+PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pool p;
+  std::vector<int32_t> ids;
+  int64_t copies;
+  if (n != 9 || !p.read(a[0], a + 3, 6) || !integers(a[1], ids) || !integer(a[2], copies) || !fits_int(copies)) NOT_TAKEN;
+  const c10::DeviceGuard guard(p.bases->device());
+  if (capturing() || (int64_t)ids.size() * copies > 1 << 24) NOT_TAKEN;
+  std::vector<int32_t> out(ids.size() * copies);
+  STATUS(rspx_pages_fork(p.pages, ids.data(), (int)ids.size(), (int)copies, out.data()));
+  STATUS(move_rows(p));
+  return list_of(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_extend(handle, seqs, counts, *pool) -> True
+PyObject* pages_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pool p;
+  std::vector<int32_t> ids;
+  std::vector<int64_t> counts;
+  if (n != 9 || !p.read(a[0], a + 3, 6) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), counts)) NOT_TAKEN;
+  const c10::DeviceGuard guard(p.bases->device());
+  if (capturing()) NOT_TAKEN;
+  STATUS(rspx_pages_extend(p.pages, ids.data(), (int)ids.size(), counts.data()));
+  STATUS(move_rows(p));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_compact(handle, seqs, starts, paths, *pool) -> True
+PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pool p;
+  std::vector<int32_t> ids;
+  std::vector<int64_t> starts, paths, ends;
+  if (n != 10 || !p.read(a[0], a + 4, 6) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), starts) ||
+      !PyList_CheckExact(a[3]) || PyList_GET_SIZE(a[3]) != (Py_ssize_t)ids.size())
+    NOT_TAKEN;
+  for (size_t i = 0; i < ids.size(); ++i) {
+    if (!integers(PyList_GET_ITEM(a[3], (Py_ssize_t)i), paths)) NOT_TAKEN;
+    ends.push_back((int64_t)paths.size());
+  }
+  const c10::DeviceGuard guard(p.bases->device());
+  if (capturing()) NOT_TAKEN;
+  STATUS(rspx_pages_compact(p.pages, ids.data(), (int)ids.size(), starts.data(), paths.data(), ends.data()));
+  STATUS(move_rows(p));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_tables(handle, seqs, *pool) -> (table, lens)
+PyObject* pages_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pool p;
+  std::vector<int32_t> ids;
+  if (n != 8 || !p.read(a[0], a + 2, 6) || !integers(a[1], ids)) NOT_TAKEN;
+  const c10::DeviceGuard guard(p.bases->device());
+  if (capturing()) NOT_TAKEN;
+  const int64_t B = (int64_t)ids.size(), width = rspx_pages_width(p.pages, ids.data(), (int)B);
+  if (width < 0) return PyLong_FromLong((long)width);
+  Tensor t = uploaded(*p.bases, B * (width + 1), [&](int* out) {
+    rspx_pages_table(p.pages, ids.data(), (int)B, (int)width, out, out + B * width);
+  });
+  return Py_BuildValue("(NN)", wrap(t.narrow(0, 0, B * width).view({B, width})), wrap(t.narrow(0, B * width, B)));
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_slots(handle, seqs, first, counts, *pool) -> slots
+PyObject* pages_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pool p;
+  std::vector<int32_t> ids;
+  std::vector<int64_t> first, counts;
+  if (n != 10 || !p.read(a[0], a + 4, 6) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), first) ||
+      !counts_of(a[3], ids.size(), counts))
+    NOT_TAKEN;
+  const c10::DeviceGuard guard(p.bases->device());
+  if (capturing()) NOT_TAKEN;
+  int64_t all = 0;
+  for (const int64_t c : counts) {
+    if (c < 0 || c > p.cap) NOT_TAKEN;   // the wrapper refuses it
+    all += c;
+  }
+  int rc = RSPX_OK;
+  Tensor t = uploaded(*p.bases, all, [&](int* out) {
+    rc = rspx_pages_slots(p.pages, ids.data(), (int)ids.size(), first.data(), counts.data(), out);
+  });
+  STATUS(rc);
+  return wrap(std::move(t));
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(silu_mul), FAST(rmsnorm), FAST(qk_norm_rope), FAST(rmsnorm_qk_norm_rope),
                          FAST(rope),     FAST(add_sq),  FAST(norm_apply),   FAST(rope_vision),
                          FAST(linear),   FAST(trie_attn), FAST(prompt_attn), FAST(paged_attn),
-                         FAST(token_logprobs), {nullptr, nullptr, 0, nullptr}};
+                         FAST(token_logprobs), FAST(pages_fork), FAST(pages_extend), FAST(pages_compact),
+                         FAST(pages_tables),   FAST(pages_slots), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -11,6 +11,8 @@ extern "C" const char* rspx_strerror(int code) {
     case RSPX_EWORKSPACE: return "workspace missing or too small";
     case RSPX_EALIGN: return "pointer or stride not 16-byte aligned";
     case RSPX_ELAUNCH: return "HIP kernel launch failed";
+    case RSPX_EFULL: return "not enough free pages or sequences";
+    case RSPX_ENOMEM: return "no host memory";
     default: return "unknown error";
   }
 }

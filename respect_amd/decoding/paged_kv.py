@@ -3,11 +3,13 @@
 No counterpart in the reference, whose buffer holds one request (kv_buffer.py here).
 Per layer one bf16 pool [HK, pages * page, D] for K and one for V; row j of a sequence is
 pool row ``table[j // page] * page + j % page``.  Who holds which page is kept on the
-host (pages are counted, so that forks share the full ones); the rows move on the GPU, all
-layers and sequences in one launch (rspx_kv_move).  ``paged_attn`` reads the pools through
-``tables``.
+host (rspx_pages_*: pages are counted, so that forks share the full ones); the rows move on
+the GPU, all layers and sequences in one launch (rspx_kv_move).  ``paged_attn`` reads the
+pools through ``tables``.
 """
 from __future__ import annotations
+
+import ctypes
 
 import numpy as np
 import torch
@@ -16,269 +18,257 @@ from .. import _lib
 from ..kernels._tensor import as_kernel_input
 
 
+def _p(a: np.ndarray) -> int:
+    return a.ctypes.data
+
+
+class PageTable:
+    """Who holds which page, without the pools: the host half of ``PagedKVCache``.  A refused
+    call (``ValueError``: no such sequence, one named twice, a bad count; ``RuntimeError``: too
+    few pages or sequences) changes nothing."""
+
+    def __init__(self, pages: int, page: int, sequences: int):
+        self._lib = _lib.lib()
+        self.handle = self._lib.rspx_pages_new(pages, page, sequences)
+        if not self.handle:
+            raise ValueError("PagedKVCache: pages and sequences >= 1, page a power of two, pages * page below 2^31")
+
+    def __del__(self):
+        if getattr(self, "handle", None):
+            self._lib.rspx_pages_delete(self.handle)
+            self.handle = None
+
+    def _call(self, what: str, *args) -> None:
+        rc = getattr(self._lib, "rspx_pages_" + what)(self.handle, *args)
+        if rc < 0:
+            self.refuse(what, rc)
+
+    @staticmethod
+    def refuse(what: str, rc: int) -> None:
+        """Raise what status ``rc`` of a bookkeeping call stands for."""
+        if rc == -1:
+            raise ValueError(f"PagedKVCache.{what}: no such sequence, one named twice, or a bad count, row or path")
+        raise RuntimeError(f"PagedKVCache.{what}: {_lib.strerror(rc)} ({rc})")
+
+    @staticmethod
+    def _ids(seqs) -> np.ndarray:
+        ids = np.asarray(list(seqs), dtype=np.int64)
+        if ids.size and (ids.min() < 0 or ids.max() >= 1 << 31):
+            raise ValueError("PagedKVCache: no such sequence")
+        return ids.astype(np.int32)
+
+    @staticmethod
+    def _counts(n, many: int) -> np.ndarray:
+        """One number for each of ``many``, or that many of them."""
+        c = np.asarray(n, dtype=np.int64)
+        if c.ndim and c.shape != (many,):
+            raise ValueError(f"PagedKVCache: {many} counts are needed")
+        return np.ascontiguousarray(np.broadcast_to(c, (many,)))
+
+    @property
+    def available(self) -> int:
+        return self._lib.rspx_pages_available(self.handle)
+
+    def length(self, seq: int) -> int:
+        n = self._lib.rspx_pages_length(self.handle, seq) if 0 <= seq < 1 << 31 else -1
+        if n < 0:
+            raise ValueError("PagedKVCache: no such sequence")
+        return n
+
+    def add(self, lengths) -> list[int]:
+        n = np.asarray(list(lengths), dtype=np.int64)
+        ids = np.empty(len(n), np.int32)
+        self._call("add", _p(n), len(n), _p(ids))
+        return ids.tolist()
+
+    def extend(self, seqs, n) -> None:
+        ids = self._ids(seqs)
+        self._call("extend", _p(ids), len(ids), _p(self._counts(n, len(ids))))
+
+    def fork(self, seqs, copies: int) -> list[int]:
+        ids = self._ids(seqs)
+        if not 0 <= copies < 1 << 31:
+            raise ValueError("PagedKVCache: counts must be >= 0")
+        if len(ids) * copies >= 1 << 24:
+            self.refuse("fork", -6)
+        out = np.empty(len(ids) * copies, np.int32)
+        self._call("fork", _p(ids), len(ids), copies, _p(out))
+        return out.tolist()
+
+    def compact(self, seqs, starts, paths) -> None:
+        ids = self._ids(seqs)
+        paths = [np.asarray(list(p), dtype=np.int64) for p in paths]
+        if len(paths) != len(ids):
+            raise ValueError("PagedKVCache: one path per sequence")
+        flat = np.concatenate(paths) if paths else np.zeros(0, np.int64)
+        ends = np.cumsum([len(p) for p in paths], dtype=np.int64)
+        self._call("compact", _p(ids), len(ids), _p(self._counts(starts, len(ids))), _p(flat), _p(ends))
+
+    def trim(self, seqs) -> None:
+        ids = self._ids(seqs)
+        self._call("trim", _p(ids), len(ids))
+
+    def free(self, seqs) -> None:
+        ids = self._ids(seqs)
+        self._call("free", _p(ids), len(ids))
+
+    def moves(self) -> tuple[np.ndarray, np.ndarray]:
+        """(groups [g + 1], moves [m, 2]) that the last call makes rows move by."""
+        g, m = ctypes.c_int32(), ctypes.c_int32()
+        self._call("moves", ctypes.addressof(g), ctypes.addressof(m))
+        out = np.zeros(g.value + 1 + 2 * m.value, np.int32)
+        if g.value:
+            self._call("copy_moves", _p(out))
+        return out[:g.value + 1], out[g.value + 1:].reshape(-1, 2)
+
+    def table(self, seqs) -> tuple[np.ndarray, np.ndarray]:
+        ids = self._ids(seqs)
+        width = self._lib.rspx_pages_width(self.handle, _p(ids), len(ids))
+        if width < 0:
+            self.refuse("tables", width)
+        table, lens = np.empty((len(ids), width), np.int32), np.empty(len(ids), np.int32)
+        self._call("table", _p(ids), len(ids), width, _p(table), _p(lens))
+        return table, lens
+
+    def slots(self, seqs, first, count) -> np.ndarray:
+        ids = self._ids(seqs)
+        lo, n = self._counts(first, len(ids)), self._counts(count, len(ids))
+        if len(n) and (n.min() < 0 or any(c > self.length(s) for s, c in zip(ids.tolist(), n.tolist()))):
+            raise ValueError("PagedKVCache.slots: rows past a sequence's end")
+        out = np.empty(int(n.sum()), np.int32)
+        self._call("slots", _p(ids), len(ids), _p(lo), _p(n), _p(out))
+        return out
+
+
 class PagedKVCache:
     """``pages`` pages of ``page`` rows (a power of two), at most ``sequences`` sequences at a
-    time.  The bookkeeping methods run on the host, enqueue their copies on the current
-    stream and cannot be captured into a graph; on a failure (``RuntimeError`` for too few
-    pages or sequences, ``ValueError`` for the rest) nothing has changed."""
+    time.  Sequences are named by the numbers that ``add`` and ``fork`` give.  The methods
+    keep books on the host and enqueue their copies on the current stream; those that do
+    cannot be captured into a graph.  A refused call (``ValueError``; ``RuntimeError`` for
+    too few pages or sequences) changes nothing.  One thread at a time."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page: int = 64, device="cuda",
                  sequences: int = 1024):
-        if layers < 1 or kv_heads < 1 or pages < 1 or sequences < 1 or head_dim < 8 or head_dim % 8:
-            raise ValueError("PagedKVCache: layers, kv_heads, pages, sequences >= 1 and head_dim a multiple of 8")
-        if page < 1 or page & (page - 1) or pages * page >= 1 << 31:
-            raise ValueError("PagedKVCache: page must be a power of two, pages * page below 2^31")
+        if layers < 1 or kv_heads < 1 or head_dim < 8 or head_dim % 8:
+            raise ValueError("PagedKVCache: layers and kv_heads >= 1 and head_dim a multiple of 8")
+        self._t = PageTable(pages, page, sequences)
         self.layers, self.HK, self.D, self.page, self.pages = layers, kv_heads, head_dim, page, pages
         self.device = torch.device(device)
         shape = (kv_heads, pages * page, head_dim)
         self.k = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
-        self.bases = torch.tensor([t.data_ptr() for kv in zip(self.k, self.v) for t in kv], dtype=torch.int64).to(device)
-        self._refs = np.zeros(pages, np.int32)                 # sequences that hold each page
-        self._table = np.full((sequences, 8), -1, np.int32)    # pages of each sequence
-        self._held = np.zeros(sequences, np.int64)             # how many of them
-        self._len = np.full(sequences, -1, np.int64)           # rows, -1: no such sequence
-
-    # ------------------------------------------------------------------ what is there
+        bases = torch.tensor([t.data_ptr() for kv in zip(self.k, self.v) for t in kv], dtype=torch.int64).to(device)
+        k0 = self.k[0]
+        self._pool = (bases, kv_heads, head_dim, k0.stride(0), k0.stride(1), pages * page)
 
     @property
     def free_pages(self) -> int:
-        return int((self._refs == 0).sum())
+        return self._t.available
 
     def length(self, seq: int) -> int:
-        return int(self._len[self._ids([seq])[0]])
+        return self._t.length(seq)
 
-    def _ids(self, seqs, distinct: bool = True) -> np.ndarray:
-        ids = np.asarray(list(seqs), dtype=np.int64)
-        if ids.size and (ids.min() < 0 or ids.max() >= len(self._len) or (self._len[ids] < 0).any()):
-            raise ValueError("PagedKVCache: no such sequence")
-        if distinct and len(np.unique(ids)) != len(ids):
-            raise ValueError("PagedKVCache: a sequence is named twice")
-        return ids
-
-    def _counts(self, n, ids: np.ndarray) -> np.ndarray:
-        c = np.broadcast_to(np.asarray(n, dtype=np.int64), ids.shape)
-        if c.size and c.min() < 0:
-            raise ValueError("PagedKVCache: counts must be >= 0")
-        return c
-
-    def _take(self, n: int) -> np.ndarray:
-        """The n lowest free pages (not yet counted)."""
-        free = np.flatnonzero(self._refs == 0)
-        if len(free) < n:
-            raise RuntimeError(f"PagedKVCache: {n} pages needed, {len(free)} free")
-        return free[:n]
-
-    def _new_ids(self, n: int) -> np.ndarray:
-        free = np.flatnonzero(self._len < 0)
-        if len(free) < n:
-            raise RuntimeError(f"PagedKVCache: {n} sequences more than the {len(self._len)} there may be")
-        return free[:n]
-
-    def _widen(self, width: int) -> None:
-        if width > self._table.shape[1]:
-            wide = np.full((len(self._table), max(width, 2 * self._table.shape[1])), -1, np.int32)
-            wide[:, :self._table.shape[1]] = self._table
-            self._table = wide
-
-    def _upload(self, *parts: np.ndarray) -> torch.Tensor:
-        """int32 arrays, one after the other, on the GPU (torch keeps the pinned memory until
-        the copy is done)."""
-        self._check_capture()
-        host = torch.empty(sum(p.size for p in parts), dtype=torch.int32, pin_memory=True)
-        np.concatenate([p.reshape(-1) for p in parts], out=host.numpy(), casting="unsafe")
-        with torch.cuda.device(self.device):
-            return host.to(self.device, non_blocking=True)
+    def _done(self, what: str, y):
+        """What a native call returned, unless that is a status: then raise it."""
+        if y.__class__ is int:
+            self._t.refuse(what, y)
+        return y
 
     def _check_capture(self) -> None:
         with torch.cuda.device(self.device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("PagedKVCache: the bookkeeping cannot be captured into a graph")
 
-    def tables(self, seqs) -> tuple[torch.Tensor, torch.Tensor]:
-        """(table [B, width] int32, lens [B] int32) on the GPU, as ``paged_attn`` takes them;
-        entries past a sequence's pages are -1."""
-        ids = self._ids(seqs, distinct=False)
-        width = int(self._held[ids].max(initial=0))
-        flat = self._upload(self._table[ids, :width], self._len[ids])
-        n = len(ids) * width
-        return flat[:n].view(len(ids), width), flat[n:]
+    def _upload(self, *parts: np.ndarray) -> torch.Tensor:
+        """int32 arrays, one after the other, on the GPU (torch keeps the pinned memory until
+        the copy is done)."""
+        host = torch.empty(sum(p.size for p in parts), dtype=torch.int32, pin_memory=True)
+        np.concatenate([p.reshape(-1) for p in parts], out=host.numpy())
+        with torch.cuda.device(self.device):
+            return host.to(self.device, non_blocking=True)
 
-    def slots(self, seqs, first, count) -> torch.Tensor:
-        """Pool rows (device int32) of rows first[s] .. first[s] + count[s] - 1 of each
-        sequence, one sequence after the other."""
-        ids = self._ids(seqs, distinct=False)
-        lo, n = self._counts(first, ids), self._counts(count, ids)
-        if (lo + n > self._len[ids]).any():
-            raise ValueError("PagedKVCache: rows past a sequence's end")
-        return self._upload(self._rows(ids, lo, n))
-
-    def _rows(self, ids, lo, n) -> np.ndarray:
-        s = np.repeat(ids, n)
-        j = np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n) + np.repeat(lo, n)
-        return self._table[s, j // self.page].astype(np.int64) * self.page + j % self.page
+    def _move(self) -> None:
+        """Enqueue the moves of the call just made."""
+        groups, moves = self._t.moves()
+        if len(groups) == 1:
+            return
+        flat = self._upload(groups, moves)
+        bases, HK, D, sh, sn, cap = self._pool
+        with torch.cuda.device(self.device):
+            rc = _lib.lib().rspx_kv_move(bases.data_ptr(), bases.numel(), HK, D, sh, sn, cap, flat.data_ptr(),
+                                         len(groups) - 1, flat.data_ptr() + 4 * len(groups), len(moves),
+                                         _lib.stream_ptr(bases.device))
+        _lib.check("rspx_kv_move", rc)
 
     # ------------------------------------------------------------------ sequences
 
     def add(self, lengths) -> list[int]:
         """New sequences of ``lengths`` rows each, whose content the caller writes."""
-        n = np.asarray(list(lengths), dtype=np.int64)
-        if n.size and n.min() < 0:
-            raise ValueError("PagedKVCache: counts must be >= 0")
-        ids, need = self._new_ids(len(n)), -(-n // self.page)
-        pages = self._take(int(need.sum()))
-        self._widen(int(need.max(initial=0)))
-        self._give(ids, np.zeros_like(need), need, pages)
-        self._len[ids] = n
-        return ids.tolist()
-
-    def _give(self, ids, held, need, pages) -> None:
-        """Sequence ids[i] gets need[i] of ``pages`` after its held[i] ones."""
-        s = np.repeat(ids, need)
-        at = np.arange(len(s)) - np.repeat(np.cumsum(need) - need, need) + np.repeat(held, need)
-        self._table[s, at] = pages
-        self._refs[pages] += 1
-        self._held[ids] = held + need
+        return self._t.add(lengths)
 
     def extend(self, seqs, n=1) -> None:
         """Room for ``n`` (one number, or one per sequence) further rows of each sequence, whose
         content the caller writes.  A begun page that is shared is copied first."""
-        ids = self._ids(seqs)
-        n = self._counts(n, ids)
-        new = self._len[ids] + n
-        need = np.maximum(-(-new // self.page) - self._held[ids], 0)
-        own = self._shared(ids, self._len[ids], new)
-        if len(own[0]):
+        y = _lib.calls().pages_extend(self._t.handle, seqs, n, *self._pool)
+        if y is None:
             self._check_capture()
-        pages = self._take(int(need.sum()) + len(own[0]))
-        self._widen(int((self._held[ids] + need).max(initial=0)))
-        self._own(own, pages[:len(own[0])])
-        self._give(ids, self._held[ids], need, pages[len(own[0]):])
-        self._len[ids] = new
-
-    def _shared(self, ids, lo, hi) -> tuple[np.ndarray, np.ndarray]:
-        """(sequence, place) of the held pages with rows in [lo, hi) that others hold too."""
-        first, last = lo // self.page, np.minimum(-(-hi // self.page), self._held[ids])
-        n = np.where(hi > lo, np.maximum(last - first, 0), 0)
-        s = np.repeat(ids, n)
-        at = np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n) + np.repeat(first, n)
-        keep = self._refs[self._table[s, at]] > 1
-        return s[keep], at[keep]
-
-    def _own(self, own, pages) -> None:
-        """Give each (sequence, place) a page of its own, with the rows of the one it shares."""
-        s, at = own
-        if not len(s):
-            return
-        old = self._table[s, at].astype(np.int64)
-        rows = np.clip(self._len[s] - at * self.page, 0, self.page)
-        self._move(old * self.page, pages * self.page, rows)
-        np.subtract.at(self._refs, old, 1)
-        self._refs[pages] += 1
-        self._table[s, at] = pages
+            self._t.extend(seqs, n)
+            self._move()
+        else:
+            self._done("extend", y)
 
     def fork(self, seqs, copies: int = 1) -> list[int]:
         """``copies`` new sequences with the content of each of ``seqs``, those of the first one
         first.  Full pages are shared; the rows of a begun page are copied."""
-        ids = self._ids(seqs, distinct=False)
-        if copies < 0:
-            raise ValueError("PagedKVCache: counts must be >= 0")
-        src = np.repeat(ids, copies)
-        new, n = self._new_ids(len(src)), self._len[src]
-        full, part = n // self.page, n % self.page
-        begun = np.flatnonzero(part)
-        if len(begun):
+        y = _lib.calls().pages_fork(self._t.handle, seqs, copies, *self._pool)
+        if y is None:
             self._check_capture()
-        pages = self._take(len(begun))
-        width = int((full + (part > 0)).max(initial=0))
-        rows = self._table[src, :width]
-        rows[np.arange(width)[None] >= full[:, None]] = -1
-        np.add.at(self._refs, rows[rows >= 0], 1)
-        self._refs[pages] += 1
-        self._move(self._table[src[begun], full[begun]].astype(np.int64) * self.page, pages * self.page, part[begun])
-        rows[begun, full[begun]] = pages
-        self._table[new] = -1
-        self._table[new, :width] = rows
-        self._held[new] = full + (part > 0)
-        self._len[new] = n
-        return new.tolist()
+            y = self._t.fork(seqs, copies)
+            self._move()
+        return self._done("fork", y)
 
     def compact(self, seqs, starts, paths) -> None:
         """The accepted path of each sequence's verified trie (kv_buffer.KVCache.compact for
         many sequences): rows start + path[i] move to start + i, and the sequence ends
         after them.  ``starts``: one number or one per sequence; paths increase.  The pages
         behind the new end stay with the sequence for its next rows (``trim``)."""
-        ids = self._ids(seqs)
-        starts = self._counts(starts, ids)
-        paths = [np.asarray(list(p), dtype=np.int64) for p in paths]
-        if len(paths) != len(ids):
-            raise ValueError("PagedKVCache: one path per sequence")
-        n = np.array([len(p) for p in paths], dtype=np.int64)
-        path = np.concatenate(paths) if len(paths) else np.zeros(0, np.int64)
-        last = np.cumsum(n)
-        seq = np.repeat(np.arange(len(ids)), n)
-        inner = np.ones(len(path), bool)
-        inner[(last - n)[n > 0]] = False                       # a path's first node follows none
-        if (path < 0).any() or (np.diff(path, prepend=0)[inner] <= 0).any():
-            raise ValueError("PagedKVCache: paths must increase")
-        end = starts.copy()
-        end[n > 0] += path[last[n > 0] - 1] + 1
-        if (end > self._len[ids]).any():
-            raise ValueError("PagedKVCache: a path runs past its sequence's end")
-        to = np.arange(len(path)) - np.repeat(last - n, n)
-        away = path != to                                      # the rows that do move
-        lo = starts + np.bincount(seq[~away], minlength=len(ids)).astype(np.int64)
-        own = self._shared(ids, lo, starts + n)
-        if len(own[0]) or away.any():
+        y = _lib.calls().pages_compact(self._t.handle, seqs, starts, paths, *self._pool)
+        if y is None:
             self._check_capture()
-        self._own(own, self._take(len(own[0])))
-        if away.any():
-            s, base = ids[seq[away]], starts[seq[away]]
-            a, b = base + path[away], base + to[away]
-            moves = np.stack((self._table[s, a // self.page].astype(np.int64) * self.page + a % self.page,
-                              self._table[s, b // self.page].astype(np.int64) * self.page + b % self.page), 1)
-            count = np.bincount(seq[away], minlength=len(ids))
-            self._launch(moves, count[count > 0])
-        self._len[ids] = starts + n
+            self._t.compact(seqs, starts, paths)
+            self._move()
+        else:
+            self._done("compact", y)
 
     def trim(self, seqs) -> None:
         """Give back the pages past each sequence's end."""
-        ids = self._ids(seqs)
-        self._drop(ids, -(-self._len[ids] // self.page))
+        self._t.trim(seqs)
 
     def free(self, seqs) -> None:
         """Forget the sequences and give back their pages."""
-        ids = self._ids(seqs)
-        self._drop(ids, np.zeros(len(ids), np.int64))
-        self._len[ids] = -1
-
-    def _drop(self, ids, keep) -> None:
-        width = int(self._held[ids].max(initial=0))
-        rows, place = self._table[ids, :width], np.arange(width)[None]
-        gone = (place >= keep[:, None]) & (place < self._held[ids][:, None])
-        np.subtract.at(self._refs, rows[gone], 1)
-        rows[gone] = -1
-        self._table[ids, :width] = rows
-        self._held[ids] = np.minimum(keep, self._held[ids])
+        self._t.free(seqs)
 
     # ------------------------------------------------------------------ rows
 
-    def _move(self, src, dst, rows) -> None:
-        """rows[i] rows from pool row src[i] to dst[i], each run a group of its own."""
-        src, dst, rows = src[rows > 0], dst[rows > 0], rows[rows > 0]
-        if len(rows):
-            j = np.arange(int(rows.sum())) - np.repeat(np.cumsum(rows) - rows, rows)
-            self._launch(np.stack((np.repeat(src, rows) + j, np.repeat(dst, rows) + j), 1), rows)
+    def tables(self, seqs) -> tuple[torch.Tensor, torch.Tensor]:
+        """(table [B, width] int32, lens [B] int32) on the GPU, as ``paged_attn`` takes them;
+        entries past a sequence's pages are -1."""
+        y = _lib.calls().pages_tables(self._t.handle, seqs, *self._pool)
+        if y is not None:
+            return self._done("tables", y)
+        self._check_capture()
+        table, lens = self._t.table(seqs)
+        flat = self._upload(table, lens)
+        return flat[:table.size].view(table.shape), flat[table.size:]
 
-    def _launch(self, moves: np.ndarray, count: np.ndarray) -> None:
-        k0 = self.k[0]
-        with torch.cuda.device(self.device):
-            flat = self._upload(np.concatenate(([0], np.cumsum(count))), moves)
-            rc = _lib.lib().rspx_kv_move(
-                self.bases.data_ptr(), 2 * self.layers, self.HK, self.D, k0.stride(0), k0.stride(1),
-                self.pages * self.page, flat.data_ptr(), len(count), flat.data_ptr() + 4 * (len(count) + 1), len(moves),
-                _lib.stream_ptr(self.device))
-        _lib.check("rspx_kv_move", rc)
+    def slots(self, seqs, first, count) -> torch.Tensor:
+        """Pool rows (device int32) of rows first[s] .. first[s] + count[s] - 1 of each
+        sequence, one sequence after the other."""
+        y = _lib.calls().pages_slots(self._t.handle, seqs, first, count, *self._pool)
+        if y is not None:
+            return self._done("slots", y)
+        self._check_capture()
+        return self._upload(self._t.slots(seqs, first, count))
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """k / v [T, HK, D] bf16 of one layer to the pool rows ``slots`` [T] (device int32, as

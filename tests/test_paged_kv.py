@@ -10,106 +10,185 @@ import torch
 BF = torch.bfloat16
 
 
-class _Dry:
-    """A PagedKVCache without device work: the moves are recorded instead of launched."""
-
-    def __new__(cls, pages, page, sequences=64):
-        from respect_amd.decoding.paged_kv import PagedKVCache
-
-        class Dry(PagedKVCache):
-            def _launch(self, moves, count):
-                self.moves.append((moves.copy(), count.copy()))
-
-            def _upload(self, *parts):
-                return torch.from_numpy(np.concatenate([p.reshape(-1) for p in parts]).astype(np.int32))
-
-            def _check_capture(self):
-                pass
-        c = Dry(1, 1, 8, pages, page=page, device="cpu", sequences=sequences)
-        c.moves = []
-        return c
+def _table(pages, page, sequences=64):
+    from respect_amd import _lib
+    from respect_amd.decoding.paged_kv import PageTable
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    return PageTable(pages, page, sequences)
 
 
-def _pages(c, s):
-    return c._table[s, :c._held[s]].tolist()
+def _pages(t, s):
+    return [p for p in t.table([s])[0][0].tolist() if p >= 0]
+
+
+def _moves(t):
+    groups, moves = t.moves()
+    assert (np.diff(groups) > 0).all() and groups[0] == 0 and groups[-1] == len(moves)
+    return moves.tolist(), np.diff(groups).tolist()
 
 
 def test_add_extend_fork_free():
-    c = _Dry(12, 4)
-    a, b = c.add([9, 4])
-    assert (a, b) == (0, 1) and _pages(c, a) == [0, 1, 2] and _pages(c, b) == [3] and c.free_pages == 8
-    c.extend([b], 1)
-    assert _pages(c, b) == [3, 4] and c.length(b) == 5
-    c.extend([a, b], [3, 0])
-    assert _pages(c, a) == [0, 1, 2] and c.length(a) == 12 and not c.moves
-    f = c.fork([b, a], 2)
+    t = _table(12, 4)
+    a, b = t.add([9, 4])
+    assert (a, b) == (0, 1) and _pages(t, a) == [0, 1, 2] and _pages(t, b) == [3] and t.available == 8
+    t.extend([b], 1)
+    assert _pages(t, b) == [3, 4] and t.length(b) == 5
+    t.extend([a, b], [3, 0])
+    assert _pages(t, a) == [0, 1, 2] and t.length(a) == 12 and _moves(t) == ([], [])
+    f = t.fork([b, a], 2)
     assert f == [2, 3, 4, 5]
-    assert [_pages(c, s) for s in f] == [[3, 5], [3, 6], [0, 1, 2], [0, 1, 2]]
-    moves, count = c.moves.pop()
-    assert moves.tolist() == [[16, 20], [16, 24]] and count.tolist() == [1, 1] and not c.moves
-    assert c.free_pages == 5
-    c.free([a, f[0]])
-    assert c.free_pages == 6 and c.add([1]) == [0] and _pages(c, 0) == [5]
+    assert [_pages(t, s) for s in f] == [[3, 5], [3, 6], [0, 1, 2], [0, 1, 2]]
+    assert _moves(t) == ([[16, 20], [16, 24]], [1, 1])
+    assert t.available == 5
+    t.free([a, f[0]])
+    assert _moves(t) == ([], [])
+    assert t.available == 6 and t.add([1]) == [0] and _pages(t, 0) == [5]
     with pytest.raises(ValueError):
-        c.length(f[0])
-    table, lens = c.tables([b, f[2], f[1]])
-    assert table.tolist() == [[3, 4, -1], [0, 1, 2], [3, 6, -1]] and lens.tolist() == [5, 12, 5]
-    assert c.slots([f[2], b], [3, 0], [2, 5]).tolist() == [3, 4, 12, 13, 14, 15, 16]
+        t.length(f[0])
+    table, lens = t.table([b, f[2], f[1], b])
+    assert table.tolist() == [[3, 4, -1], [0, 1, 2], [3, 6, -1], [3, 4, -1]] and lens.tolist() == [5, 12, 5, 5]
+    assert t.slots([f[2], b], [3, 0], [2, 5]).tolist() == [3, 4, 12, 13, 14, 15, 16]
+    assert t.table([])[0].shape == (0, 0) and t.slots([], 0, 0).tolist() == []
 
 
 def test_compact_and_shared_pages():
-    c = _Dry(20, 4)
-    a, = c.add([13])
-    c.compact([a], 6, [[0, 2, 5]])               # rows 8, 11 -> 7, 8; row 6 stays
-    moves, count = c.moves.pop()
-    assert moves.tolist() == [[8, 7], [11, 8]] and count.tolist() == [2]
-    assert c.length(a) == 9 and _pages(c, a) == [0, 1, 2, 3]
-    c.trim([a])
-    assert _pages(c, a) == [0, 1, 2]
-    b, = c.fork([a])                             # pages 0, 1 shared, the begun one copied
-    assert _pages(c, b) == [0, 1, 3]
-    assert c.moves.pop()[0].tolist() == [[8, 12]]
-    c.compact([b], 5, [[1]])                     # row 6 -> 5 of a page that a holds too
-    own, path = c.moves
-    assert own[0].tolist() == [[4, 16], [5, 17], [6, 18], [7, 19]] and path[0].tolist() == [[18, 17]]
-    assert _pages(c, b) == [0, 4, 3] and _pages(c, a) == [0, 1, 2] and c.length(b) == 6
-    c.moves.clear()
-    d, = c.fork([a])
-    c.compact([d], 2, [[]])                      # cut back into a shared page
-    assert c.length(d) == 2
-    c.moves.clear()
-    c.extend([d], 3)
-    new = _pages(c, d)[0]
-    assert new != 0 and c.moves.pop()[0].tolist() == [[0, 4 * new], [1, 4 * new + 1]]
-    assert c._refs[0] == 2 and c.length(d) == 5
-    c.free([a, b, d])
-    assert c.free_pages == 20
+    t = _table(20, 4)
+    a, = t.add([13])
+    t.compact([a], 6, [[0, 2, 5]])               # rows 8, 11 -> 7, 8; row 6 stays
+    assert _moves(t) == ([[8, 7], [11, 8]], [2])
+    assert t.length(a) == 9 and _pages(t, a) == [0, 1, 2, 3]
+    t.trim([a])
+    assert _pages(t, a) == [0, 1, 2]
+    b, = t.fork([a], 1)                          # pages 0, 1 shared, the begun one copied
+    assert _pages(t, b) == [0, 1, 3] and _moves(t)[0] == [[8, 12]]
+    t.compact([b], 5, [[1]])                     # row 6 -> 5 of a page that a holds too: a new page
+    assert _moves(t) == ([[6, 17], [4, 16]], [2])
+    assert _pages(t, b) == [0, 4, 3] and _pages(t, a) == [0, 1, 2] and t.length(b) == 6
+    d, = t.fork([a], 1)
+    t.compact([d], 2, [[]])                      # cut back into a shared page
+    assert t.length(d) == 2 and _moves(t) == ([], [])
+    t.extend([d], 3)
+    new = _pages(t, d)[0]
+    assert new != 0 and _moves(t)[0] == [[0, 4 * new], [1, 4 * new + 1]] and t.length(d) == 5
+    t.free([a, b, d])
+    assert t.available == 20
+
+
+def test_all_who_share_a_page_move_away_from_it():
+    """Both holders of a page compact into it in one call: neither writes what the other reads."""
+    t = _table(9, 4)
+    a, = t.add([8])
+    b, = t.fork([a], 1)
+    t.compact([a, b], [0, 4], [[1, 2, 7], [3]])
+    moves, count = _moves(t)
+    assert count == [3, 1]
+    old = set(range(8))
+    assert {m[0] for m in moves} <= old and not {m[1] for m in moves} & old
+    assert t.available == 9 - 3 - 1 and sorted(_pages(t, a) + _pages(t, b)) == [0, 1, 2, 3]
+    assert t.available + len(set(_pages(t, a) + _pages(t, b))) == 9
+    t.free([a, b])
+    assert t.available == 9
 
 
 def test_failures_change_nothing():
-    c = _Dry(6, 4, sequences=3)
-    a, b = c.add([7, 9])
-    before = (c._refs.copy(), c._table.copy(), c._held.copy(), c._len.copy())
+    t = _table(6, 4, sequences=3)
+    a, b = t.add([7, 9])
+    f = []
 
-    def same():
-        return all((x == y).all() for x, y in zip(before, (c._refs, c._table, c._held, c._len)))
-    for call in (lambda: c.add([5]), lambda: c.extend([a, b], 8), lambda: c.fork([a], 2), lambda: c.add([0, 0])):
+    def state():
+        live = [a, b] + f
+        table, lens = t.table(live)
+        return table.tolist(), lens.tolist(), t.available
+    before = state()
+    for call in (lambda: t.add([5]), lambda: t.extend([a, b], 8), lambda: t.fork([a], 2), lambda: t.add([0, 0]),
+                 lambda: t.extend([a], 1 << 40), lambda: t.add([1 << 40]), lambda: t.fork([a], 1 << 30)):
         with pytest.raises(RuntimeError):
             call()
-        assert same()
-    for call in (lambda: c.add([-1]), lambda: c.extend([a], -1), lambda: c.extend([a, a]), lambda: c.free([a, a]),
-                 lambda: c.free([2]), lambda: c.free([-1]), lambda: c.extend([99]), lambda: c.fork([a], -1),
-                 lambda: c.compact([a], 3, [[0, 4]]), lambda: c.compact([a], 3, [[1, 1]]),
-                 lambda: c.compact([a, b], 3, [[0]]), lambda: c.compact([a], 8, [[]]), lambda: c.compact([a], 0, [[-1]]),
-                 lambda: c.slots([a], 5, 3), lambda: c.compact([a, b], [0, 1], [[2, 1], [0]])):
+        assert state() == before
+    for call in (lambda: t.add([-1]), lambda: t.extend([a], -1), lambda: t.extend([a, a], 1), lambda: t.free([a, a]),
+                 lambda: t.free([2]), lambda: t.free([-1]), lambda: t.extend([99], 1), lambda: t.fork([a], -1),
+                 lambda: t.compact([a], 3, [[0, 4]]), lambda: t.compact([a], 3, [[1, 1]]),
+                 lambda: t.compact([a, b], 3, [[0]]), lambda: t.compact([a], 8, [[]]), lambda: t.compact([a], 0, [[-1]]),
+                 lambda: t.slots([a], 5, 3), lambda: t.slots([a], 8, 0), lambda: t.compact([a, b], [0, 1], [[2, 1], [0]]),
+                 lambda: t.extend([a, b], [1]), lambda: t.free([1 << 40]), lambda: t.length(-1), lambda: t.length(1 << 40)):
         with pytest.raises(ValueError):
             call()
-        assert same()
-    for bad in (dict(pages=0), dict(page=3), dict(pages=1 << 28), dict(head_dim=12), dict(layers=0)):
+        assert state() == before
+    assert t.fork([a, b], 0) == [] and t.add([]) == [] and state() == before
+    # A full page is shared without any to spare; a begun one is not.
+    c, = t.fork([b], 1)
+    f.append(c)
+    with pytest.raises(RuntimeError):
+        t.extend([a], 2)
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    for bad in (dict(pages=0), dict(page=3), dict(pages=1 << 28), dict(head_dim=12), dict(layers=0), dict(sequences=0)):
         with pytest.raises(ValueError):
-            from respect_amd.decoding.paged_kv import PagedKVCache
             PagedKVCache(**{**dict(layers=1, kv_heads=1, head_dim=8, pages=4, page=16, device="cpu"), **bad})
-    assert c.fork([a, b], 0) == [] and c.add([]) == [] and same()
+
+
+def test_random_bookkeeping_keeps_count():
+    """Random calls: every page is held by as many as the count says, and never written by a move
+    that another sequence's rows depend on."""
+    rng = random.Random(3)
+    t = _table(40, 4, sequences=12)
+    live = {}                                    # sequence -> its rows' tokens
+    pool, fresh = [None] * 160, iter(range(10 ** 9))
+
+    def run_moves():
+        groups, moves = t.moves()
+        before = list(pool)                      # different groups: in any order
+        for g in rng.sample(range(len(groups) - 1), len(groups) - 1):
+            mine = moves[groups[g]:groups[g + 1]].tolist()
+            for i, (src, dst) in enumerate(mine):
+                assert all(dst != s for s, _ in mine[i + 1:])
+                assert pool[src] == before[src] or any(dst2 == src for _, dst2 in mine[:i])
+                pool[dst] = pool[src]
+    for _ in range(400):
+        some = rng.sample(sorted(live), rng.randint(0, len(live)))
+        what = rng.choice(["add", "extend", "fork", "compact", "compact", "trim", "free"])
+        try:
+            if what == "add":
+                n = [rng.randint(0, 11) for _ in range(2)]
+                for s, k in zip(t.add(n), n):
+                    live[s] = [next(fresh) for _ in range(k)]
+                    for slot, x in zip(t.slots([s], 0, k), live[s]):
+                        pool[slot] = x
+            elif what == "extend":
+                n = [rng.randint(0, 6) for _ in some]
+                t.extend(some, n)
+                run_moves()
+                for s, k in zip(some, n):
+                    new = [next(fresh) for _ in range(k)]
+                    for slot, x in zip(t.slots([s], len(live[s]), k), new):
+                        pool[slot] = x
+                    live[s] = live[s] + new
+            elif what == "fork":
+                for i, s in enumerate(t.fork(some[:2], 2)):
+                    live[s] = list(live[some[i // 2]])
+                run_moves()
+            elif what == "compact":
+                starts = [rng.randint(0, len(live[s])) for s in some]
+                paths = [sorted(rng.sample(range(len(live[s]) - a), rng.randint(0, len(live[s]) - a))) for s, a in zip(some, starts)]
+                t.compact(some, starts, paths)
+                run_moves()
+                for s, a, q in zip(some, starts, paths):
+                    live[s] = live[s][:a] + [live[s][a + i] for i in q]
+            elif what == "trim":
+                t.trim(some)
+            else:
+                t.free(some[:1])
+                for s in some[:1]:
+                    del live[s]
+        except RuntimeError:
+            pass                                 # full
+        held = set()
+        for s, rows in live.items():
+            assert t.length(s) == len(rows) and [pool[x] for x in t.slots([s], 0, len(rows))] == rows
+            held |= set(_pages(t, s))
+        assert t.available == 40 - len(held)
+    t.free(list(live))
+    assert t.available == 40
 
 
 def test_c_refusals():
@@ -131,6 +210,15 @@ def test_c_refusals():
     assert write(T=-1) == -1 and write(cap=-1) == -1 and write(p=0) == -1 and write(slots=0) == -1
     assert write(D=60) == -2 and write(p=8) == -4 and write(s=68) == -4
     assert write(T=0) == 0
+    assert L.rspx_pages_new(0, 4, 1) is None and L.rspx_pages_new(4, 3, 1) is None and L.rspx_pages_new(4, 4, 0) is None
+    assert L.rspx_pages_new(1 << 28, 16, 1) is None
+    assert L.rspx_pages_add(None, None, 0, None) == -1 and L.rspx_pages_available(None) == -1
+    assert L.rspx_pages_length(None, 0) == -1
+    p = L.rspx_pages_new(4, 4, 2)
+    assert L.rspx_pages_add(p, None, 1, None) == -1 and L.rspx_pages_fork(p, None, 1, 1, None) == -1
+    assert L.rspx_pages_extend(p, None, -1, None) == -1 and L.rspx_pages_extend(p, None, 0, None) == 0
+    L.rspx_pages_delete(p)
+    L.rspx_pages_delete(None)
 
 
 class _Model:
@@ -141,11 +229,11 @@ class _Model:
 
     def check(self):
         c = self.c
-        pages = [p for s in self.rows for p in _pages(c, s)]
-        assert (np.bincount(np.array(pages, dtype=int), minlength=c.pages) == c._refs).all()
+        table, _ = c.tables(list(self.rows))
+        assert c.free_pages == c.pages - len(set(table[table >= 0].tolist()))
         for s, want in self.rows.items():
             n = c.length(s)
-            assert n == want.shape[3] and c._held[s] >= -(-n // c.page)
+            assert n == want.shape[3]
             slots = c.slots([s], 0, n).long()
             got = torch.stack([torch.stack((k[:, slots], v[:, slots])) for k, v in zip(c.k, c.v)])
             assert torch.equal(got.cpu(), want), f"sequence {s}"
@@ -231,7 +319,7 @@ def test_long_groups_in_order_and_skipped_slots():
     before = [t.clone() for t in c.k + c.v]
     flat = torch.tensor([0, 4, -5, 3, 3, 1 << 20, 1024, 0, 7, 5], dtype=torch.int32, device="cuda")
     k0 = c.k[0]
-    assert _lib.lib().rspx_kv_move(c.bases.data_ptr(), 4, 2, 128, k0.stride(0), k0.stride(1), 1024, flat.data_ptr(), 1,
+    assert _lib.lib().rspx_kv_move(c._pool[0].data_ptr(), 4, 2, 128, k0.stride(0), k0.stride(1), 1024, flat.data_ptr(), 1,
                                    flat.data_ptr() + 8, 4, _lib.stream_ptr(c.device)) == 0
     c.write(0, torch.ones(3, 2, 128, dtype=BF, device="cuda"), torch.ones(3, 2, 128, dtype=BF, device="cuda"),
             torch.tensor([-1, 1024, 9], dtype=torch.int32, device="cuda"))

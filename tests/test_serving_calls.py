@@ -75,3 +75,45 @@ def test_calls_equal_the_wrappers_own_path(monkeypatch):
             b = call()
         for y, z in zip(*(((a,), (b,)) if isinstance(a, torch.Tensor) else (a, b))):
             assert y.shape == z.shape and y.dtype == z.dtype and torch.equal(y, z)
+
+
+@pytest.mark.gpu
+def test_pages_calls_equal_the_wrappers_own_path(monkeypatch):
+    """The same run of bookkeeping calls natively and through the wrapper: pools, tables, slots and
+    errors are the same; tuples, ranges and numpy numbers are left to the wrapper."""
+    import numpy as np
+    from respect_amd import _lib
+    from respect_amd.decoding.paged_kv import PagedKVCache
+
+    class Leave:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    def play():
+        c = PagedKVCache(2, 2, 64, pages=30, page=4, sequences=9)
+        g = torch.Generator(device="cuda")
+        g.manual_seed(0)
+        for t in c.k + c.v:
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        out = []
+        seqs = c.add([9, 4, 13])
+        out.append(c.fork(seqs, 2))
+        c.extend(out[0][:2], [3, 1])
+        c.extend(range(3))
+        c.compact(seqs, [1, 0, 6], [[0, 2, 5], [], [3, 4]])
+        c.compact(np.array(out[0][:1]), 2, [range(1, 4)])
+        out += [c.slots(seqs, 0, [2, 0, 3]).tolist(), c.slots(tuple(seqs), [1, 0, 1], 0).tolist()]
+        table, lens = c.tables(seqs + out[0])
+        out += [table.tolist(), lens.tolist(), c.free_pages]
+        for call in (lambda: c.fork([77]), lambda: c.fork(seqs, 9), lambda: c.extend(seqs, -1), lambda: c.extend(seqs, 500),
+                     lambda: c.compact(seqs, 0, [[0]]), lambda: c.compact(seqs, 0, [[9], [], []]), lambda: c.tables([-1]),
+                     lambda: c.slots(seqs, 0, 99), lambda: c.slots([seqs[0]], -1, 1), lambda: c.fork([1 << 70])):
+            with pytest.raises((ValueError, RuntimeError, OverflowError)) as e:
+                call()
+            out.append(type(e.value))
+        return out, [t.clone() for t in c.k + c.v]
+    a, ta = play()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "_calls", Leave())
+        b, tb = play()
+    assert a == b and all(torch.equal(x, y) for x, y in zip(ta, tb))
