@@ -4,7 +4,11 @@
 //                  a forked sequence, the accepted path of a verified trie
 //   rspx_kv_write  new K and V rows of one layer to their slots
 //
-// Copies only; what bounds them is the bytes of the rows, read once and written once.
+// Copies only; what bounds them is the bytes of the rows.  kv_move stores past the caches, so
+// that the copies of one row do not push it out between them: 32 sequences forked 4 times
+// (24 layers, 8 heads of 128, 69 MB read and 277 written) 79 us, 4.4 TB/s; 125 with ordinary
+// stores, 82 with four units per thread, 130 with loads past the caches too.  32 paths of 13
+// moved rows (82 MB): 14.4 us.
 #include "common.h"
 #include "respect_amd.h"
 
@@ -13,7 +17,7 @@ namespace rspx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;            // 16-byte units a thread holds at once
+constexpr int kBatch = 8;            // 16-byte units a thread holds at once
 
 // Workgroup (group, head, tensor): the group's moves in order, kThreads * kBatch units of
 // 16 bytes at a time, all of them read before any is written.  A slot outside [0, cap) is
@@ -43,7 +47,7 @@ __global__ __launch_bounds__(kThreads) void kv_move_kernel(const uint64_t* bases
     __syncthreads();   // the batch has been read
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      if (to[i]) *reinterpret_cast<u32x4*>(to[i]) = buf[i];
+      if (to[i]) __builtin_nontemporal_store(buf[i], reinterpret_cast<u32x4*>(to[i]));
   }
 }
 
