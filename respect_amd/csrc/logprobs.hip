@@ -12,11 +12,14 @@
 // The best pairs are a set under a total order (value, lowest index first, NaN the
 // largest), so their selection may take any order.  Each wave keeps a list of candidates in
 // LDS and the bound that a pair must pass to enter it, the top-th best found so far: most
-// steps add few or none.  Where a step would add too many (the first one, rising scores, ties) the
-// top-th best of the lanes' best pairs bounds them first: at most 16 of each of `top` lanes pass.
-// Lists are cut to their best by counting.
+// steps add few or none.  Where a step would add many (the first one, rising scores, ties) they
+// are bounded first by what the best pairs of `top` lanes pass, found to 16 bits of the value by
+// a search over ballots, or, where ties let more through than the list has room for, exactly:
+// at most 16 of each of `top` lanes then pass.  Lists are cut to their best by counting.
 //
-// What bounds it: the read of the scores.
+// What bounds it: the read of the scores, where there are many (1500 rows of 151936, top 5:
+// 911 MB in 190 us, 4.8 TB/s; torch's sum over them reads 4.0); for one row two launches and
+// the selection's dependent steps (6.5 us without alternatives, 10.0 with one, 14.2 with 20).
 #include "common.h"
 #include "respect_amd.h"
 
@@ -131,35 +134,53 @@ __device__ __forceinline__ uint64_t prune(uint64_t* list, int& n, int top) {
   return n < top ? 0 : best[top - 1];
 }
 
+// How many of the wave's keys pass the bound.
+__device__ __forceinline__ int passing(const uint64_t (&key)[kPer], uint64_t bound) {
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] > bound));
+  return count;
+}
+
 // Adds the wave's step x (columns j0 + 256 (i / 4) + i % 4, j0 the lane's own) to its list.
 __device__ __forceinline__ void enlist(const float (&x)[kPer], int j0, int V, int top, uint64_t* list, int& n,
                                        uint64_t& bound) {
   uint64_t key[kPer];
-  int count = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int j = j0 + 256 * (i / 4) + i % 4;
     key[i] = j < V ? pair_key(x[i], j) : 0;
-    count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] > bound));
   }
-  if (n + count > 3 * top) {   // many: the top-th best of the lanes' best bounds them
-    if (n > top) bound = prune(list, n, top);
+  if (n + passing(key, bound) > 3 * top) {
+    // Many: bounded by what the best pairs of `top` lanes pass, to 16 bits of the value.
     uint64_t best = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) best = key[i] > best ? key[i] : best;
-    int r = 0;
-#pragma unroll 16
-    for (int l = 0; l < 64; ++l) {
-      const uint64_t o = (uint64_t)__builtin_amdgcn_readlane((int)(best >> 32), l) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)best, l);
-      r += o > best;
+    uint32_t p = 0;
+    for (int b = 15; b >= 0; --b) {
+      const uint32_t t = p | 1u << b;
+      if (__builtin_popcountll(__builtin_amdgcn_ballot_w64((uint32_t)(best >> 48) >= t)) >= top) p = t;
     }
-    const uint64_t at = __builtin_amdgcn_ballot_w64(r == top - 1 && best != 0);   // keys differ: one lane at most
-    if (at) {
-      const int l = __builtin_ctzll(at);
-      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(best >> 32), l) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)best, l);
-      if (o - 1 > bound) bound = o - 1;
+    if (p && ((uint64_t)p << 48) - 1 > bound) bound = ((uint64_t)p << 48) - 1;
+    if (n + passing(key, bound) > (kPer + 1) * top) {      // still too many: by the top-th best pair of the lanes
+      if (n > top) {
+        const uint64_t last = prune(list, n, top);
+        if (last > bound) bound = last;
+      }
+      int r = 0;
+#pragma unroll 4
+      for (int l = 0; l < 64; ++l) {
+        const uint64_t o = (uint64_t)__builtin_amdgcn_readlane((int)(best >> 32), l) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)best, l);
+        r += o > best;
+      }
+      const uint64_t at = __builtin_amdgcn_ballot_w64(r == top - 1 && best != 0);   // keys differ: one lane at most
+      if (at) {
+        const int l = __builtin_ctzll(at);
+        const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(best >> 32), l) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)best, l);
+        if (o - 1 > bound) bound = o - 1;
+      }
     }
   }
 #pragma unroll
@@ -171,7 +192,7 @@ __device__ __forceinline__ void enlist(const float (&x)[kPer], int j0, int V, in
       n += __builtin_popcountll(in);
     }
   }
-  if (n > 2 * top || bound == 0) {
+  if (n > 2 * top) {
     const uint64_t last = prune(list, n, top);
     if (last > bound) bound = last;
   }
@@ -256,23 +277,24 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogArgs A) {
     }
   }
   if constexpr (TOP) {
-    if (n > A.top) prune(list, n, A.top);
+    if (n > A.top && A.top > 24) prune(list, n, A.top);    // ranking long lists costs more than this
     if (lane == 0) counts[w] = n;
     __syncthreads();
     // The best of the four waves' lists, ranked by counting.
     uint64_t* out = A.best + (row * A.parts + blockIdx.x) * A.top;
-    int all = 0;
-    for (int k = 0; k < 4; ++k) all += counts[k];
-    for (int i = threadIdx.x; i < 4 * A.top; i += kThreads) {
-      const int from = i / A.top, at = i % A.top;
-      if (at < counts[from]) {
-        const uint64_t key = lists[from * list_room(A.top) + at];
-        int r = 0;
-        for (int k = 0; k < 4; ++k)
+    const int room = list_room(A.top), all = counts[0] + counts[1] + counts[2] + counts[3];
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+      int from = 0, at = i;
+      for (int k = 0; k < 3; ++k)
+        if (from == k && at >= counts[k]) at -= counts[k], ++from;
+      const uint64_t key = lists[from * room + at];
+      int r = 0;
+      for (int k = 0; k < 4; ++k) {
+        const int m = counts[k];
 #pragma unroll 8
-          for (int j = 0; j < counts[k]; ++j) r += lists[k * list_room(A.top) + j] > key;
-        if (r < A.top) out[r] = key;
+        for (int j = 0; j < m; ++j) r += lists[k * room + j] > key;
       }
+      if (r < A.top) out[r] = key;
     }
     for (int i = all + threadIdx.x; i < A.top; i += kThreads) out[i] = 0;
   }
