@@ -26,8 +26,10 @@
 // What bounds it: the K/V bytes, read once, where there are enough of them (one sequence of
 // 131072 keys and five shorter ones, 32 / 8 heads of 128: 822 MB in 149 us, 5.5 TB/s; 64
 // sequences of up to 8000: 260 MB in 64 us); below that the chain of dependent reads --
-// lengths, table, K/V, the second launch's partial sums (13 us for one sequence of 4097).
-// Splits of 128 keys: 67 us instead of 64 for the batch; at most 64 splits: no difference.
+// lengths, table, K/V, the second launch's partial sums (13 us for one sequence of 4097, whose
+// 17 MB take 3.3 of them).  Splits of 128 keys: 67 us instead of 64 for the batch, of 512: 17
+// instead of 13 for the one; at most 64 splits, or two tiles per wave requested at once: no
+// difference.
 #include "common.h"
 #include "respect_amd.h"
 
@@ -50,12 +52,12 @@ constexpr float kNone = -1e30f;      // reference maximum before the first key
 
 // Keys per split of a sequence of n keys: a multiple of kSplitKeys.
 __host__ __device__ __forceinline__ int split_keys(int n) {
-  const int per = (int)(((int64_t)n + kMaxSplits - 1) / kMaxSplits);
-  return per <= kSplitKeys ? kSplitKeys : (per + kSplitKeys - 1) / kSplitKeys * kSplitKeys;
+  const unsigned per = ((unsigned)n + kMaxSplits - 1) / kMaxSplits;
+  return per <= kSplitKeys ? kSplitKeys : (int)((per + kSplitKeys - 1) / kSplitKeys * kSplitKeys);
 }
 __host__ __device__ __forceinline__ int split_count(int n) {
-  const int k = split_keys(n);
-  return (int)(((int64_t)n + k - 1) / k);
+  const unsigned k = (unsigned)split_keys(n);
+  return (int)(((unsigned)n + k - 1) / k);
 }
 // The most splits that any length up to n gives.
 __host__ __forceinline__ int split_bound(int64_t n) { return n >= (int64_t)kSplitKeys * kMaxSplits ? kMaxSplits : split_count((int)n); }
@@ -72,16 +74,20 @@ struct PagedArgs {
 };
 
 // first[b]: the splits of sequences before b (one for a sequence without any, whose rows
-// are written too); returns their number.  All 256 threads call it.
-__device__ __forceinline__ int list_items(const int* lens, int B, int64_t cap, int* first) {
+// are written too), length[b]: lens[b]; returns the number of splits.  All 256 threads call it.
+__device__ __forceinline__ int list_items(const int* lens, int B, int64_t cap, int* first, int* length) {
   __shared__ int waves[4];
   constexpr int kPer = kSeqs / 256;
   int cnt[kPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int b = threadIdx.x * kPer + i;
-    const int n = b < B ? lens[b] : 0;
-    cnt[i] = b >= B ? 0 : n <= 0 || n > cap ? 1 : split_count(n);
+    cnt[i] = 0;
+    if (b < B) {
+      const int n = lens[b];
+      length[b] = n;
+      cnt[i] = n <= 0 || n > cap ? 1 : split_count(n);
+    }
     sum += cnt[i];
   }
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -161,12 +167,12 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
   constexpr int VL = kTile * U / 64;                       // 16-byte loads of a V tile per lane
   __shared__ __align__(16) char stage[kWaves][kTile * D * 2];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
-  __shared__ int first[kSeqs + 1];
+  __shared__ int first[kSeqs + 1], length[kSeqs];
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, c16 = lane & 15, r4 = lane >> 4;
   const int64_t cap = (int64_t)A.width << A.shift;
-  const int items = list_items(A.lens, A.B, cap, first) * A.HK;
+  const int items = list_items(A.lens, A.B, cap, first, length) * A.HK;
   if ((int)blockIdx.x >= items) return;
 
   auto decode = [&](int i) {
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
     x.g = i % A.HK;
     x.b = find_seq(first, A.B, i / A.HK);
     x.split = i / A.HK - __builtin_amdgcn_readfirstlane(first[x.b]);
-    x.n = __builtin_amdgcn_readfirstlane(A.lens[x.b]);
+    x.n = __builtin_amdgcn_readfirstlane(length[x.b]);
     x.splits = x.t = x.tend = 0;
     if (x.n > 0 && x.n <= cap) {
       const int per = split_keys(x.n);
@@ -369,12 +375,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
   __shared__ float wt[kMaxSplits];
   __shared__ __align__(16) f32x4 sums[P][L];
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63;
-  const int n = A.lens[b];
   const int64_t p = ((int64_t)b * A.HK * A.G + h) * A.smax;
+  const f32x2 held = lane < A.smax ? A.pml[p + lane] : f32x2{kNone, 0.f};   // beside the length
+  const int n = A.lens[b];
   if (n <= 0 || n > ((int64_t)A.width << A.shift)) return;
   const int splits = split_count(n);
   if (splits == 1) return;
-  const f32x2 ml = lane < splits ? A.pml[p + lane] : f32x2{kNone, 0.f};
+  const f32x2 ml = lane < splits ? held : f32x2{kNone, 0.f};
   const int c = threadIdx.x % L, part = threadIdx.x / L;
   constexpr int N = (kMaxSplits + P - 1) / P;
   f32x4 x[N];
