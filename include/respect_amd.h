@@ -471,6 +471,10 @@ int rspx_rope_vision(const void* x, int64_t sxl, int64_t sxh, const float* cos, 
  * other sequences, on the tiles' size or order, or on what later keys and values hold.
  */
 int rspx_prompt_attn_tile_rows(int H, int HK);
+/* The tiles of n sequences packed one after the other, sequence i of rows[i] rows in q and
+ * keys[i] in k and v, causal from the end (the last row sees all keys), longest first: writes
+ * them to tiles, host memory, and returns their number (tiles NULL: the number alone). */
+int64_t rspx_prompt_attn_tiles(const int64_t* rows, const int64_t* keys, int n, int tile_rows, int32_t* tiles);
 int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh, const void* v,
                      int64_t svt, int64_t svh, const int32_t* tiles, int n_tiles, void* out, int64_t sot, int64_t soh,
                      int H, int HK, int Tq, int Tk, int D, float sm_scale, void* stream);

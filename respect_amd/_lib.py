@@ -88,6 +88,7 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_qkv_rope_cache_partials": (_i32, [_c_p, _i32, _c_p, _c_p, _c_p, _c_p, _i64, _c_p, _i32, _c_p, _i64, _i64, _c_p,
                                             _i64, _i64, _c_p, _i32, _i32, _i32, _i32, _f32, _c_p]),
     "rspx_prompt_attn_tile_rows": (_i32, [_i32, _i32]),
+    "rspx_prompt_attn_tiles": (_i64, [_c_p, _c_p, _i32, _i32, _c_p]),
     "rspx_prompt_attn": (_i32, [_c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i32, _c_p, _i64, _i64,
                                 _i32, _i32, _i32, _i32, _i32, _f32, _c_p]),
     "rspx_paged_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),

@@ -26,6 +26,7 @@
 // the time with few workgroups, but 337 us instead of 289 for 24 packed prompts, and the
 // choice may not depend on the pack), three and four steps in LDS (no gain), MFMAs and
 // exponentials interleaved by scheduling barriers (5 to 30 % slower), wave priorities (2 %).
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -361,6 +362,35 @@ using namespace rspx;
 extern "C" int rspx_prompt_attn_tile_rows(int H, int HK) {
   if (H < 1 || HK < 1 || H % HK) return -1;
   return kRows * (4 / heads_per_group(H / HK));
+}
+
+extern "C" int64_t rspx_prompt_attn_tiles(const int64_t* rows, const int64_t* keys, int n, int tile_rows, int32_t* tiles) {
+  if (n < 0 || tile_rows < 1 || (n > 0 && (!rows || !keys))) return RSPX_EINVAL;
+  int64_t tq = 0, tk = 0, count = 0;
+  for (int i = 0; i < n; ++i) {
+    if (rows[i] < 0 || keys[i] < 0 || rows[i] > INT32_MAX || keys[i] > INT32_MAX) return RSPX_EINVAL;
+    tq += rows[i], tk += keys[i], count += (rows[i] + tile_rows - 1) / tile_rows;
+    if (tq > INT32_MAX || tk > INT32_MAX) return RSPX_EINVAL;
+  }
+  if (!tiles) return count;
+  struct Tile {
+    int32_t x[4];
+  };
+  Tile* out = reinterpret_cast<Tile*>(tiles);
+  tq = tk = count = 0;
+  for (int i = 0; i < n; ++i) {
+    for (int64_t r = 0; r < rows[i]; r += tile_rows) {
+      const int64_t m = rows[i] - r < tile_rows ? rows[i] - r : tile_rows;
+      out[count++] = Tile{{(int32_t)(tq + r), (int32_t)m, (int32_t)tk, (int32_t)(keys[i] - rows[i] + r + 1)}};
+    }
+    tq += rows[i], tk += keys[i];
+  }
+  // The longest first, so that the device is busy to the end (ties: in the order of the rows).
+  std::sort(out, out + count, [](const Tile& a, const Tile& b) {
+    const int64_t x = (int64_t)a.x[1] + a.x[3], y = (int64_t)b.x[1] + b.x[3];
+    return x != y ? x > y : a.x[0] < b.x[0];
+  });
+  return count;
 }
 
 extern "C" int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const void* k, int64_t skt, int64_t skh,

@@ -29,22 +29,23 @@ class PackedPrompts:
         k = r if keys is None else np.asarray(list(keys), dtype=np.int64)
         if r.ndim != 1 or r.shape != k.shape or (r < 0).any() or (k < 0).any():
             raise ValueError("PackedPrompts: rows and keys must be equally many lengths >= 0")
-        self.Tq, self.Tk = int(r.sum()), int(k.sum())
-        if max(self.Tq, self.Tk) >= 1 << 31:
-            raise ValueError("PackedPrompts: at most 2^31 - 1 tokens")
         self.rows, self.keys = r.tolist(), k.tolist()
+        self.Tq, self.Tk = sum(self.rows), sum(self.keys)
         self.device = torch.device(device)
-        q0, k0 = np.cumsum(r) - r, np.cumsum(k) - k
-        parts = []
-        for size in TILE_ROWS:
-            n = -(-r // size)
-            s = np.repeat(np.arange(len(r)), n)                  # the sequence of each tile
-            first = (np.arange(len(s)) - np.repeat(np.cumsum(n) - n, n)) * size
-            t = np.stack((q0[s] + first, np.minimum(size, r[s] - first), k0[s], k[s] - r[s] + first + 1), 1)
-            # The longest first: the device is then busy to the end.
-            parts.append(t[np.argsort(-(t[:, 1] + t[:, 3]), kind="stable")].astype(np.int32))
-        flat = torch.from_numpy(np.concatenate(parts)).to(self.device)
-        self._lists = flat.split([len(t) for t in parts])
+        L, args = _lib.lib(), (r.ctypes.data, k.ctypes.data, len(r))
+        count = [L.rspx_prompt_attn_tiles(*args, size, None) for size in TILE_ROWS]
+        if min(count) < 0:
+            raise ValueError("PackedPrompts: at most 2^31 - 1 tokens")
+        on_gpu = self.device.type == "cuda"
+        if on_gpu and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("PackedPrompts: make the plan before a graph is captured")
+        host = torch.empty((sum(count), 4), dtype=torch.int32, pin_memory=on_gpu)
+        at = host.data_ptr()
+        for size, n in zip(TILE_ROWS, count):
+            if n:
+                L.rspx_prompt_attn_tiles(*args, size, at)
+            at += 16 * n
+        self._lists = host.to(self.device).split(count)   # waited for: any stream may use the plan
 
     def tiles(self, H: int, HK: int) -> torch.Tensor:
         """Device int32 [n, 4]: the tiles rspx_prompt_attn takes for these heads."""

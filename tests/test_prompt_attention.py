@@ -60,6 +60,8 @@ def _check(got, want, bound):
 def test_plan_tiles_cover_every_row_once():
     from respect_amd import _lib
     from respect_amd.kernels.prompt_attention import TILE_ROWS, PackedPrompts
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
     rows, keys = [0, 5, 64, 1, 131, 300], [7, 5, 10, 1, 200, 300]
     plan = PackedPrompts(rows, keys, device="cpu")
     assert (plan.Tq, plan.Tk, plan.rows, plan.keys) == (sum(rows), sum(keys), rows, keys)
@@ -77,20 +79,19 @@ def test_plan_tiles_cover_every_row_once():
             assert (first[q0:q0 + n] == k0).all() and (sees[q0:q0 + n] == m - n + 1 + np.arange(n)).all()
             q0, k0 = q0 + n, k0 + m
         assert (np.diff(t[:, 1] + t[:, 3]) <= 0).all()
-    if _lib.LIB_PATH.exists():
-        got = [_lib.lib().rspx_prompt_attn_tile_rows(h, hk) for h, hk in ((32, 8), (16, 2), (4, 2), (6, 2), (5, 5))]
-        assert got == [32, 32, 64, 128, 128]
-    assert PackedPrompts([], device="cpu").Tq == 0
+    got = [_lib.lib().rspx_prompt_attn_tile_rows(h, hk) for h, hk in ((32, 8), (16, 2), (4, 2), (6, 2), (5, 5))]
+    assert got == [32, 32, 64, 128, 128]
+    assert PackedPrompts([], device="cpu").Tq == 0 and len(PackedPrompts([0, 0], device="cpu")._lists[0]) == 0
 
 
 def test_refusals():
     from respect_amd import _lib
     from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
-    for bad in (([1, -1], None), ([1, 2], [1]), ([1 << 31], None)):
-        with pytest.raises(ValueError):
-            PackedPrompts(*bad, device="cpu")
     if not _lib.LIB_PATH.exists():
         pytest.skip("librespect_amd.so not built")
+    for bad in (([1, -1], None), ([1, 2], [1]), ([1 << 31], None), ([1 << 30] * 2, [0, 0]), ([1, 1], [1 << 30, 1 << 30])):
+        with pytest.raises(ValueError):
+            PackedPrompts(*bad, device="cpu")
     plan = PackedPrompts([4], device="cpu")
     q, k, v = _inputs([4], [4], 4, 2, 64)
     with pytest.raises(RuntimeError, match="GPU"):
@@ -225,6 +226,8 @@ def test_graph_replays_and_streams():
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         out = prompt_attn(q, k, v, plan)
+        with pytest.raises(RuntimeError, match="captured"):
+            PackedPrompts(rows)
     side = torch.cuda.Stream()
     for seed in range(3):
         for t, x in zip((q, k, v), _inputs(rows, rows, 8, 2, 128, seed=20 + seed)):
