@@ -485,7 +485,7 @@ int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const void* k, int
  *   strides); table [B][width] int32 (row stride stb): key j of sequence b is pool row
  *   table[b][j / page] * page + j % page; lens [B] int32: the keys of each sequence, the
  *   new token's own among them.  D contiguous, 16-byte aligned bases and strides (out:
- *   any).  page a power of two; H / HK <= 16; D in {32, 64, 128, 256}; sm_scale > 0.
+ *   any).  page a power of two; H / HK <= 16; HK <= 4096; D in {32, 64, 128, 256}; sm_scale > 0.
  * lens[b] == 0 gives zeros.  A length that is negative or above width * page, and a
  * page that is none among those a sequence reads, give NaN rows; nothing outside the
  * pool is read.  Table entries past a sequence's length are not read.
@@ -502,7 +502,7 @@ int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int
 
 /* ---------------------------------------------------------------- rows of a paged cache
  * rspx_kv_move: for each of n_tensors pools (device array `bases` of base addresses,
- * each [HK][cap][D] bf16, head stride sh, slot stride sn) and each head, the moves
+ * each [HK][cap][D] bf16, 16-byte aligned, head stride sh, slot stride sn) and each head, the moves
  * (src slot, dst slot) of device int32 moves[n_moves][2].  groups [n_groups + 1] cuts
  * them into groups: those of one group take effect in order, provided no destination
  * is the source of a later move of the group (rows moved down in increasing order are
@@ -561,7 +561,7 @@ int rspx_pages_slots(rspx_pages* p, const int32_t* ids, int n, const int64_t* fi
  * and the `top` largest scores' log p (values [M, top], best first) and columns (ids
  * [M, top]).  Ties go to the lowest index, NaN is the largest value; a row that holds a
  * NaN or +inf has NaN results.  A token outside [0, V): given NaN.  A row with every
- * score -inf: -inf, entropy 0.  top <= 64 and <= V; 0: values / ids unused.
+ * score -inf: -inf, entropy 0.  top <= 64 and <= V; 0: values / ids unused.  V <= 2^30.
  * A row's bits do not depend on M.  workspace: rspx_token_logprobs_workspace_bytes
  * bytes, 8-byte aligned, of any content.
  */

@@ -32,6 +32,7 @@ constexpr int kPer = 16;                       // elements per lane
 constexpr int kSub = 64 * kPer;                // columns of a wave's step: the unit of the sums
 constexpr int kChunk = 4 * kSub;               // columns of a workgroup's step
 constexpr int kMaxTop = 64;
+constexpr int kMaxV = 1 << 30;                 // columns are counted in 32 bits
 constexpr int kGroups = 64;                    // groups of four threads
 constexpr float kL2E = 1.44269504088896340736f;
 
@@ -406,7 +407,7 @@ constexpr int kRowsPerLaunch = 65535;
 using namespace rspx;
 
 extern "C" int64_t rspx_token_logprobs_workspace_bytes(int M, int V, int top) {
-  if (M < 0 || V <= 0 || top < 0 || top > kMaxTop) return -1;
+  if (M < 0 || V <= 0 || V > kMaxV || top < 0 || top > kMaxTop) return -1;
   const int64_t chunks = ((int64_t)V + kChunk - 1) / kChunk;
   return (int64_t)M * (8 * (int64_t)top * (M ? parts_of(M, (int)chunks, top) : 0) + 48 * chunks) + 8;
 }
@@ -415,7 +416,7 @@ extern "C" int rspx_token_logprobs(const float* logits, int64_t sl, int M, int V
                                    int top, float* given, float* entropy, float* values, int64_t* ids, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
   if (M < 0 || V <= 0 || sl < V || off < 0 || size < 0 || top < 0 || top > V) return RSPX_EINVAL;
-  if (top > kMaxTop) return RSPX_EUNSUPPORTED;
+  if (top > kMaxTop || V > kMaxV) return RSPX_EUNSUPPORTED;
   if (M == 0) return RSPX_OK;
   if (!logits || !tokens || !given || !entropy || (top && (!values || !ids))) return RSPX_EINVAL;
   if ((reinterpret_cast<uintptr_t>(logits) & 15u) || sl % 4) return RSPX_EALIGN;

@@ -454,10 +454,11 @@ extern "C" int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const vo
   if (B < 0 || H < 1 || HK < 1 || H % HK || pages < 1 || page < 1 || (page & (page - 1)) || width < 0) return RSPX_EINVAL;
   if (!(sm_scale > 0.f) || sm_scale > 3e38f) return RSPX_EINVAL;
   if ((int64_t)pages * page > INT32_MAX || (int64_t)width * page > INT32_MAX - 4096) return RSPX_EINVAL;
-  if (!head_dim_ok(D) || H / HK > 16 || HK > 65535) return RSPX_EUNSUPPORTED;
+  if (!head_dim_ok(D) || H / HK > 16 || HK > 4096) return RSPX_EUNSUPPORTED;   // items of a launch are counted in 32 bits
   if (B == 0) return RSPX_OK;
   if (!q || !kc || !vc || !lens || !out || (width && !table)) return RSPX_EINVAL;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  if (reinterpret_cast<uintptr_t>(out) & 1u) return RSPX_EALIGN;
   if (!al(q) || !al(kc) || !al(vc) || sqb % 8 || sqh % 8 || skh % 8 || skn % 8 || svh % 8 || svn % 8) return RSPX_EALIGN;
   const int64_t need = rspx_paged_attn_workspace_bytes(B, H, D, page, width);
   if (need > 0 && (!workspace || workspace_bytes < need)) return RSPX_EWORKSPACE;

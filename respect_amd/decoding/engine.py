@@ -372,9 +372,17 @@ class Decoder:
         seqs = list(seqs)
         if tuple(ids.shape) != (len(seqs),) or not seqs:
             raise ValueError("step_batch: one token per sequence, at least one")
-        cfg, B = self.cfg, len(seqs)
         cache.extend(seqs, 1)
         n = [cache.length(s) for s in seqs]
+        try:
+            return self._step_batch(ids, cache, seqs, n)
+        except BaseException:
+            cache.compact(seqs, [m - 1 for m in n], [[] for _ in n])
+            raise
+
+    def _step_batch(self, ids, cache, seqs, n: list[int]) -> torch.Tensor:
+        """step_batch for sequences that have been extended to ``n`` rows."""
+        cfg, B = self.cfg, len(seqs)
         slots = cache.slots(seqs, [m - 1 for m in n], 1)
         table, lens = cache.tables(seqs)
         att = torch.empty((B, cfg.heads, cfg.head_dim), dtype=torch.bfloat16, device=self.device)

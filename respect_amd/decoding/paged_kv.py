@@ -144,8 +144,10 @@ class PagedKVCache:
     """``pages`` pages of ``page`` rows (a power of two), at most ``sequences`` sequences at a
     time.  Sequences are named by the numbers that ``add`` and ``fork`` give.  The methods
     keep books on the host and enqueue their copies on the current stream; those that do
-    cannot be captured into a graph.  A refused call (``ValueError``; ``RuntimeError`` for
-    too few pages or sequences) changes nothing.  One thread at a time."""
+    cannot be captured into a graph.  Pages given back are taken again at once: calls that
+    still read them have to be on the same stream, or waited for.  A refused call
+    (``ValueError``; ``RuntimeError`` for too few pages or sequences) changes nothing.  One
+    thread at a time."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page: int = 64, device="cuda",
                  sequences: int = 1024):
@@ -153,11 +155,11 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: layers and kv_heads >= 1 and head_dim a multiple of 8")
         self._t = PageTable(pages, page, sequences)
         self.layers, self.HK, self.D, self.page, self.pages = layers, kv_heads, head_dim, page, pages
-        self.device = torch.device(device)
         shape = (kv_heads, pages * page, head_dim)
         self.k = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
-        bases = torch.tensor([t.data_ptr() for kv in zip(self.k, self.v) for t in kv], dtype=torch.int64).to(device)
+        self.device = self.k[0].device
+        bases = torch.tensor([t.data_ptr() for kv in zip(self.k, self.v) for t in kv], dtype=torch.int64).to(self.device)
         k0 = self.k[0]
         self._pool = (bases, kv_heads, head_dim, k0.stride(0), k0.stride(1), pages * page)
 

@@ -88,7 +88,7 @@ def test_refusals():
     assert call(H=3) == -1 and call(B=-1) == -1 and call(pages=0) == -1 and call(page=12) == -1 and call(width=-1) == -1
     assert call(scale=0.0) == -1 and call(scale=float("nan")) == -1 and call(p=0) == -1 and call(lens=0) == -1
     assert call(table=0) == -1 and call(pages=1 << 28) == -1 and call(width=1 << 28) == -1
-    assert call(D=96) == -2 and call(H=34) == -2
+    assert call(D=96) == -2 and call(H=34) == -2 and call(H=5000, HK=5000) == -2
     assert call(p=8) == -4 and call(st=100) == -4
     assert call(width=1024, ws=16) == -3
     assert call(B=0) == 0

@@ -370,3 +370,7 @@ def test_gpu_refusals():
         c.write(0, k.float(), k.float(), slots)
     with pytest.raises(RuntimeError):
         c.write(0, k, k, slots.cpu())
+    c.write(0, k[:0], k[:0], slots[:0])
+    table, lens = c.tables([])
+    assert table.shape == (0, 0) and lens.shape == (0,) and c.slots([], 0, 0).shape == (0,)
+    assert c.device.index is not None

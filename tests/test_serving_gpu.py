@@ -120,4 +120,9 @@ def test_refusals(model):
         model.step_batch(torch.tensor([1], device="cuda"), cache, [seqs[0] + 1])
     with pytest.raises(ValueError):
         model.step_batch(torch.tensor([1, 2], device="cuda"), cache, seqs * 2)
+    with pytest.raises(RuntimeError):
+        model.step_batch(torch.tensor([1]), cache, seqs)            # fails past the extension
+    with pytest.raises(RuntimeError):
+        model.prefill_batch([torch.tensor([1, 2, 3])], cache)
+    assert cache.free_pages == 63
     assert cache.length(seqs[0]) == 3
