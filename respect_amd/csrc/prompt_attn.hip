@@ -11,23 +11,27 @@
 // row: the softmax (fp32, a running maximum that moves only when a score passes it by
 // 2^kTau) needs no lane exchange but the rare move's.  The probabilities, rounded to bf16
 // as the trie attention rounds them (half a step each, against fp32 sums), are used in place
-// as the B operand of O^T += V^T P^T with V read transposed from LDS.  The products of the
-// next step's scores run beside a step's exponentials.
+// as the B operand of O^T += V^T P^T with V read transposed from LDS.  In steps that every
+// row sees whole, the next step's score products and this step's exponentials, then the
+// products with V and the next maximum, stand alternating in the code: four simple
+// instructions or two exponentials cost nothing beside a product of the same wave.
 //
 // Every row is computed from its own column of the MFMA tiles in 64-key steps from the
 // sequence's first key on: its bits depend on its sequence alone, not on the pack, on the
 // tile it falls in or on later rows.
 //
-// What bounds it: in long prompts the power budget (16384 tokens, 32 / 8 heads of 128: 1.98 ms,
-// 1.11 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.8 GHz, the
-// MFMAs are busy 58 % of it, VALU half; LDS reads 29 %, no bank conflicts); in short ones and
-// few heads the serial chain of a step at one wave per SIMD (1.0 us at D = 128).  Measured and
-// not kept: eight waves per tile that take the steps in turn and are joined (three quarters of
-// the time with few workgroups, but 337 us instead of 289 for 24 packed prompts, and the
-// choice may not depend on the pack), three and four steps in LDS (no gain), MFMAs and
-// exponentials interleaved by scheduling barriers (5 to 30 % slower), wave priorities (2 %).
+// What bounds it: in long prompts the power budget (16384 tokens, 32 / 8 heads of 128: 1.9 ms,
+// 1.15 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.8 GHz, the
+// MFMAs are busy 60 % of it, VALU half; LDS reads 29 %, no bank conflicts); in short ones and
+// few heads the serial chain of a step at one wave per SIMD (1.0 us at D = 128).  The order of
+// the whole steps, held by scheduling barriers, took 3 % off the long cases (the compiler's
+// own: 1.93 ms beside 1.87, 24 packed prompts 278 us beside 270) and nothing off the short.
+// Measured and not kept: eight waves per tile that take the steps in turn and are joined
+// (three quarters of the time with few workgroups, but 337 us instead of 289 for 24 packed
+// prompts, and the choice may not depend on the pack), three and four steps in LDS (no
+// gain), the compiler's own interleaving groups (5 to 30 % slower), wave priorities (2 %),
+// whole steps not unrolled by two, which copies the scores (270 -> 278 us).
 #include <algorithm>
-#include <type_traits>
 
 #include "common.h"
 #include "respect_amd.h"
@@ -189,7 +193,7 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
         o[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[i], o[kb], 0, 0, 0);
       }
   };
-  f32x16 s[2];
+  f32x16 s[2], next[2];
   if (steps > 0) {
     issue_k(0);
     issue_v(0);
@@ -206,46 +210,24 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
 
-  const int first_edge = min(whole, steps - 1);            // the last step has no scores to run ahead
-  // One step of 64 keys, whose scores are in s; the next ones' products run beside its softmax.
-  // `edge`: some row may not see all of its keys.
-  auto step = [&](int t, auto edge) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of V and the next K
-    lds_barrier();                                         // everyone's; and the step before is read
-    issue_k(t + 2);
-    issue_v(t + 1);
-    lds_char* sv = (lds_char*)lds + kBytes * (2 + (t & 1));
-    // A key that a row does not see has p = 0, but 0 * inf and 0 * NaN are NaN: such a value
-    // among the step's may not reach the rows before it.  Each wave looks a quarter of V over.
-    bool odd = false;
-    if constexpr (edge) {
-      uint32_t found = 0;
+  // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
+  // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
+  auto vread = [&](const lds_char* sv, int i, int j) __attribute__((always_inline)) {
+    s16x4 h[2];
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const u32x4 x = read16(sv + 1024 * (4 * j + w) + 16 * lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) found |= (x[e] & 0x7f807f80u) + 0x00800080u;   // an exponent of ones carries
-      }
-      if (__builtin_amdgcn_ballot_w64((found & 0x80008000u) != 0) != 0 && lane == 0) flags[t - first_edge] = 1;
-      lds_barrier();
-      odd = __builtin_amdgcn_readfirstlane(flags[t - first_edge]) != 0;
+    for (int z = 0; z < 2; ++z) {
+      const int l16 = lane & 15;
+      const int key = 16 * i + 8 * z + 4 * half + (l16 >> 2);
+      const int u = 4 * j + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+      h[z] = tr_read(sv + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1));
     }
-
-    bf16x8 p[4];
-    if constexpr (edge) {   // keys that a row does not see
-      const int mine = seen - t * kKeys - 4 * half;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (32 * kb + 8 * (e / 4) + e % 4 >= mine) s[kb][e] = kNegInf;
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // The running maximum moved, and what hangs on it, where a row's largest score passes it.
+  auto move = [&](float mx) __attribute__((always_inline)) {
     if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
       const float top = fmaxf(mx, shfl_xor(mx, 32)) * A.c;
-      const float mn = top > mref + kTau ? top : mref;   // rows that stay get a factor of exactly 1
+      const float mn = top > mref + kTau ? top : mref;     // rows that stay get a factor of exactly 1
       const float alpha = fexp2(mref - mn);
       lsum = lsum * alpha;
       mref = mn;
@@ -254,76 +236,152 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
     }
-    f32x16 ahead[2];
-    if constexpr (!edge) scores(t + 1, ahead);
+  };
+  // Two probabilities of the row, of scores r and r + 1, as bf16.
+  auto pair = [&](const f32x16 (&s)[2], int r) __attribute__((always_inline)) {
+    const float a = fexp2(__builtin_fmaf(s[r / 16][r % 16], A.c, -mref));
+    const float b = fexp2(__builtin_fmaf(s[r / 16][r % 16 + 1], A.c, -mref));
+    lsum = lsum + a;
+    lsum = lsum + b;
+    return pack_bf16x2(a, b);
+  };
+
+  const int first_edge = min(whole, steps - 1);            // the last step has no scores to run ahead
+  // One step that every row sees whole, its scores in s and the maximum moved; the next
+  // step's scores come to `next`.  In program order, which the barriers keep: a matrix
+  // product, the operands of the third after it, and as much of the softmax as fits beside it.
+  auto whole_step = [&](int t, const f32x16 (&s)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
+    constexpr int NA = 2 * NS, NB = 4 * DT, Z = 3;
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of V and the next K
+    lds_barrier();                                         // everyone's; and the step before is read
+    issue_k(t + 2);
+    issue_v(t + 1);
+    const lds_char* sk = (const lds_char*)lds + kBytes * ((t + 1) & 1);
+    const lds_char* sv = (const lds_char*)lds + kBytes * (2 + (t & 1));
+    auto kread = [&](int n) __attribute__((always_inline)) {
+      const int key = 32 * (n % 2) + col;
+      return __builtin_bit_cast(bf16x8, read16(sk + 16 * (key * U + ((2 * (n / 2) + half) ^ kswizzle<D>(key)))));
+    };
+    bf16x8 x[Z + 1];
+    u32x4 p[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u32x4 x;
+    for (int n = 0; n < Z; ++n) x[n] = kread(n);
+    f32x16 zero;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 8 * i + 2 * e;
-        const float a = fexp2(__builtin_fmaf(s[r / 16][r % 16], A.c, -mref));
-        const float b = fexp2(__builtin_fmaf(s[r / 16][r % 16 + 1], A.c, -mref));
-        lsum = lsum + a;
-        lsum = lsum + b;
-        x[e] = pack_bf16x2(a, b);
-      }
-      p[i] = __builtin_bit_cast(bf16x8, x);
+    for (int e = 0; e < 16; ++e) zero[e] = 0.f;
+    // The next scores beside the first half of the exponentials.
+#pragma unroll
+    for (int n = 0; n < NA; ++n) {
+      if (n + Z < NA) x[(n + Z) % (Z + 1)] = kread(n + Z);
+      else x[(n + Z) % (Z + 1)] = vread(sv, (n + Z - NA) / DT, (n + Z - NA) % DT);
+      next[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[n % (Z + 1)], qf[n / 2], n < 2 ? zero : next[n % 2], 0, 0, 0);
+#pragma unroll
+      for (int i = 8 * n / NA; i < 8 * (n + 1) / NA; ++i) p[i / 4][i % 4] = pair(s, 2 * i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (edge) {
-      if (odd) {
-        // The values that are not finite go to the rows that see them one by one, and the
-        // product runs without them: every other sum keeps its bits.
-        const int mine = seen - t * kKeys;               // keys of the step that this lane's row sees
+    // The product with V beside the other half, then beside the next scores' maximum.
+    float mx = kNegInf;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      if (n + Z < NB) x[(NA + n + Z) % (Z + 1)] = vread(sv, (n + Z) / DT, (n + Z) % DT);
+      acc[n % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[(NA + n) % (Z + 1)], __builtin_bit_cast(bf16x8, p[n / DT]),
+                                                            acc[n % DT], 0, 0, 0);
+      if (n < NB / 2) {
+#pragma unroll
+        for (int i = 8 + 16 * n / NB; i < 8 + 16 * (n + 1) / NB; ++i) p[i / 4][i % 4] = pair(s, 2 * i);
+      } else {
+#pragma unroll
+        for (int i = 64 * (n - NB / 2) / NB; i < 64 * (n - NB / 2 + 1) / NB; ++i) mx = fmaxf(mx, next[i / 16][i % 16]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (t + 1 < first_edge) move(mx);
+  };
+  // One step of 64 keys that some row may not see all of, or the last one; its scores are in s.
+  auto edge_step = [&](int t) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0): this wave's part of V and the next K
+    lds_barrier();                                         // everyone's; and the step before is read
+    issue_k(t + 2);
+    issue_v(t + 1);
+    lds_char* sv = (lds_char*)lds + kBytes * (2 + (t & 1));
+    // A key that a row does not see has p = 0, but 0 * inf and 0 * NaN are NaN: such a value
+    // among the step's may not reach the rows before it.  Each wave looks a quarter of V over.
+    uint32_t found = 0;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const u32x4 x = read16(sv + 1024 * (4 * j + w) + 16 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) found |= (x[e] & 0x7f807f80u) + 0x00800080u;   // an exponent of ones carries
+    }
+    if (__builtin_amdgcn_ballot_w64((found & 0x80008000u) != 0) != 0 && lane == 0) flags[t - first_edge] = 1;
+    lds_barrier();
+
+    const int mine = seen - t * kKeys;                     // keys of the step that this lane's row sees
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (32 * kb + 8 * (e / 4) + 4 * half + e % 4 >= mine) s[kb][e] = kNegInf;
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+    move(mx);
+    u32x4 p[4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i / 4][i % 4] = pair(s, 2 * i);
+    if (__builtin_amdgcn_readfirstlane(flags[t - first_edge]) != 0) {
+      // The values that are not finite go to the rows that see them one by one, and the
+      // product runs without them: every other sum keeps its bits.
 #pragma unroll 1
-        for (int key = 0; key < kKeys; ++key)
+      for (int key = 0; key < kKeys; ++key)
 #pragma unroll
-          for (int j = 0; j < DT; ++j)
+        for (int j = 0; j < DT; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int d = 32 * j + 8 * (e / 4) + 4 * half + e % 4;
-              const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
-                  sv + 16 * (key * U + ((d / 8) ^ vswizzle<D>(key))) + 2 * (d % 8));
-              if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + bf16_to_f32(x);
-            }
-        lds_barrier();
-#pragma unroll 1
-        for (int j = 0; j < kLoads; ++j) {
-          auto* at = (__attribute__((address_space(3))) u32x4*)(sv + 1024 * (4 * j + w) + 16 * lane);
-          u32x4 x = *at;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u;
-            if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
+          for (int e = 0; e < 16; ++e) {
+            const int d = 32 * j + 8 * (e / 4) + 4 * half + e % 4;
+            const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
+                sv + 16 * (key * U + ((d / 8) ^ vswizzle<D>(key))) + 2 * (d % 8));
+            if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + bf16_to_f32(x);
           }
-          *at = x;
+      lds_barrier();
+#pragma unroll 1
+      for (int j = 0; j < kLoads; ++j) {
+        auto* at = (__attribute__((address_space(3))) u32x4*)(sv + 1024 * (4 * j + w) + 16 * lane);
+        u32x4 x = *at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u;
+          if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
         }
-        lds_barrier();
+        *at = x;
       }
+      lds_barrier();
     }
-    // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
-    // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < DT; ++j) {
-        s16x4 h[2];
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int l16 = lane & 15;
-          const int key = 16 * i + 8 * z + 4 * half + (l16 >> 2);
-          const int u = 4 * j + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-          h[z] = tr_read(sv + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1));
-        }
-        const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, p[i], acc[j], 0, 0, 0);
-      }
-    if constexpr (!edge) s[0] = ahead[0], s[1] = ahead[1];
-    else if (t + 1 < steps) scores(t + 1, s);
+      for (int j = 0; j < DT; ++j)
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(sv, i, j), __builtin_bit_cast(bf16x8, p[i]), acc[j], 0, 0, 0);
+    if (t + 1 < steps) scores(t + 1, s);
   };
+
   int t = 0;
-  for (; t < first_edge; ++t) step(t, std::false_type());
-  for (; t < steps; ++t) step(t, std::true_type());
+  if (first_edge > 0) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+    move(mx);
+  }
+  for (; t + 1 < first_edge; t += 2) {                     // the scores change places: no copies
+    whole_step(t, s, next);
+    whole_step(t + 1, next, s);
+  }
+  if (t < first_edge) {
+    whole_step(t, s, next);
+    s[0] = next[0], s[1] = next[1];
+    ++t;
+  }
+  for (; t < steps; ++t) edge_step(t);
 
   // Lane (col, half): row col, head_dim 32 j + 8 (e / 4) + 4 half + e % 4.
   if (!live) return;
