@@ -21,11 +21,12 @@
 // tile it falls in or on later rows.
 //
 // What bounds it: in long prompts the power budget (16384 tokens, 32 / 8 heads of 128: 1.9 ms,
-// 1.15 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.8 GHz, the
-// MFMAs are busy 60 % of it, VALU half; LDS reads 29 %, no bank conflicts); in short ones and
-// few heads the serial chain of a step at one wave per SIMD (1.0 us at D = 128).  The order of
-// the whole steps, held by scheduling barriers, took 3 % off the long cases (the compiler's
-// own: 1.93 ms beside 1.87, 24 packed prompts 278 us beside 270) and nothing off the short.
+// 1.15 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.7 GHz, the
+// MFMAs are busy 65 % of it, VALU half; the LDS reads, 128 KB per step and workgroup, take as
+// long as the MFMAs, without bank conflicts); in short ones and few heads the serial chain of
+// a step at one wave per SIMD (1.0 us at D = 128).  The order of the whole steps, held by
+// scheduling barriers, took 3 % off the long cases (the compiler's own: 1.93 ms beside 1.87,
+// 24 packed prompts 278 us beside 270) and nothing off the short.
 // Measured and not kept: eight waves per tile that take the steps in turn and are joined
 // (three quarters of the time with few workgroups, but 337 us instead of 289 for 24 packed
 // prompts, and the choice may not depend on the pack), three and four steps in LDS (no

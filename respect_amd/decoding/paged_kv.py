@@ -274,7 +274,7 @@ class PagedKVCache:
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """k / v [T, HK, D] bf16 of one layer to the pool rows ``slots`` [T] (device int32, as
-        ``slots`` gives them).  Can be captured."""
+        ``slots`` gives them; one named twice keeps parts of either row).  Can be captured."""
         T = k.shape[0]
         if tuple(k.shape) != (T, self.HK, self.D) or v.shape != k.shape or tuple(slots.shape) != (T,):
             raise ValueError(f"PagedKVCache: k and v must be [T, {self.HK}, {self.D}], slots [T]")

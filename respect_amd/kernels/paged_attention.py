@@ -19,7 +19,8 @@ def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None):
 
     All on one GPU; table and lens are read there, so that a captured call follows them.
     A sequence of length 0 gets zeros; one whose length is negative or beyond its table, or
-    that reads a page outside the pool, gets NaN.  ``page``: a power of two."""
+    that reads a page outside the pool, gets NaN.  ``page``: a power of two.  ``out``: written
+    in place if given; no memory of the other tensors.  Scores as for ``prompt_attn``."""
     if out is None:
         y = _lib.calls().paged_attn(q, kc, vc, table, lens, page, sm_scale)
         if y is not None:

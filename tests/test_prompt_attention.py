@@ -178,6 +178,29 @@ def test_rows_do_not_depend_on_the_pack(H, HK, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,HK,D", [(4, 1, 128), (4, 2, 64), (2, 2, 32), (8, 2, 256)])
+def test_chunks_give_the_bits_of_the_whole_prompt(H, HK, D):
+    """A prompt in one pass, and in chunks after its earlier keys, between other sequences: a row
+    falls in other tiles, and steps that a tile sees whole are seen in part elsewhere.  Scores
+    that grow and fall, so that the running maximum moves in every kind of step."""
+    from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
+    n = 700
+    q, k, v = _inputs([n], [n], H, HK, D, seed=21)
+    k = (k.float() * (1 + 5 * torch.sin(torch.arange(n) / 37.0).abs())[:, None, None]).to(BF)
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    whole = prompt_attn(q, k, v, PackedPrompts([n]))
+    for chunk in (1, 64, 100, 333):
+        ends = list(range(chunk, n, chunk)) + [n] if chunk > 1 else [1, 64, 65, 128, 129, 640, 700]
+        firsts = [max(0, e - chunk) for e in ends] if chunk == 1 else [0] + ends[:-1]
+        rows = [e - f for f, e in zip(firsts, ends)]
+        qs = torch.cat([q[f:e] for f, e in zip(firsts, ends)])
+        ks, vs = (torch.cat([t[:e] for e in ends]) for t in (k, v))
+        got = prompt_attn(qs, ks, vs, PackedPrompts(rows, ends))
+        want = torch.cat([whole[f:e] for f, e in zip(firsts, ends)])
+        assert torch.equal(got, want), chunk
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("D", [64, 128])
 def test_values_behind_a_row_do_not_reach_it(what, D):
