@@ -10,11 +10,12 @@
 // A wave computes S^T = K Q^T by v_mfma_f32_32x32x16_bf16, so a lane holds 32 scores of one
 // row: the softmax (fp32, a running maximum that moves only when a score passes it by
 // 2^kTau) needs no lane exchange but the rare move's.  The probabilities, rounded to bf16
-// as the trie attention rounds them (half a step each, against fp32 sums), are used in place
-// as the B operand of O^T += V^T P^T with V read transposed from LDS.  In steps that every
-// row sees whole, the next step's score products and this step's exponentials, then the
-// products with V and the next maximum, stand alternating in the code: four simple
-// instructions or two exponentials cost nothing beside a product of the same wave.
+// as the trie attention rounds them (half a step each), are summed in fp32 as rounded, so that
+// numerator and denominator weigh alike, and used in place as the B operand of O^T += V^T P^T
+// with V read transposed from LDS.  In steps that every row sees whole, the next step's score
+// products and this step's exponentials, then the products with V and the next maximum, stand
+// alternating in the code: four simple instructions or two exponentials cost nothing beside a
+// product of the same wave.
 //
 // Every row is computed from its own column of the MFMA tiles in 64-key steps from the
 // sequence's first key on: its bits depend on its sequence alone, not on the pack, on the
@@ -22,16 +23,19 @@
 //
 // What bounds it: in long prompts the power budget (16384 tokens, 32 / 8 heads of 128: 1.9 ms,
 // 1.15 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.7 GHz, the
-// MFMAs are busy 65 % of it, VALU half; the LDS reads, 128 KB per step and workgroup, take as
-// long as the MFMAs, without bank conflicts); in short ones and few heads the serial chain of
-// a step at one wave per SIMD (1.0 us at D = 128).  The order of the whole steps, held by
-// scheduling barriers, took 3 % off the long cases (the compiler's own: 1.93 ms beside 1.87,
-// 24 packed prompts 278 us beside 270) and nothing off the short.
+// MFMAs are busy 65 % of it, VALU half; the LDS reads, 128 KB per step and workgroup, take half
+// as long as the MFMAs, without bank conflicts); in short ones and few heads what one wave per
+// SIMD issues in a step (0.87 us at D = 128, of which the MFMAs are 0.48; memory has no part
+// in it: keys that all lie in one row take as long).  The order of the whole steps, held by
+// scheduling barriers, took 3 % off the long cases (the compiler's own: 1.93 ms beside 1.87, 24
+// packed prompts 278 us beside 270) and nothing off the short; addresses worked out once and
+// probabilities summed in pairs 2 to 3 % off these (219 instructions a step instead of 268).
 // Measured and not kept: eight waves per tile that take the steps in turn and are joined
 // (three quarters of the time with few workgroups, but 337 us instead of 289 for 24 packed
 // prompts, and the choice may not depend on the pack), three and four steps in LDS (no
 // gain), the compiler's own interleaving groups (5 to 30 % slower), wave priorities (2 %),
-// whole steps not unrolled by two, which copies the scores (270 -> 278 us).
+// whole steps not unrolled by two, which copies the scores (270 -> 278 us), and the barrier in
+// the middle of a step, operands of the next one requested before its end (0 to 2 %).
 #include <algorithm>
 
 #include "common.h"
@@ -77,6 +81,12 @@ __device__ __forceinline__ s16x4 tr_read(const lds_char* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
 }
 
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+// c + both bf16 of x, rounded to nearest (measured: 63 of 64 sums as one rounding, none by more
+// than 0.52 of a step).
+__device__ __forceinline__ float dot2(uint32_t x, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b16x2, x), __builtin_bit_cast(b16x2, 0x3f803f80u), c, false);
+}
 // LDS reads of what is in place (its loads waited for, the barrier passed).  __restrict__:
 // without alias information the compiler waits for every load to LDS in flight, the next
 // steps' included, ahead of the first read.
@@ -178,6 +188,20 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) to_lds(r, vo[j], dst + 1024 * (4 * j + w));
   };
+  // Byte offsets in a step's K and V of this lane's first operands: those of the others differ
+  // by constants, added for keys and xored, as the swizzles are, for head_dim.  Made once: the
+  // compiler would work them out anew in every step.
+  int k_at = 16 * (col * U + (half ^ kswizzle<D>(col)));
+  int v_at;
+  {
+    const int l16 = lane & 15, key = 4 * half + (l16 >> 2), u = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    v_at = 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1);
+  }
+  asm("" : "+v"(k_at), "+v"(v_at));
+  // A operand of the scores: keys 32 kb + col, head_dim 16 i + 8 half .. + 7.
+  auto kread = [&](const lds_char* sk, int i, int kb) __attribute__((always_inline)) {
+    return __builtin_bit_cast(bf16x8, read16(sk + (k_at ^ (32 * i)) + 16 * 32 * U * kb));
+  };
   // S^T of a step: two blocks of 32 keys.  Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
   auto scores = [&](int t, f32x16 (&o)[2]) __attribute__((always_inline)) {
     const lds_char* sk = (const lds_char*)lds + kBytes * (t & 1);
@@ -188,11 +212,8 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 #pragma unroll
     for (int i = 0; i < NS; ++i)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const int key = 32 * kb + col;
-        const u32x4 x = read16(sk + 16 * (key * U + ((2 * i + half) ^ kswizzle<D>(key))));
-        o[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), qf[i], o[kb], 0, 0, 0);
-      }
+      for (int kb = 0; kb < 2; ++kb)
+        o[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kread(sk, i, kb), qf[i], o[kb], 0, 0, 0);
   };
   f32x16 s[2], next[2];
   if (steps > 0) {
@@ -216,12 +237,7 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
   auto vread = [&](const lds_char* sv, int i, int j) __attribute__((always_inline)) {
     s16x4 h[2];
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      const int l16 = lane & 15;
-      const int key = 16 * i + 8 * z + 4 * half + (l16 >> 2);
-      const int u = 4 * j + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-      h[z] = tr_read(sv + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1));
-    }
+    for (int z = 0; z < 2; ++z) h[z] = tr_read(sv + (v_at ^ (64 * j)) + 16 * U * (16 * i + 8 * z));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
   // The running maximum moved, and what hangs on it, where a row's largest score passes it.
@@ -242,9 +258,9 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
   auto pair = [&](const f32x16 (&s)[2], int r) __attribute__((always_inline)) {
     const float a = fexp2(__builtin_fmaf(s[r / 16][r % 16], A.c, -mref));
     const float b = fexp2(__builtin_fmaf(s[r / 16][r % 16 + 1], A.c, -mref));
-    lsum = lsum + a;
-    lsum = lsum + b;
-    return pack_bf16x2(a, b);
+    const uint32_t x = pack_bf16x2(a, b);
+    lsum = dot2(x, lsum);
+    return x;
   };
 
   const int first_edge = min(whole, steps - 1);            // the last step has no scores to run ahead
@@ -259,21 +275,17 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
     issue_v(t + 1);
     const lds_char* sk = (const lds_char*)lds + kBytes * ((t + 1) & 1);
     const lds_char* sv = (const lds_char*)lds + kBytes * (2 + (t & 1));
-    auto kread = [&](int n) __attribute__((always_inline)) {
-      const int key = 32 * (n % 2) + col;
-      return __builtin_bit_cast(bf16x8, read16(sk + 16 * (key * U + ((2 * (n / 2) + half) ^ kswizzle<D>(key)))));
-    };
     bf16x8 x[Z + 1];
     u32x4 p[4];
 #pragma unroll
-    for (int n = 0; n < Z; ++n) x[n] = kread(n);
+    for (int n = 0; n < Z; ++n) x[n] = kread(sk, n / 2, n % 2);
     f32x16 zero;
 #pragma unroll
     for (int e = 0; e < 16; ++e) zero[e] = 0.f;
     // The next scores beside the first half of the exponentials.
 #pragma unroll
     for (int n = 0; n < NA; ++n) {
-      if (n + Z < NA) x[(n + Z) % (Z + 1)] = kread(n + Z);
+      if (n + Z < NA) x[(n + Z) % (Z + 1)] = kread(sk, (n + Z) / 2, (n + Z) % 2);
       else x[(n + Z) % (Z + 1)] = vread(sv, (n + Z - NA) / DT, (n + Z - NA) % DT);
       next[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[n % (Z + 1)], qf[n / 2], n < 2 ? zero : next[n % 2], 0, 0, 0);
 #pragma unroll

@@ -24,7 +24,8 @@ def _inputs(rows, keys, H, HK, D, seed=0):
 
 def _exact(q, k, v, rows, keys, scale=None):
     """(result, bound) in float64.  The bound, to first order: every p rounded to bf16 (half a
-    step is 2^-8 of it) and the result once; scores accumulated over D products and sums over n
+    step, d_i <= 2^-8 of it) in numerator and denominator alike, so that the result moves by
+    sum p_i d_i v_i - o sum p_i d_i = sum p_i d_i (v_i - o), and the result once; scores accumulated over D products and sums over n
     keys in fp32, whose steps are 2^-24 each; a score's error moves p by that much relative,
     in the numerator and in the denominator."""
     T, H, D = q.shape
@@ -44,7 +45,8 @@ def _exact(q, k, v, rows, keys, scale=None):
                 o, a = p @ vd[:seen], p @ vd[:seen].abs()
                 es = 2.0 ** -24 * ((D + 8) * float((kd[:seen].abs() @ qd[i].abs()).max()) * scale + 8)
                 out[t + i, h] = o
-                bound[t + i, h] = (a * (2.0 ** -8 + 2 * es + 2 * (seen + 64) * 2.0 ** -24) + o.abs() * 2.0 ** -8) * 1.02
+                off = p @ (vd[:seen] - o).abs()
+                bound[t + i, h] = (off * 2.0 ** -8 + a * (2 * es + 2 * (seen + 64) * 2.0 ** -24) + o.abs() * 2.0 ** -8) * 1.02
         t, j = t + n, j + m
     return out, bound
 
