@@ -556,7 +556,7 @@ int rspx_pages_table(rspx_pages* p, const int32_t* ids, int n, int width, int32_
 int rspx_pages_slots(rspx_pages* p, const int32_t* ids, int n, const int64_t* first, const int64_t* counts, int32_t* out);
 
 /* ---------------------------------------------------------------- scores of given tokens
- * Per row of logits [M, V] (fp32, row stride sl, 16-byte aligned rows), with columns
+ * Per row of logits [M, V] (fp32, row stride sl, any 4-byte alignment), with columns
  * [off, off + size) counted as -inf: given[m] = log p of tokens[m], entropy[m] (nats),
  * and the `top` largest scores' log p (values [M, top], best first) and columns (ids
  * [M, top]).  Ties go to the lowest index, NaN is the largest value; a row that holds a

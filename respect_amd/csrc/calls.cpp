@@ -473,9 +473,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
       t->device() != x->device() || !integer(a[2], top) || !integer(a[3], off) || !integer(a[4], size))
     NOT_TAKEN;
   const int64_t M = x->size(0), V = x->size(1), s = x->stride(0);
-  if (top < 0 || V < 1 || s < V || s % 4 || reinterpret_cast<uintptr_t>(x->const_data_ptr()) % 16 || !fits_int(M) || !fits_int(V) ||
-      !fits_int(off) || !fits_int(size))
-    NOT_TAKEN;
+  if (top < 0 || V < 1 || s < V || !fits_int(M) || !fits_int(V) || !fits_int(off) || !fits_int(size)) NOT_TAKEN;
   const int k = (int)std::min(top, V);
   const int64_t need = rspx_token_logprobs_workspace_bytes((int)M, (int)V, k);
   if (need < 0) NOT_TAKEN;

@@ -36,6 +36,10 @@ constexpr int kMaxV = 1 << 30;                 // columns are counted in 32 bits
 constexpr int kGroups = 64;                    // groups of four threads
 constexpr float kL2E = 1.44269504088896340736f;
 
+// Four scores of a row that starts anywhere: rows of an odd vocabulary are read as they are, as
+// fast as aligned ones (1000 rows, top 5: of 50257 60.8 us, of 50256 60.2).
+typedef float row4 __attribute__((ext_vector_type(4), aligned(4)));
+
 // The order of the pairs as one unsigned number: larger is better.
 __device__ __forceinline__ uint64_t pair_key(float v, int j) {
   uint32_t u = __float_as_uint(v + 0.0f);                  // -0 and +0 tie
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogArgs A) {
     for (int i = 0; i < kPer / 4; ++i) {
       const int j = j0 + 256 * i;
       f32x4 v = {kNegInf, kNegInf, kNegInf, kNegInf};
-      if (j + 3 < A.V) v = *reinterpret_cast<const f32x4*>(xr + j);
+      if (j + 3 < A.V) v = *reinterpret_cast<const row4*>(xr + j);
       else
         for (int e = 0; e < 4; ++e)
           if (j + e < A.V) v[e] = xr[j + e];
@@ -419,7 +423,7 @@ extern "C" int rspx_token_logprobs(const float* logits, int64_t sl, int M, int V
   if (top > kMaxTop || V > kMaxV) return RSPX_EUNSUPPORTED;
   if (M == 0) return RSPX_OK;
   if (!logits || !tokens || !given || !entropy || (top && (!values || !ids))) return RSPX_EINVAL;
-  if ((reinterpret_cast<uintptr_t>(logits) & 15u) || sl % 4) return RSPX_EALIGN;
+  if (reinterpret_cast<uintptr_t>(logits) & 3u) return RSPX_EALIGN;
   if (!workspace || workspace_bytes < rspx_token_logprobs_workspace_bytes(M, V, top)) return RSPX_EWORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 7u) return RSPX_EALIGN;
   LogArgs A;

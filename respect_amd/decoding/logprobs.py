@@ -27,11 +27,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
         raise TypeError(f"token_logprobs: tokens must be int64 [{M}] on the GPU of the logits")
     if V == 0 or not 0 <= top <= MAX_TOP:
         raise ValueError(f"token_logprobs: V {V}, top {top} (0 to {MAX_TOP})")
-    if logits.stride(0) % 4 or logits.stride(0) < V or logits.data_ptr() % 16:
-        # rows that start 16-byte aligned
-        padded = torch.empty((M, -(-V // 4) * 4), dtype=torch.float32, device=logits.device)
-        padded[:, :V] = logits
-        logits = padded
+    if logits.stride(0) < V:   # rows that overlap
+        logits = logits.clone(memory_format=torch.contiguous_format)
     tokens = tokens.contiguous()
     dev, n = logits.device, min(top, V)
     given, entropy = torch.empty((2, M), dtype=torch.float32, device=dev)

@@ -51,7 +51,9 @@ def test_calls_equal_the_wrappers_own_path(monkeypatch):
         (False, lambda: paged_attn(q[:2], kc, kc, table.t().contiguous().t(), lens, 16)),
         (True, lambda: token_logprobs(x, t)),
         (True, lambda: token_logprobs(x, t, top=9, offset=3, size=40)),
-        (False, lambda: token_logprobs(x[:, 1:], t, top=9)),
+        (True, lambda: token_logprobs(x[:, 1:], t, top=9)),
+        (False, lambda: token_logprobs(x[:1].expand(3, 5000), t, top=9)),
+        (False, lambda: token_logprobs(x[0].as_strided((1, 5000), (0, 1)), t[:1], top=9)),
     ]
     native = _lib.calls()
     for taken, call in calls:
