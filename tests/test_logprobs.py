@@ -65,7 +65,7 @@ def test_refusals():
     assert call(M=-1) == -1 and call(V=0) == -1 and call(sl=96) == -1 and call(off=-1) == -1 and call(size=-1) == -1
     assert call(top=-1) == -1 and call(V=3, top=4) == -1 and call(p=0) == -1 and call(t=0) == -1
     assert call(top=65) == -2 and call(V=(1 << 30) + 4, sl=(1 << 30) + 4) == -2
-    assert call(p=8) == -4 and call(sl=101) == -4 and call(wp=20) == -4
+    assert call(p=18) == -4 and call(wp=20) == -4
     assert call(ws=64) == -3 and call(wp=0) == -3
     assert call(M=0) == 0
     assert L.rspx_token_logprobs_workspace_bytes(1, 0, 1) == -1
