@@ -620,6 +620,17 @@ PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// pages_free(handle, seqs) -> True
+PyObject* pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t h;
+  std::vector<int32_t> ids;
+  if (n != 2 || !integer(a[0], h) || h == 0 || !integers(a[1], ids)) NOT_TAKEN;
+  STATUS(rspx_pages_free(reinterpret_cast<rspx_pages*>(h), ids.data(), (int)ids.size()));
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // pages_tables(handle, seqs, *pool) -> (table, lens)
 PyObject* pages_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -667,7 +678,7 @@ PyMethodDef methods[] = {FAST(silu_mul), FAST(rmsnorm), FAST(qk_norm_rope), FAST
                          FAST(rope),     FAST(add_sq),  FAST(norm_apply),   FAST(rope_vision),
                          FAST(linear),   FAST(trie_attn), FAST(prompt_attn), FAST(paged_attn),
                          FAST(token_logprobs), FAST(pages_fork), FAST(pages_extend), FAST(pages_compact),
-                         FAST(pages_tables),   FAST(pages_slots), {nullptr, nullptr, 0, nullptr}};
+                         FAST(pages_tables),   FAST(pages_slots), FAST(pages_free), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -248,7 +248,11 @@ class PagedKVCache:
 
     def free(self, seqs) -> None:
         """Forget the sequences and give back their pages."""
-        self._t.free(seqs)
+        y = _lib.calls().pages_free(self._t.handle, seqs)
+        if y is None:
+            self._t.free(seqs)
+        else:
+            self._done("free", y)
 
     # ------------------------------------------------------------------ rows
 

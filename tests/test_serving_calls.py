@@ -113,6 +113,14 @@ def test_pages_calls_equal_the_wrappers_own_path(monkeypatch):
             with pytest.raises((ValueError, RuntimeError, OverflowError)) as e:
                 call()
             out.append(type(e.value))
+        for bad in ([77], [seqs[0], seqs[0]], [1 << 70]):
+            with pytest.raises((ValueError, RuntimeError, OverflowError)) as e:
+                c.free(bad)
+            out.append(type(e.value))
+        c.free(out[0][2:4])
+        c.free(tuple(seqs[:1]))
+        c.free([])
+        out += [c.free_pages, c.add([1, 1, 1])]
         return out, [t.clone() for t in c.k + c.v]
     a, ta = play()
     with monkeypatch.context() as m:
