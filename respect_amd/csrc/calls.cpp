@@ -546,6 +546,14 @@ int move_rows(const Pool& p) {
   int32_t groups = 0, moves = 0;
   rspx_pages_moves(p.pages, &groups, &moves);
   if (groups == 0) return RSPX_OK;
+  if ((int64_t)groups + 1 + 2 * (int64_t)moves <= RSPX_KV_MOVE_VALUES) {
+    int32_t lists[RSPX_KV_MOVE_VALUES];
+    rspx_pages_copy_moves(p.pages, lists);
+    return call([&] {
+      return rspx_kv_move_values(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel(), (int)p.HK, (int)p.D, p.sh,
+                                 p.sn, (int)p.cap, lists, groups, lists + groups + 1, moves, stream_of(*p.bases));
+    });
+  }
   Tensor t = uploaded(*p.bases, (int64_t)groups + 1 + 2 * (int64_t)moves, [&](int* out) { rspx_pages_copy_moves(p.pages, out); });
   return call([&] {
     const int32_t* d = t.const_data_ptr<int>();

@@ -221,6 +221,21 @@ def test_c_refusals():
     L.rspx_pages_delete(None)
 
 
+def test_c_refusals_of_moves_by_value():
+    from respect_amd import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    L = _lib.lib()
+
+    def move(n_tensors=2, HK=2, D=64, sh=4096, sn=64, cap=64, groups=16, ng=1, moves=16, nm=1, bases=16):
+        return L.rspx_kv_move_values(bases, n_tensors, HK, D, sh, sn, cap, groups, ng, moves, nm, None)
+    assert move(n_tensors=-1) == -1 and move(HK=0) == -1 and move(cap=-1) == -1 and move(ng=-1) == -1
+    assert move(nm=-1) == -1 and move(sn=32) == -1 and move(bases=0) == -1 and move(groups=0) == -1 and move(moves=0) == -1
+    assert move(D=12) == -2 and move(HK=70000) == -2 and move(sh=4100) == -4 and move(sn=68) == -4
+    assert move(ng=1, nm=480) == -2 and move(ng=960, nm=0) == -2 and move(nm=(1 << 31) - 1) == -2
+    assert move(ng=0) == 0 and move(nm=0) == 0 and move(n_tensors=0) == 0
+
+
 class _Model:
     """Every sequence's rows, as plain tensors [layers, 2, HK, n, D]."""
 
@@ -328,6 +343,68 @@ def test_long_groups_in_order_and_skipped_slots():
         if i in (0, 2):
             b[:, 9] = 1
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_groups,n_moves", [(1, 479), (3, 478), (1, 1), (5, 30)])
+def test_moves_by_value_are_the_moves(n_groups, n_moves):
+    """Lists that go with the launch, up to the most that do, in a captured launch too (the lists
+    changed behind it): the rows that the same lists on the device move.  Slots outside the
+    cache are skipped, groups that reach past the moves are cut."""
+    import numpy as np
+    from respect_amd import _lib
+    L, rng = _lib.lib(), np.random.default_rng(n_groups * 1000 + n_moves)
+    HK, cap, D = 2, 1024, 64
+    pools = [torch.randn(HK, cap, D, device="cuda").to(BF) for _ in range(4)]
+    slots = rng.permutation(cap)
+    moves = np.stack((slots[:n_moves], slots[n_moves:2 * n_moves]), 1).astype(np.int32)
+    if n_moves > 4:
+        moves[0, 0], moves[1, 1], moves[2, 0] = -1, cap, 1 << 30
+    groups = np.concatenate(([0], np.sort(rng.integers(0, n_moves + 1, n_groups - 1)), [n_moves + 7])).astype(np.int32)
+    flat = torch.from_numpy(np.concatenate((groups, moves.reshape(-1)))).cuda()
+
+    def run(pools, call, g, m):
+        bases = torch.tensor([t.data_ptr() for t in pools], device="cuda")
+        p = pools[0]
+        assert call(bases.data_ptr(), len(pools), HK, D, p.stride(0), p.stride(1), cap, g, n_groups, m, n_moves,
+                    _lib.stream_ptr(p.device)) == 0
+        return bases
+    want = [t.clone() for t in pools]
+    keep = run(want, L.rspx_kv_move, flat.data_ptr(), flat.data_ptr() + 4 * len(groups))
+    got = [t.clone() for t in pools]
+    run(got, L.rspx_kv_move_values, groups.ctypes.data, moves.ctypes.data)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert any(not torch.equal(a, b) for a, b in zip(got, pools)) or n_moves < 4
+    got = [t.clone() for t in pools]
+    bases = torch.tensor([t.data_ptr() for t in got], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert L.rspx_kv_move_values(bases.data_ptr(), 4, HK, D, got[0].stride(0), got[0].stride(1), cap, groups.ctypes.data,
+                                     n_groups, moves.ctypes.data, n_moves, _lib.stream_ptr(got[0].device)) == 0
+    groups[:], moves[:] = 0, 0
+    for _ in range(3):
+        for a, b in zip(got, pools):
+            a.copy_(b)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del keep
+
+
+@pytest.mark.gpu
+def test_fork_on_both_sides_of_what_goes_with_a_launch():
+    """Begun pages of 63 rows copied 7 and 8 times: 441 moves go with the launch, 504 do not."""
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    c = PagedKVCache(2, 2, 64, pages=40, page=64)
+    for t in c.k + c.v:
+        t.copy_(torch.randn(t.shape, device="cuda"))
+    s, = c.add([127])
+    want = [t[:, :127].clone() for t in c.k + c.v]
+    for copies in (7, 8):
+        forks = c.fork([s], copies)
+        for f in forks:
+            at = c.slots([f], 0, 127).long()
+            assert all(torch.equal(t[:, at], w) for t, w in zip(c.k + c.v, want))
+        c.free(forks)
 
 
 @pytest.mark.gpu
