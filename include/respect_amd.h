@@ -508,17 +508,19 @@ int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int
  * is the source of a later move of the group (rows moved down in increasing order are
  * that); different groups must not touch each other's destinations.  A move with a
  * slot outside [0, cap) is skipped.  D % 8 == 0.
- * rspx_kv_move_values: the same for lists in host memory of at most RSPX_KV_MOVE_VALUES
+ * rspx_kv_move_values: the same for lists in host memory of at most RSPX_VALUES
  * numbers in all (n_groups + 1 + 2 n_moves; RSPX_EUNSUPPORTED past it), which go with the
  * launch: read before the call returns.
+ * rspx_values: up to RSPX_VALUES numbers of host memory to out, likewise (tables, slots).
  * rspx_kv_write: rows k / v [T, HK, D] of one layer to slots[t] of its pools; a slot
  * outside [0, cap) is skipped; slots differ.
  */
 int rspx_kv_move(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh, int64_t sn, int cap,
                  const int32_t* groups, int n_groups, const int32_t* moves, int n_moves, void* stream);
-#define RSPX_KV_MOVE_VALUES 960
+#define RSPX_VALUES 960
 int rspx_kv_move_values(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh, int64_t sn, int cap,
                         const int32_t* groups, int n_groups, const int32_t* moves, int n_moves, void* stream);
+int rspx_values(const int32_t* values, int n, int32_t* out, void* stream);
 int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh,
                   const int32_t* slots, int T, int cap, void* cache_k, int64_t sckh, int64_t sckn, void* cache_v,
                   int64_t scvh, int64_t scvn, int HK, int D, void* stream);

@@ -96,6 +96,7 @@ SIGNATURES: dict[str, tuple] = {
                                _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _c_p, _i64, _c_p]),
     "rspx_kv_move": (_i32, [_c_p, _i32, _i32, _i32, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
     "rspx_kv_move_values": (_i32, [_c_p, _i32, _i32, _i32, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
+    "rspx_values": (_i32, [_c_p, _i32, _c_p, _c_p]),
     "rspx_kv_write": (_i32, [_c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i32, _i32, _c_p, _i64, _i64, _c_p, _i64, _i64,
                              _i32, _i32, _c_p]),
     "rspx_pages_new": (_c_p, [_i32, _i32, _i32]),

@@ -532,10 +532,17 @@ struct Pool {
   }
 };
 
-// int32 numbers that fill(host pointer) writes, on the device.  torch keeps the pinned
-// memory until the copy is done.
+// int32 numbers that fill(host pointer) writes, on the device: few with a launch, more by a
+// copy, whose pinned memory torch keeps until it is done.
 template <class F>
 Tensor uploaded(const Tensor& like, int64_t n, F&& fill) {
+  if (n <= RSPX_VALUES) {
+    int32_t values[RSPX_VALUES] = {};
+    fill(values);
+    Tensor t = empty_like_of(like, {n}, at::kInt);
+    TORCH_CHECK(call([&] { return rspx_values(values, (int)n, t.data_ptr<int>(), stream_of(like)); }) == RSPX_OK, "rspx_values");
+    return t;
+  }
   Tensor host = at::empty({n}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
   fill(host.data_ptr<int>());
   return host.to(like.device(), at::kInt, /*non_blocking=*/true);
@@ -546,8 +553,8 @@ int move_rows(const Pool& p) {
   int32_t groups = 0, moves = 0;
   rspx_pages_moves(p.pages, &groups, &moves);
   if (groups == 0) return RSPX_OK;
-  if ((int64_t)groups + 1 + 2 * (int64_t)moves <= RSPX_KV_MOVE_VALUES) {
-    int32_t lists[RSPX_KV_MOVE_VALUES];
+  if ((int64_t)groups + 1 + 2 * (int64_t)moves <= RSPX_VALUES) {
+    int32_t lists[RSPX_VALUES];
     rspx_pages_copy_moves(p.pages, lists);
     return call([&] {
       return rspx_kv_move_values(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel(), (int)p.HK, (int)p.D, p.sh,

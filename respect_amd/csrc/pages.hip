@@ -61,12 +61,18 @@ __global__ __launch_bounds__(kThreads) void kv_move_kernel(const uint64_t* bases
 // The lists among the kernel's arguments: no copy to the device ahead of the launch (one prompt
 // forked 4 times, with its tables and the forks freed: 16.0 us instead of 24.2; 32 paths of 13
 // moved rows: 36.5 instead of 44).
-struct MoveLists {
-  int x[RSPX_KV_MOVE_VALUES];
+struct Values {
+  int x[RSPX_VALUES];
 };
 __global__ __launch_bounds__(kThreads) void kv_move_values_kernel(const uint64_t* bases, int64_t sh, int64_t sn, int U, int cap,
-                                                                  int n_groups, int n_moves, MoveLists lists) {
+                                                                  int n_groups, int n_moves, Values lists) {
   move_group(bases, sh, sn, U, cap, lists.x, lists.x + n_groups + 1, n_moves, 0);
+}
+
+// Tables and slots of a few sequences, likewise (the two calls above: 12.0 us and 32).
+__global__ __launch_bounds__(kThreads) void values_kernel(int* out, int n, Values values) {
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  if (i < n) out[i] = values.x[i];
 }
 
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v,
@@ -106,14 +112,27 @@ static int check_move(const uint64_t* bases, int n_tensors, int HK, int D, int64
 extern "C" int rspx_kv_move_values(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh, int64_t sn, int cap,
                                    const int32_t* groups, int n_groups, const int32_t* moves, int n_moves, void* stream) {
   if (const int rc = check_move(bases, n_tensors, HK, D, sh, sn, cap, groups, n_groups, moves, n_moves)) return rc;
-  if ((int64_t)n_groups + 1 + 2 * (int64_t)n_moves > RSPX_KV_MOVE_VALUES) return RSPX_EUNSUPPORTED;
+  if ((int64_t)n_groups + 1 + 2 * (int64_t)n_moves > RSPX_VALUES) return RSPX_EUNSUPPORTED;
   if (n_groups == 0 || n_moves == 0 || n_tensors == 0) return RSPX_OK;
-  MoveLists lists;
+  Values lists;
   std::copy(groups, groups + n_groups + 1, lists.x);
   std::copy(moves, moves + 2 * n_moves, lists.x + n_groups + 1);
-  std::fill(lists.x + n_groups + 1 + 2 * n_moves, lists.x + RSPX_KV_MOVE_VALUES, 0);
+  std::fill(lists.x + n_groups + 1 + 2 * n_moves, lists.x + RSPX_VALUES, 0);
   hipLaunchKernelGGL(kv_move_values_kernel, dim3(n_groups, HK, n_tensors), dim3(kThreads), 0,
                      static_cast<hipStream_t>(stream), bases, sh, sn, D / 8, cap, n_groups, n_moves, lists);
+  return hipGetLastError() == hipSuccess ? RSPX_OK : RSPX_ELAUNCH;
+}
+
+extern "C" int rspx_values(const int32_t* values, int n, int32_t* out, void* stream) {
+  if (n < 0) return RSPX_EINVAL;
+  if (n > RSPX_VALUES) return RSPX_EUNSUPPORTED;
+  if (n == 0) return RSPX_OK;
+  if (!values || !out) return RSPX_EINVAL;
+  if (reinterpret_cast<uintptr_t>(out) & 3u) return RSPX_EALIGN;
+  Values v;
+  std::fill(std::copy(values, values + n, v.x), v.x + RSPX_VALUES, 0);
+  hipLaunchKernelGGL(values_kernel, dim3((n + kThreads - 1) / kThreads), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
+                     out, n, v);
   return hipGetLastError() == hipSuccess ? RSPX_OK : RSPX_ELAUNCH;
 }
 

@@ -234,6 +234,9 @@ def test_c_refusals_of_moves_by_value():
     assert move(D=12) == -2 and move(HK=70000) == -2 and move(sh=4100) == -4 and move(sn=68) == -4
     assert move(ng=1, nm=480) == -2 and move(ng=960, nm=0) == -2 and move(nm=(1 << 31) - 1) == -2
     assert move(ng=0) == 0 and move(nm=0) == 0 and move(n_tensors=0) == 0
+    assert L.rspx_values(16, -1, 16, None) == -1 and L.rspx_values(None, 1, 16, None) == -1
+    assert L.rspx_values(16, 1, None, None) == -1 and L.rspx_values(16, 961, 16, None) == -2
+    assert L.rspx_values(16, 1, 18, None) == -4 and L.rspx_values(None, 0, None, None) == 0
 
 
 class _Model:
@@ -388,6 +391,29 @@ def test_moves_by_value_are_the_moves(n_groups, n_moves):
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     del keep
+
+
+@pytest.mark.gpu
+def test_tables_and_slots_on_both_sides_of_what_goes_with_a_launch():
+    """Tables and slots of up to 960 numbers and of more, several of them before any is looked at:
+    what the books say, and nothing past the numbers is written."""
+    import numpy as np
+    from respect_amd import _lib
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    c = PagedKVCache(1, 1, 8, pages=1300, page=4)
+    seqs = c.add([956, 3836, 1])
+    took = [(s, c.tables(s), c._t.table(s)) for s in ([seqs[0]], seqs[1:2], seqs, [], seqs[2:])]
+    for s, (table, lens), (want, n) in took:   # 240, 960, 2880, 0 and 2 numbers
+        assert table.cpu().numpy().tolist() == want.tolist() and lens.tolist() == n.tolist()
+    slots = [(k, c.slots([seqs[1]], 5, k), c._t.slots([seqs[1]], 5, k)) for k in (0, 1, 255, 256, 257, 959, 960, 961, 3000)]
+    for k, got, want in slots:
+        assert got.tolist() == want.tolist() and len(want) == k
+    out = torch.full((1000,), 7, dtype=torch.int32, device="cuda")
+    v = np.arange(960, dtype=np.int32)
+    for n in (1, 300, 960):
+        out.fill_(7)
+        assert _lib.lib().rspx_values(v.ctypes.data, n, out.data_ptr(), _lib.stream_ptr(out.device)) == 0
+        assert out[:n].tolist() == list(range(n)) and (out[n:] == 7).all()
 
 
 @pytest.mark.gpu
