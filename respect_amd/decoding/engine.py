@@ -82,6 +82,20 @@ def _reach(n: int) -> int:
     return 1 << max(10, (n - 1).bit_length())
 
 
+class _CallScratch:
+    """Scratch of one call, from torch: no other call's, on whatever stream that runs, and given
+    back at the end."""
+
+    def __init__(self, device):
+        self.device, self._held = device, {}
+
+    def __call__(self, name: str, nbytes: int) -> torch.Tensor:
+        t = self._held.get(name)
+        if t is None or t.numel() < nbytes:
+            t = self._held[name] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return t
+
+
 class Layer:
     """One decoder layer.  The projections are held tiled (``t*``, what the
     kernels read); ``wqkv``, ``wo``, ``wgu`` and ``wd`` give them back as
@@ -159,7 +173,8 @@ class Decoder:
 
     def _workspace(self, name: str, nbytes: int) -> torch.Tensor:
         """Scratch owned by the model, grown (never while a graph is being
-        captured) so that captured kernels keep pointing at live memory."""
+        captured) so that captured kernels keep pointing at live memory.  ``forward``,
+        ``prefill`` and their graphs share it: they run on one stream at a time."""
         ws = self._ws.get(name)
         if ws is None or ws.numel() < nbytes:
             if torch.cuda.is_current_stream_capturing():
@@ -188,26 +203,27 @@ class Decoder:
         idx = positions.clamp(0, t[0].shape[0] - 1)
         return t[0].index_select(0, idx), t[1].index_select(0, idx)
 
-    def _linear(self, x: int, sx: int, M: int, w: TiledWeight, out_dtype=torch.bfloat16) -> torch.Tensor:
-        """x (device pointer, row stride sx or RSPX_TILED, M rows) . w^T."""
+    def _linear(self, x: int, sx: int, M: int, w: TiledWeight, out_dtype=torch.bfloat16, scratch=None) -> torch.Tensor:
+        """x (device pointer, row stride sx or RSPX_TILED, M rows) . w^T.  ``scratch(name, bytes)``:
+        where its scratch comes from, the model's own by default."""
         L = _lib.lib()
         N, K = w.shape
         need = L.rspx_linear_workspace_bytes(M, N, K)
-        ws = self._workspace("linear", max(need, 16))
+        ws = (scratch or self._workspace)("linear", max(need, 16))
         out = torch.empty((M, N), dtype=out_dtype, device=self.device)
         _lib.check("rspx_linear", L.rspx_linear(
             x, sx, w.data_ptr(), w.stride(0), out.data_ptr(), out.stride(0), M, N, K,
             1 if out_dtype == torch.float32 else 0, ws.data_ptr(), ws.numel(), _lib.stream_ptr(self.device)))
         return out
 
-    def _partials(self, x: int, sx: int, M: int, w: TiledWeight) -> tuple[int, int]:
+    def _partials(self, x: int, sx: int, M: int, w: TiledWeight, scratch) -> tuple[int, int]:
         """x (device pointer, row stride sx or RSPX_TILED, M rows) . w^T left as
-        fp32 chunk partials in the model's partial buffer; returns (pointer,
+        fp32 chunk partials in ``scratch``'s partial buffer; returns (pointer,
         chunk count) for a consumer that sums them."""
         L = _lib.lib()
         N, K = w.shape
         S = L.rspx_linear_splits(N, K)
-        buf = self._workspace("partials", S * M * N * 4)
+        buf = scratch("partials", S * M * N * 4)
         _lib.check("rspx_linear_partials", L.rspx_linear_partials(
             x, sx, w.data_ptr(), w.stride(0), buf.data_ptr(), M, N, K, _lib.stream_ptr(self.device)))
         return buf.data_ptr(), S
@@ -246,13 +262,14 @@ class Decoder:
             return att.data_ptr(), _lib.RSPX_TILED
 
         return self._stack(ids, slots.to(torch.int32), positions, cache.cap,
-                           lambda li: (cache.k[li], cache.v[li], cache.cap), attend, kv_only)
+                           lambda li: (cache.k[li], cache.v[li], cache.cap), attend, self._workspace, kv_only)
 
-    def _stack(self, ids, slots32, positions, reach: int, kv, attend, kv_only: bool = False) -> torch.Tensor | None:
+    def _stack(self, ids, slots32, positions, reach: int, kv, attend, scratch,
+               kv_only: bool = False) -> torch.Tensor | None:
         """Every layer over the tokens ``ids``, whose positions lie below ``reach``.  ``kv(layer)``:
         (K [HK, cap, D], V, cap), where a token's K/V go to slots32 of it; ``attend(layer, q
         [T, HQ, D])``, once they are written: the attention's result as the o projection's x
-        (device pointer, row stride)."""
+        (device pointer, row stride); ``scratch``: as for ``_linear``."""
         cfg = self.cfg
         L = _lib.lib()
         dev = self.device
@@ -271,7 +288,7 @@ class Decoder:
         mlp = torch.empty(rows * cfg.ffn, dtype=bf, device=dev)  # SwiGLU output [T, F], tiled when fused
         for li, lay in enumerate(self.layers):
             ck, cv, cap = kv(li)
-            qkvp, S = self._partials(y.data_ptr(), TILED, T, lay.tqkv)
+            qkvp, S = self._partials(y.data_ptr(), TILED, T, lay.tqkv, scratch)
             _lib.check("rspx_qkv_rope_cache_partials", L.rspx_qkv_rope_cache_partials(
                 qkvp, S, lay.q_norm.data_ptr(), lay.k_norm.data_ptr(), cos.data_ptr(),
                 sin.data_ptr(), cos.stride(0), slots32.data_ptr(), cap, ck.data_ptr(), ck.stride(0), ck.stride(1),
@@ -279,7 +296,7 @@ class Decoder:
             if kv_only and li + 1 == len(self.layers):
                 return None
             ax, sax = attend(li, qo)
-            hp, S = self._partials(ax, sax, T, lay.tout)
+            hp, S = self._partials(ax, sax, T, lay.tout, scratch)
             _lib.check("rspx_add_rmsnorm_partials", L.rspx_add_rmsnorm_partials(
                 x.data_ptr(), Hd, hp, S, lay.post_norm.data_ptr(), x.data_ptr(), Hd, y.data_ptr(), TILED,
                 T, Hd, cfg.eps, s))
@@ -290,11 +307,11 @@ class Decoder:
                     TILED, T, 2 * F, Hd, s))
                 msx = TILED
             else:
-                gu = self._linear(y.data_ptr(), TILED, T, lay.tgu)
+                gu = self._linear(y.data_ptr(), TILED, T, lay.tgu, scratch=scratch)
                 _lib.check("rspx_silu_mul", L.rspx_silu_mul(gu.data_ptr(), gu.stride(0), gu.data_ptr() + 2 * F,
                                                             gu.stride(0), mlp.data_ptr(), F, T, F, s))
                 msx = F
-            hp, S = self._partials(mlp.data_ptr(), msx, T, lay.tdown)
+            hp, S = self._partials(mlp.data_ptr(), msx, T, lay.tdown, scratch)
             nxt = self.layers[li + 1].in_norm if li + 1 < len(self.layers) else self.final_norm
             _lib.check("rspx_add_rmsnorm_partials", L.rspx_add_rmsnorm_partials(
                 x.data_ptr(), Hd, hp, S, nxt.data_ptr(), x.data_ptr(), Hd, y.data_ptr(), TILED,
@@ -332,7 +349,9 @@ class Decoder:
         """New sequences of the PagedKVCache ``cache`` holding ``prompts`` (1-D token tensors on the
         GPU, none empty), all in one pass.  Returns (sequences, logits [B, V] of each prompt's
         last token).  A prompt's results do not depend on the others; its attention runs in
-        ``prompt_attn``'s order, so its bits are not those of ``prefill``."""
+        ``prompt_attn``'s order, so its bits are not those of ``prefill``.  The pass takes scratch
+        in proportion to all tokens (98 KB each at the 8B sizes), which goes back to torch with
+        its end."""
         self._check_paged(cache)
         rows = [int(p.shape[0]) for p in prompts]
         if not rows or min(rows) < 1:
@@ -353,12 +372,14 @@ class Decoder:
                 prompt_attn(qo, kt, vt, plan, self.sm_scale, out=att)
                 return att.data_ptr(), cfg.heads * cfg.head_dim
 
+            scratch = _CallScratch(dev)
             y = self._stack(ids, torch.arange(T, dtype=torch.int32, device=dev), positions, _reach(max(rows)),
-                            lambda li: (k, v, T), attend)
+                            lambda li: (k, v, T), attend, scratch)
             # the last rows of the tiled rows (RSPX_TILED): elements 32 b + 8 g + e at [b, g, e]
             m = torch.tensor(rows, device=dev).cumsum(0) - 1
             last = y.view(-1, cfg.hidden // 32, 4, 4, 16, 8)[m // 64, :, m % 64 // 16, :, m % 16].reshape(len(rows), -1)
-            return seqs, self._linear(last.data_ptr(), last.stride(0), len(rows), self.t_lm_head, out_dtype=torch.float32)
+            return seqs, self._linear(last.data_ptr(), last.stride(0), len(rows), self.t_lm_head, out_dtype=torch.float32,
+                                      scratch=scratch)
         except BaseException:
             cache.free(seqs)
             raise
@@ -391,9 +412,10 @@ class Decoder:
             paged_attn(qo, cache.k[li], cache.v[li], table, lens, cache.page, self.sm_scale, out=att)
             return att.data_ptr(), cfg.heads * cfg.head_dim
 
+        scratch = _CallScratch(self.device)
         y = self._stack(ids, slots, lens - 1, _reach(max(n)), lambda li: (cache.k[li], cache.v[li], cache.pages * cache.page),
-                        attend)
-        return self._linear(y.data_ptr(), _lib.RSPX_TILED, B, self.t_lm_head, out_dtype=torch.float32)
+                        attend, scratch)
+        return self._linear(y.data_ptr(), _lib.RSPX_TILED, B, self.t_lm_head, out_dtype=torch.float32, scratch=scratch)
 
     def _check_paged(self, cache) -> None:
         c = self.cfg

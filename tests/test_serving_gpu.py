@@ -104,6 +104,55 @@ def test_forks_rejected_tokens_and_pages(model):
     assert cache.free_pages == 80
 
 
+def test_growing_batches_leave_no_memory_behind(model):
+    """Batches that each set a new record: the model keeps rotary tables (256 bytes a position and
+    table, doubled as they grow: 4 MB at 4096) and no scratch (32 KB a token)."""
+    cache = _cache(pages=300)
+    cache.free(model.prefill_batch(_prompts([20]), cache)[0])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for n in (500, 1000, 2000, 4000):
+        seqs, logits = model.prefill_batch(_prompts([n, 7]), cache)
+        model.step_batch(torch.tensor([1, 2], device="cuda"), cache, seqs)
+        cache.free(seqs)
+        del logits
+        assert torch.cuda.memory_allocated() - before < 8 << 20, n
+
+
+def test_two_streams_at_once(model):
+    """Steps of two batches and a prefill, enqueued on two streams behind work that holds both back:
+    the bits of the same calls one after the other."""
+    def start():
+        cache = _cache(pages=400)
+        return cache, [model.prefill_batch(_prompts(lens, seed), cache)[0] for seed, lens in ((1, [90, 400]), (2, [33, 5, 300]))]
+
+    def calls(cache, seqs, which, step):
+        tok = torch.arange(len(seqs[which]), device="cuda") + 10 * step + which
+        if step == 3 and which:
+            return model.prefill_batch(_prompts([170, 60], seed=9), cache)[1]
+        return model.step_batch(tok, cache, seqs[which])
+    cache, seqs = start()
+    want = [[calls(cache, seqs, w, i) for w in (0, 1)] for i in range(6)]
+    cache, seqs = start()
+    a = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            for _ in range(8):
+                torch.mm(a, a)
+    got = []
+    for i in range(6):
+        got.append([])
+        for w in (0, 1):
+            with torch.cuda.stream(streams[w]):
+                got[-1].append(calls(cache, seqs, w, i))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for w in (0, 1):
+            assert torch.equal(got[i][w], want[i][w]), (i, w)
+
+
 def test_refusals(model):
     from respect_amd.decoding.paged_kv import PagedKVCache
     cache = _cache()
