@@ -199,6 +199,7 @@ class Decoder:
                 self._ws_retired.append(t)
             cfg = self.cfg
             t = rope_tables(torch.arange(cap, device=self.device), cfg.head_dim, cfg.theta, device=self.device)
+            torch.cuda.current_stream(self.device).synchronize()   # the next call may run on another stream
             self._rope = t
         idx = positions.clamp(0, t[0].shape[0] - 1)
         return t[0].index_select(0, idx), t[1].index_select(0, idx)

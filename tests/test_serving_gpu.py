@@ -153,6 +153,31 @@ def test_two_streams_at_once(model):
             assert torch.equal(got[i][w], want[i][w]), (i, w)
 
 
+def test_tables_made_on_one_stream_serve_another(model):
+    """The call that makes the rotary tables runs on a stream held back; the next one runs on another
+    stream at once."""
+    def start():
+        cache = _cache(pages=40)
+        return cache, [model.prefill_batch(_prompts([n], n), cache)[0] for n in (90, 200)]
+    tok = torch.tensor([3], device="cuda")
+    cache, seqs = start()
+    want = [model.step_batch(tok, cache, s) for s in seqs]
+    cache, seqs = start()
+    model._rope = None
+    a = torch.randn(4096, 4096, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        for _ in range(8):
+            torch.mm(a, a)
+    got = []
+    for stream, s in zip(streams, seqs):
+        with torch.cuda.stream(stream):
+            got.append(model.step_batch(tok, cache, s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_refusals(model):
     from respect_amd.decoding.paged_kv import PagedKVCache
     cache = _cache()
