@@ -538,6 +538,8 @@ int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_
  *   compact  row starts[i] + path[k] becomes row starts[i] + k, and the sequence ends after
  *            them; its pages stay with it.  Path i is paths[ends[i - 1] .. ends[i]), increasing
  *   trim     the pages past the end are given back;  free: the sequences are forgotten
+ *   undo     the last extend, fork or compact taken back (nothing, once add, trim, free or a
+ *            refused call came after it), for a caller whose moves could not be enqueued
  * The rows that a call makes move on the device are its moves: rspx_pages_moves gives their
  * number and that of their groups, rspx_pages_copy_moves writes groups [n_groups + 1] and
  * then moves [n_moves][2], as rspx_kv_move takes them (nothing at all for no group).
@@ -557,6 +559,7 @@ int rspx_pages_compact(rspx_pages* p, const int32_t* ids, int n, const int64_t* 
                        const int64_t* ends);
 int rspx_pages_trim(rspx_pages* p, const int32_t* ids, int n);
 int rspx_pages_free(rspx_pages* p, const int32_t* ids, int n);
+int rspx_pages_undo(rspx_pages* p);
 int rspx_pages_moves(const rspx_pages* p, int32_t* n_groups, int32_t* n_moves);
 int rspx_pages_copy_moves(const rspx_pages* p, int32_t* out);
 int rspx_pages_width(rspx_pages* p, const int32_t* ids, int n);

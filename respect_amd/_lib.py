@@ -109,6 +109,7 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_pages_compact": (_i32, [_c_p, _c_p, _i32, _c_p, _c_p, _c_p]),
     "rspx_pages_trim": (_i32, [_c_p, _c_p, _i32]),
     "rspx_pages_free": (_i32, [_c_p, _c_p, _i32]),
+    "rspx_pages_undo": (_i32, [_c_p]),
     "rspx_pages_moves": (_i32, [_c_p, _c_p, _c_p]),
     "rspx_pages_copy_moves": (_i32, [_c_p, _c_p]),
     "rspx_pages_width": (_i32, [_c_p, _c_p, _i32]),

@@ -549,7 +549,7 @@ Tensor uploaded(const Tensor& like, int64_t n, F&& fill) {
 }
 
 // Enqueues the moves of the call just made.
-int move_rows(const Pool& p) {
+int enqueue_moves(const Pool& p) {
   int32_t groups = 0, moves = 0;
   rspx_pages_moves(p.pages, &groups, &moves);
   if (groups == 0) return RSPX_OK;
@@ -567,6 +567,18 @@ int move_rows(const Pool& p) {
     return rspx_kv_move(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel(), (int)p.HK, (int)p.D, p.sh, p.sn,
                         (int)p.cap, d, groups, d + groups + 1, moves, stream_of(*p.bases));
   });
+}
+
+// The same; where it fails (no memory for the lists, a refused launch) the call is taken back.
+int move_rows(const Pool& p) {
+  try {
+    const int rc = enqueue_moves(p);
+    if (rc != RSPX_OK) rspx_pages_undo(p.pages);
+    return rc;
+  } catch (...) {
+    rspx_pages_undo(p.pages);
+    throw;
+  }
 }
 
 PyObject* list_of(const std::vector<int32_t>& v) {
@@ -595,7 +607,9 @@ PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   std::vector<int32_t> out(ids.size() * copies);
   STATUS(rspx_pages_fork(p.pages, ids.data(), (int)ids.size(), (int)copies, out.data()));
   STATUS(move_rows(p));
-  return list_of(out);
+  PyObject* l = list_of(out);
+  if (!l) rspx_pages_undo(p.pages);
+  return l;
   END_HANDLE_TH_ERRORS
 }
 

@@ -3,7 +3,8 @@
 // Pages are counted (a page that several sequences share is held by each of them) and taken
 // lowest first.  A call checks everything and reserves what it needs before it changes
 // anything, so a refused one leaves the table as it was; the rows that have to move on the
-// device are left as (source slot, destination slot) pairs in groups for rspx_kv_move.
+// device are left as (source slot, destination slot) pairs in groups for rspx_kv_move.  What a
+// call changed is noted, so that it can be taken back where its rows could not be moved.
 #include <stdint.h>
 
 #include <algorithm>
@@ -22,6 +23,15 @@ struct rspx_pages {
   uint32_t stamp = 0;
   std::vector<int32_t> groups, moves; // of the last call
   std::vector<int32_t> left;          // pages that the call gives up
+  struct Before {
+    int32_t seq, pages;
+    int64_t len;
+  };
+  struct Own {
+    int32_t seq, at, old;             // held[seq][at] was `old`
+  };
+  std::vector<Before> before;         // of the last call: its sequences as they were,
+  std::vector<Own> owned;             // and the shared pages that they left
 };
 
 namespace {
@@ -61,10 +71,15 @@ void drop(Pages& p, int32_t page) {
   }
 }
 
-void clear_moves(Pages& p) {
+// A call's begin: the last one's moves and notes are forgotten.
+void begin(Pages& p) {
   p.groups.clear();
   p.moves.clear();
+  p.before.clear();
+  p.owned.clear();
 }
+
+void note(Pages& p, int32_t seq) { p.before.push_back({seq, (int32_t)p.held[seq].size(), p.len[seq]}); }
 
 int32_t slot(const Pages& p, const std::vector<int32_t>& held, int64_t row) {
   return held[row / p.page] * p.page + (int32_t)(row % p.page);
@@ -79,16 +94,18 @@ int64_t shared(const Pages& p, const std::vector<int32_t>& held, int64_t lo, int
 }
 
 // Gives the sequence pages of its own where it shares the ones with rows in [lo, hi), and
-// copies the rows before lo that they hold.  Room for pages and moves is there.  The pages
+// copies the rows before lo that they hold.  Room for pages, moves and notes is there.  The pages
 // left count as held until the call ends (leave): what its moves read is neither taken nor,
 // by another sequence of the call that holds it then alone, written.
-void own(Pages& p, std::vector<int32_t>& held, int64_t lo, int64_t hi) {
+void own(Pages& p, int32_t seq, int64_t lo, int64_t hi) {
+  std::vector<int32_t>& held = p.held[seq];
   if (hi <= lo) return;
   for (int64_t i = lo / p.page; i < std::min<int64_t>(pages_for(p, hi), held.size()); ++i) {
     const int32_t old = held[i];
     if (p.refs[old] <= 1) continue;
     held[i] = take(p);
     p.left.push_back(old);
+    p.owned.push_back({seq, (int32_t)i, old});
     for (int64_t r = 0; r < std::min<int64_t>(p.page, lo - i * p.page); ++r) {
       p.moves.push_back(old * p.page + (int32_t)r);
       p.moves.push_back(held[i] * p.page + (int32_t)r);
@@ -149,7 +166,7 @@ extern "C" int64_t rspx_pages_length(const rspx_pages* p, int seq) {
 extern "C" int rspx_pages_add(rspx_pages* p, const int64_t* lengths, int n, int32_t* ids) {
   if (!p || n < 0 || (n > 0 && (!lengths || !ids))) return RSPX_EINVAL;
   return guarded([&] {
-    clear_moves(*p);
+    begin(*p);
     int64_t need = 0;
     for (int i = 0; i < n; ++i) {
       if (lengths[i] < 0) return RSPX_EINVAL;
@@ -175,7 +192,7 @@ extern "C" int rspx_pages_add(rspx_pages* p, const int64_t* lengths, int n, int3
 extern "C" int rspx_pages_extend(rspx_pages* p, const int32_t* ids, int n, const int64_t* counts) {
   if (!p || (n > 0 && !counts)) return RSPX_EINVAL;
   return guarded([&] {
-    clear_moves(*p);
+    begin(*p);
     if (const int rc = check_ids(*p, ids, n, true)) return rc;
     int64_t need = 0, copied = 0;
     for (int i = 0; i < n; ++i) {
@@ -191,10 +208,13 @@ extern "C" int rspx_pages_extend(rspx_pages* p, const int32_t* ids, int n, const
     p->moves.reserve(2 * copied * p->page);
     p->groups.reserve(n + 1);
     p->left.reserve(copied);
+    p->owned.reserve(copied);
+    p->before.reserve(n);
     for (int i = 0; i < n; ++i) {
       std::vector<int32_t>& held = p->held[ids[i]];
       int64_t& len = p->len[ids[i]];
-      own(*p, held, len, len + counts[i]);
+      note(*p, ids[i]);
+      own(*p, ids[i], len, len + counts[i]);
       end_group(*p);
       len += counts[i];
       while ((int64_t)held.size() < pages_for(*p, len)) held.push_back(take(*p));
@@ -207,7 +227,7 @@ extern "C" int rspx_pages_extend(rspx_pages* p, const int32_t* ids, int n, const
 extern "C" int rspx_pages_fork(rspx_pages* p, const int32_t* ids, int n, int copies, int32_t* out) {
   if (!p || copies < 0 || (n > 0 && copies > 0 && !out)) return RSPX_EINVAL;
   return guarded([&] {
-    clear_moves(*p);
+    begin(*p);
     if (const int rc = check_ids(*p, ids, n, false)) return rc;
     const int64_t all = (int64_t)n * copies;
     if (all > (int64_t)p->len.size()) return RSPX_EFULL;
@@ -227,8 +247,10 @@ extern "C" int rspx_pages_fork(rspx_pages* p, const int32_t* ids, int n, int cop
     if (got < all) return RSPX_EFULL;
     p->moves.reserve(2 * rows);
     p->groups.reserve(all + 1);
+    p->before.reserve(all);
     for (int64_t k = 0; k < all; ++k) {
       const int32_t src = ids[k / copies];
+      note(*p, out[k]);
       std::vector<int32_t>& held = p->held[out[k]];
       const int64_t len = p->len[src], whole = len / p->page, begun = len % p->page;
       for (int64_t i = 0; i < whole; ++i) {
@@ -254,7 +276,7 @@ extern "C" int rspx_pages_compact(rspx_pages* p, const int32_t* ids, int n, cons
                                   const int64_t* ends) {
   if (!p || (n > 0 && (!starts || !ends))) return RSPX_EINVAL;
   return guarded([&] {
-    clear_moves(*p);
+    begin(*p);
     if (const int rc = check_ids(*p, ids, n, true)) return rc;
     int64_t need = 0, rows = 0;
     for (int i = 0; i < n; ++i) {
@@ -273,9 +295,12 @@ extern "C" int rspx_pages_compact(rspx_pages* p, const int32_t* ids, int n, cons
     p->moves.reserve(2 * rows);
     p->groups.reserve(n + 1);
     p->left.reserve(need);
+    p->owned.reserve(need);
+    p->before.reserve(n);
     for (int i = 0; i < n; ++i) {
       const int64_t a = i ? ends[i - 1] : 0, b = ends[i];
       std::vector<int32_t>& held = p->held[ids[i]];
+      note(*p, ids[i]);
       int64_t still = 0;
       while (a + still < b && paths[a + still] == still) ++still;
       // Sources in the pages as they were: a shared one is copied from, never written.  Every
@@ -287,7 +312,7 @@ extern "C" int rspx_pages_compact(rspx_pages* p, const int32_t* ids, int n, cons
         p->moves.push_back(0);
       }
       const size_t last = p->moves.size();
-      own(*p, held, starts[i] + still, starts[i] + b - a);
+      own(*p, ids[i], starts[i] + still, starts[i] + b - a);
       for (size_t m = first, k = still; m < last; m += 2, ++k) p->moves[m + 1] = slot(*p, held, starts[i] + (int64_t)k);
       end_group(*p);
       p->len[ids[i]] = starts[i] + b - a;
@@ -299,7 +324,7 @@ extern "C" int rspx_pages_compact(rspx_pages* p, const int32_t* ids, int n, cons
 
 extern "C" int rspx_pages_trim(rspx_pages* p, const int32_t* ids, int n) {
   if (!p) return RSPX_EINVAL;
-  clear_moves(*p);
+  begin(*p);
   if (const int rc = check_ids(*p, ids, n, true)) return rc;
   for (int i = 0; i < n; ++i) {
     std::vector<int32_t>& held = p->held[ids[i]];
@@ -313,13 +338,33 @@ extern "C" int rspx_pages_trim(rspx_pages* p, const int32_t* ids, int n) {
 
 extern "C" int rspx_pages_free(rspx_pages* p, const int32_t* ids, int n) {
   if (!p) return RSPX_EINVAL;
-  clear_moves(*p);
+  begin(*p);
   if (const int rc = check_ids(*p, ids, n, true)) return rc;
   for (int i = 0; i < n; ++i) {
     for (const int32_t page : p->held[ids[i]]) drop(*p, page);
     p->held[ids[i]].clear();
     p->len[ids[i]] = -1;
   }
+  return RSPX_OK;
+}
+
+// Every page's count is what it was, hence so are the free pages; `lowest` may lie lower.
+extern "C" int rspx_pages_undo(rspx_pages* p) {
+  if (!p) return RSPX_EINVAL;
+  for (size_t i = p->owned.size(); i-- > 0;) {
+    const rspx_pages::Own& o = p->owned[i];
+    int32_t& page = p->held[o.seq][o.at];
+    if (p->refs[o.old]++ == 0) --p->free_pages;
+    drop(*p, page);
+    page = o.old;
+  }
+  for (size_t i = p->before.size(); i-- > 0;) {
+    const rspx_pages::Before& b = p->before[i];
+    std::vector<int32_t>& held = p->held[b.seq];
+    for (; (int32_t)held.size() > b.pages; held.pop_back()) drop(*p, held.back());
+    p->len[b.seq] = b.len;
+  }
+  begin(*p);
   return RSPX_OK;
 }
 

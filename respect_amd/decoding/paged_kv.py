@@ -112,6 +112,11 @@ class PageTable:
         ids = self._ids(seqs)
         self._call("free", _p(ids), len(ids))
 
+    def undo(self) -> None:
+        """Take back the last extend, fork or compact, if no other call that changes the table
+        came after it."""
+        self._call("undo")
+
     def moves(self) -> tuple[np.ndarray, np.ndarray]:
         """(groups [g + 1], moves [m, 2]) that the last call makes rows move by."""
         g, m = ctypes.c_int32(), ctypes.c_int32()
@@ -145,9 +150,9 @@ class PagedKVCache:
     time.  Sequences are named by the numbers that ``add`` and ``fork`` give.  The methods
     keep books on the host and enqueue their copies on the current stream; those that do
     cannot be captured into a graph.  Pages given back are taken again at once: calls that
-    still read them have to be on the same stream, or waited for.  A refused call
-    (``ValueError``; ``RuntimeError`` for too few pages or sequences) changes nothing.  One
-    thread at a time."""
+    still read them have to be on the same stream, or waited for.  A call that is refused
+    (``ValueError``; ``RuntimeError`` for too few pages or sequences) or whose copies cannot be
+    enqueued changes nothing.  One thread at a time."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page: int = 64, device="cuda",
                  sequences: int = 1024):
@@ -189,6 +194,15 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             return host.to(self.device, non_blocking=True)
 
+    def _move_rows(self) -> None:
+        """``_move``; where it fails (no memory for the lists, a refused launch) the call is taken
+        back."""
+        try:
+            self._move()
+        except BaseException:
+            self._t.undo()
+            raise
+
     def _move(self) -> None:
         """Enqueue the moves of the call just made."""
         groups, moves = self._t.moves()
@@ -215,7 +229,7 @@ class PagedKVCache:
         if y is None:
             self._check_capture()
             self._t.extend(seqs, n)
-            self._move()
+            self._move_rows()
         else:
             self._done("extend", y)
 
@@ -226,7 +240,7 @@ class PagedKVCache:
         if y is None:
             self._check_capture()
             y = self._t.fork(seqs, copies)
-            self._move()
+            self._move_rows()
         return self._done("fork", y)
 
     def compact(self, seqs, starts, paths) -> None:
@@ -238,7 +252,7 @@ class PagedKVCache:
         if y is None:
             self._check_capture()
             self._t.compact(seqs, starts, paths)
-            self._move()
+            self._move_rows()
         else:
             self._done("compact", y)
 

@@ -433,6 +433,131 @@ def test_fork_on_both_sides_of_what_goes_with_a_launch():
         c.free(forks)
 
 
+def _books(c, seqs):
+    table, lens = c._t.table(seqs)
+    return table.tolist(), lens.tolist(), c.free_pages
+
+
+def test_undo_after_random_calls():
+    """extend, fork and compact taken back: every sequence's pages and length, the free pages and the
+    numbers and pages taken next are those of a table that never saw the call."""
+    def play(seed, undone):
+        rng, t = random.Random(seed), _table(30, 4, sequences=10)
+        live, log = [], []
+        for _ in range(120):
+            some = rng.sample(live, rng.randint(0, len(live)))
+            what = rng.choice(["add", "extend", "extend", "fork", "compact", "compact", "trim", "free"])
+            n = [rng.randint(0, 6) for _ in some]
+            room = [t.length(s) for s in some]
+            starts = [rng.randint(0, k) for k in room]
+            paths = [sorted(rng.sample(range(k - a), rng.randint(0, k - a))) for k, a in zip(room, starts)]
+            back = rng.random() < 0.4 and what in ("extend", "fork", "compact")
+            if back and not undone:
+                continue
+            try:
+                if what == "add":
+                    live += t.add([rng.randint(0, 9)])
+                elif what == "extend":
+                    t.extend(some, n)
+                elif what == "fork":
+                    new = t.fork(some[:2], 2)
+                    live += [] if back else new
+                elif what == "compact":
+                    t.compact(some, starts, paths)
+                elif what == "trim":
+                    t.trim(some)
+                else:
+                    t.free(some[:1])
+                    live = [s for s in live if s not in some[:1]]
+            except RuntimeError:
+                continue
+            if back:
+                t.undo()
+                assert _moves(t) == ([], [])
+                t.undo()                         # and nothing more
+            table, lens = t.table(live)
+            log.append((back, live[:], table.tolist(), lens.tolist(), t.available))
+        return [x[1:] for x in log if not x[0]], sum(x[0] for x in log)
+    took = 0
+    for seed in range(30):
+        with_, n = play(seed, True)
+        assert with_ == play(seed, False)[0]
+        took += n
+    assert took > 200
+    t = _table(8, 4)
+    t.extend(t.add([3]), 4)
+    t.add([1])
+    t.undo()                                     # behind an add: nothing
+    assert t.length(0) == 7 and t.available == 5
+
+
+def test_a_copy_that_fails_takes_the_books_back(monkeypatch):
+    """The rows of a call cannot be moved (no memory for the lists, a refused launch): lengths, pages
+    and free pages are as before it, and the next sequences get the numbers they would have."""
+    from respect_amd import _lib
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    c = PagedKVCache(1, 1, 8, pages=20, page=4, device="cpu")
+    monkeypatch.setattr(c, "_check_capture", lambda: None)
+    monkeypatch.setattr(c, "_move", lambda: None)
+    a, b = c.add([9, 6])
+    f, = c.fork([a])
+    c.compact([f], 2, [[]])                     # its next rows lie in a page that a holds too
+    seqs = [a, b, f]
+    before = _books(c, seqs)
+
+    def fail():
+        raise RuntimeError("out of memory")
+    monkeypatch.setattr(c, "_move", fail)
+    for call in (lambda: c.fork([a, b], 2), lambda: c.extend([f, a], [3, 9]), lambda: c.compact([b, f], [0, 0], [[1, 2], [1]])):
+        with pytest.raises(RuntimeError, match="memory"):
+            call()
+        assert _books(c, seqs) == before
+    monkeypatch.setattr(c, "_move", lambda: None)
+    assert c.fork([b]) == [3] and c.add([0]) == [4]
+    c.free([a, b, f, 3, 4])
+    assert c.free_pages == 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("copies", [2, 60])
+def test_moves_that_the_library_refuses_take_the_books_back(native, copies, monkeypatch):
+    """The same with the real copies refused (a head_dim that is none), for lists that go with the
+    launch and longer ones; afterwards the calls do what they should."""
+    from respect_amd import _lib
+    from respect_amd.decoding.paged_kv import PagedKVCache
+
+    class Leave:
+        def __getattr__(self, name):
+            return lambda *a: None
+    if not native:
+        monkeypatch.setattr(_lib, "_calls", Leave())
+    c = PagedKVCache(2, 2, 64, pages=200, page=16)
+    for t in c.k + c.v:
+        t.copy_(torch.randn(t.shape, device="cuda"))
+    s, u = c.add([45, 30])
+    want = [t[:, :45].clone() for t in c.k + c.v]
+    before, pool = _books(c, [s, u]), c._pool
+    c._pool = pool[:2] + (12,) + pool[3:]
+    for call in (lambda: c.fork([s], copies), lambda: c.compact([s, u], 0, [[1, 2], [3]])):
+        with pytest.raises(RuntimeError):
+            call()
+        assert _books(c, [s, u]) == before
+    c._pool = pool
+    forks = c.fork([s], copies)
+    assert forks == list(range(2, 2 + copies))
+    for f in forks:
+        at = c.slots([f], 0, 45).long()
+        assert all(torch.equal(t[:, at], w) for t, w in zip(c.k + c.v, want))
+    c.compact([s], 0, [[1, 2]])
+    at = c.slots([s], 0, 2).long()
+    assert all(torch.equal(t[:, at], w[:, 1:3]) for t, w in zip(c.k + c.v, want))
+    c.free([s, u] + forks)
+    assert c.free_pages == 200
+
+
 @pytest.mark.gpu
 def test_capture_is_refused_and_write_is_captured():
     from respect_amd.decoding.paged_kv import PagedKVCache
