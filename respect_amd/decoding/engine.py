@@ -389,7 +389,8 @@ class Decoder:
     def step_batch(self, ids: torch.Tensor, cache, seqs) -> torch.Tensor:
         """One token (``ids`` [B] on the GPU) of each of the sequences ``seqs`` of the PagedKVCache
         ``cache``, appended to them.  Returns fp32 logits [B, V].  A sequence's results do not
-        depend on the others."""
+        depend on the others.  A step that fails leaves the sequences and the free pages as
+        they were."""
         self._check_paged(cache)
         seqs = list(seqs)
         if tuple(ids.shape) != (len(seqs),) or not seqs:
@@ -399,7 +400,7 @@ class Decoder:
         try:
             return self._step_batch(ids, cache, seqs, n)
         except BaseException:
-            cache.compact(seqs, [m - 1 for m in n], [[] for _ in n])
+            cache._t.undo()   # the extension: nothing else has changed the books since
             raise
 
     def _step_batch(self, ids, cache, seqs, n: list[int]) -> torch.Tensor:

@@ -178,6 +178,24 @@ def test_tables_made_on_one_stream_serve_another(model):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_a_failed_step_gives_its_page_back(model):
+    """A step that fails past the extension, at a page's end: no page stays taken."""
+    cache = _cache(pages=8)
+    (s,), _ = model.prefill_batch(_prompts([16]), cache)
+    f, = cache.fork([s])
+    cache.compact([f], 3, [[]])                                 # its next row lies in a shared page
+    free = cache.free_pages
+    with pytest.raises(RuntimeError):
+        model.step_batch(torch.tensor([1, 2]), cache, [s, f])   # tokens on the CPU
+    assert cache.free_pages == free and cache.length(s) == 16 and cache.length(f) == 3
+    tok = torch.tensor([1, 2], device="cuda")
+    a = model.step_batch(tok, cache, [s, f])
+    other = _cache()
+    p, = _prompts([16])
+    seqs, _ = model.prefill_batch([p, p[:3]], other)
+    assert torch.equal(model.step_batch(tok, other, seqs), a)
+
+
 def test_refusals(model):
     from respect_amd.decoding.paged_kv import PagedKVCache
     cache = _cache()
