@@ -468,7 +468,9 @@ int rspx_rope_vision(const void* x, int64_t sxl, int64_t sxh, const float* cos, 
  * points outside [0, Tq) or [0, Tk) is cut to them.  sm_scale > 0.
  * fp32 softmax, probabilities rounded to bf16 for the product with v, one rounding of
  * the result.  A row's bits depend on its own sequence up to the row alone: not on the
- * other sequences, on the tiles' size or order, or on what later keys and values hold.
+ * other sequences, on the tiles' size or order, or on what later keys and values hold.  A
+ * value that is not finite reaches the rows that see it alone; an infinite one makes NaN
+ * where its p is 0 in fp32.
  */
 int rspx_prompt_attn_tile_rows(int H, int HK);
 /* The tiles of n sequences packed one after the other, sequence i of rows[i] rows in q and

@@ -344,9 +344,17 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
     for (int i = 0; i < 16; ++i) p[i / 4][i % 4] = pair(s, 2 * i);
     if (__builtin_amdgcn_readfirstlane(flags[t - first_edge]) != 0) {
       // The values that are not finite go to the rows that see them one by one, and the
-      // product runs without them: every other sum keeps its bits.
+      // product runs without them: every other sum keeps its bits.  Where p is 0 they are NaN,
+      // as the product makes them in a step seen whole.
+      uint32_t none[2] = {0, 0};                           // scores with p = 0, of this lane and the row's other one
+#pragma unroll
+      for (int r = 0; r < 32; ++r)
+        if ((p[r / 8][r / 2 % 4] >> (16 * (r % 2)) & 0xffffu) == 0) none[0] |= 1u << r;
+      none[1] = (uint32_t)__shfl_xor((int)none[0], 32);
 #pragma unroll 1
-      for (int key = 0; key < kKeys; ++key)
+      for (int key = 0; key < kKeys; ++key) {
+        const int r = 16 * (key / 32) + 4 * (key % 32 / 8) + key % 4;   // key's place among its lane's scores
+        const bool zero = (none[key / 4 % 2 != half] >> r & 1) != 0;
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
@@ -354,8 +362,9 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
             const int d = 32 * j + 8 * (e / 4) + 4 * half + e % 4;
             const uint16_t x = *(const __attribute__((address_space(3))) uint16_t*)(
                 sv + 16 * (key * U + ((d / 8) ^ vswizzle<D>(key))) + 2 * (d % 8));
-            if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + bf16_to_f32(x);
+            if ((x & 0x7f80) == 0x7f80 && key < mine) acc[j][e] = acc[j][e] + (zero ? __builtin_nanf("") : bf16_to_f32(x));
           }
+      }
       lds_barrier();
 #pragma unroll 1
       for (int j = 0; j < kLoads; ++j) {

@@ -284,3 +284,30 @@ def test_gpu_refusals_and_empty():
         prompt_attn(q, k, v, PackedPrompts([4]), sm_scale=0.0)
     assert prompt_attn(q[:0], k[:0], v[:0], PackedPrompts([])).shape == (0, 4, 64)
     assert (prompt_attn(q, k[:0], v[:0], PackedPrompts([4], [0])) == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("H,HK,D", [(4, 1, 128), (4, 2, 64), (2, 2, 32), (8, 2, 256)])
+def test_values_that_are_not_finite_in_whole_and_partial_steps(what, H, HK, D):
+    """Two values that are not finite, one behind a score so low that p is 0 in fp32 (0 times it is
+    NaN), one with an ordinary p: a row has the same result whether its tile sees their steps whole
+    (the prompt in one pass) or in part or last (the row alone after its earlier keys)."""
+    from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
+    n = 200
+    q, k, v = _inputs([n], [n], H, HK, D, seed=31)
+    q = q.abs()
+    k[5] = -200.0
+    v[5, :, 3], v[70, :, 4] = what, what
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    whole = prompt_attn(q, k, v, PackedPrompts([n])).float()
+    assert torch.isfinite(whole[:5]).all() and torch.isfinite(whole[:70, :, 4]).all()
+    assert torch.isnan(whole[6:, :, 3]).all()
+    want = torch.full_like(whole[70:, :, 4], what)
+    assert torch.equal(whole[70:, :, 4].nan_to_num(7.0), want.nan_to_num(7.0))
+    rest = [d for d in range(D) if d not in (3, 4)]
+    assert torch.isfinite(whole[:, :, rest]).all()
+    for end in (5, 6, 7, 40, 64, 65, 71, 128, 129, 192, 200):
+        one = prompt_attn(q[end - 1:end], k[:end], v[:end], PackedPrompts([1], [end])).float()[0]
+        assert torch.equal(torch.isnan(one), torch.isnan(whole[end - 1])), end
+        assert torch.equal(one.nan_to_num(7.0), whole[end - 1].nan_to_num(7.0)), end
