@@ -56,6 +56,7 @@ constexpr int kRows = 32;            // rows of a wave
 constexpr float kTau = 8.0f;         // log2 headroom before the reference maximum moves
 constexpr float kNone = -1e30f;      // reference maximum before the first key
 
+constexpr int kGroups = 1 << 23;     // workgroups of a launch: a grid dimension holds 2^32 threads
 constexpr int kEdges = 8;            // more than the steps that some row of a tile sees in part
 // Waves per SIMD, that is workgroups per CU, that the registers and the LDS allow.
 constexpr int waves_per_simd(int D) { return D >= 256 ? 1 : D >= 128 ? 2 : D >= 64 ? 3 : 4; }
@@ -425,11 +426,14 @@ __global__ __launch_bounds__(256, waves_per_simd(D)) void prompt_attn_kernel(Pro
 int heads_per_group(int G) { return G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1; }
 
 template <int D>
-int launch(const PromptArgs& A, int HW, int n, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)A.units * n));
-  if (HW == 4) hipLaunchKernelGGL((prompt_attn_kernel<D, 4>), grid, dim3(256), 0, s, A);
-  else if (HW == 2) hipLaunchKernelGGL((prompt_attn_kernel<D, 2>), grid, dim3(256), 0, s, A);
-  else hipLaunchKernelGGL((prompt_attn_kernel<D, 1>), grid, dim3(256), 0, s, A);
+int launch(PromptArgs A, int HW, int n, hipStream_t s) {
+  const int per = kGroups / A.units;
+  for (; n > 0; n -= per, A.tiles += 4 * (int64_t)per) {
+    const dim3 grid((unsigned)(A.units * std::min(n, per)));
+    if (HW == 4) hipLaunchKernelGGL((prompt_attn_kernel<D, 4>), grid, dim3(256), 0, s, A);
+    else if (HW == 2) hipLaunchKernelGGL((prompt_attn_kernel<D, 2>), grid, dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((prompt_attn_kernel<D, 1>), grid, dim3(256), 0, s, A);
+  }
   return hipGetLastError() == hipSuccess ? RSPX_OK : RSPX_ELAUNCH;
 }
 
@@ -501,7 +505,7 @@ extern "C" int rspx_prompt_attn(const void* q, int64_t sqt, int64_t sqh, const v
   A.G = H / HK, A.Tq = Tq, A.Tk = Tk;
   const int HW = heads_per_group(A.G);
   A.units = H / HW;
-  if ((int64_t)A.units * n_tiles > INT32_MAX) return RSPX_EINVAL;
+  if (A.units > kGroups) return RSPX_EUNSUPPORTED;
   A.c = sm_scale * 1.44269504088896340736f;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (D) {

@@ -311,3 +311,23 @@ def test_values_that_are_not_finite_in_whole_and_partial_steps(what, H, HK, D):
         one = prompt_attn(q[end - 1:end], k[:end], v[:end], PackedPrompts([1], [end])).float()[0]
         assert torch.equal(torch.isnan(one), torch.isnan(whole[end - 1])), end
         assert torch.equal(one.nan_to_num(7.0), whole[end - 1].nan_to_num(7.0)), end
+
+
+@pytest.mark.gpu
+def test_more_workgroups_than_a_grid_holds():
+    """32900 one-token sequences of 512 heads: 16.8 M workgroups, more than the 2^32 threads of a grid
+    dimension, whose count would start again at 0; every result is its one value."""
+    from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
+    n = 32900
+    x = torch.randn(n, 512, 32, device="cuda").to(BF)
+    assert torch.equal(prompt_attn(x, x, x, PackedPrompts([1] * n)), x)
+
+
+def test_more_heads_than_a_grid_holds_are_refused():
+    from respect_amd import _lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    for H, want in ((1 << 23, 0), ((1 << 23) + 1, -2), ((1 << 31) - 1, -2)):
+        got = _lib.lib().rspx_prompt_attn(16, 64, 64, 16, 64, 64, 16, 64, 64, 16, 0 if want == 0 else 1, 16, 64, 64, H, H, 4, 4,
+                                          64, 0.1, None)
+        assert got == want
