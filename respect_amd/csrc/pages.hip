@@ -78,8 +78,9 @@ __global__ __launch_bounds__(kThreads) void values_kernel(int* out, int n, Value
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const uint16_t* k, int64_t skt, int64_t skh, const uint16_t* v,
                                                             int64_t svt, int64_t svh, const int* slots, int cap,
                                                             uint16_t* ck, int64_t sckh, int64_t sckn, uint16_t* cv,
-                                                            int64_t scvh, int64_t scvn, int U, int HK, int64_t total) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+                                                            int64_t scvh, int64_t scvn, int U, int HK, int64_t first,
+                                                            int64_t total) {
+  const int64_t i = first + (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (i >= total) return;
   const int64_t r = i / U;
   const int c = (int)(i - r * U), h = (int)(r % HK);
@@ -93,6 +94,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const uint16_t* k, i
 }
 
 constexpr int kGroupsPerLaunch = 1 << 20;
+constexpr int64_t kBlocksPerLaunch = 1 << 23;   // a grid dimension holds 2^32 threads
 
 }  // namespace
 
@@ -162,10 +164,10 @@ extern "C" int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void
     if (x % 8) return RSPX_EALIGN;
   const int U = D / 8;
   const int64_t total = (int64_t)T * HK * U, blocks = (total + kThreads - 1) / kThreads;
-  if (blocks > INT32_MAX) return RSPX_EINVAL;
-  hipLaunchKernelGGL(kv_write_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const uint16_t*>(k), skt, skh, static_cast<const uint16_t*>(v), svt, svh, slots, cap,
-                     static_cast<uint16_t*>(cache_k), sckh, sckn, static_cast<uint16_t*>(cache_v), scvh, scvn, U, HK,
-                     total);
+  for (int64_t b0 = 0; b0 < blocks; b0 += kBlocksPerLaunch)
+    hipLaunchKernelGGL(kv_write_kernel, dim3((unsigned)std::min(blocks - b0, kBlocksPerLaunch)), dim3(kThreads), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const uint16_t*>(k), skt, skh,
+                       static_cast<const uint16_t*>(v), svt, svh, slots, cap, static_cast<uint16_t*>(cache_k), sckh, sckn,
+                       static_cast<uint16_t*>(cache_v), scvh, scvn, U, HK, b0 * kThreads, total);
   return hipGetLastError() == hipSuccess ? RSPX_OK : RSPX_ELAUNCH;
 }

@@ -582,6 +582,20 @@ def test_capture_is_refused_and_write_is_captured():
 
 
 @pytest.mark.gpu
+def test_write_of_more_threads_than_a_grid_holds():
+    """4097 tokens of 2^20 16-byte pieces each, 2^32 and more threads: the last token is written too.
+    All are the same row, all but two go nowhere."""
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    c = PagedKVCache(1, 4096, 2048, pages=2, page=1)
+    k, v = (torch.randn(1, 4096, 2048, device="cuda").to(BF) for _ in range(2))
+    slots = torch.full((4097,), -1, dtype=torch.int32, device="cuda")
+    slots[0], slots[4096] = 0, 1
+    c.write(0, k.expand(4097, -1, -1), v.expand(4097, -1, -1), slots)
+    for pool, x in ((c.k[0], k), (c.v[0], v)):
+        assert torch.equal(pool[:, 0], x[0]) and torch.equal(pool[:, 1], x[0])
+
+
+@pytest.mark.gpu
 def test_gpu_refusals():
     from respect_amd.decoding.paged_kv import PagedKVCache
     c = PagedKVCache(1, 2, 64, pages=8, page=4)
