@@ -10,6 +10,7 @@ pools through ``tables``.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import numpy as np
 import torch
@@ -22,10 +23,15 @@ def _p(a: np.ndarray) -> int:
     return a.ctypes.data
 
 
+def _whole(numbers) -> np.ndarray:
+    """int64 of an iterable of whole numbers (``TypeError`` for any other: none is cut to one)."""
+    return np.array([operator.index(x) for x in numbers], dtype=np.int64)
+
+
 class PageTable:
     """Who holds which page, without the pools: the host half of ``PagedKVCache``.  A refused
-    call (``ValueError``: no such sequence, one named twice, a bad count; ``RuntimeError``: too
-    few pages or sequences) changes nothing."""
+    call (``ValueError``: no such sequence, one named twice, a bad count; ``TypeError``: not a
+    whole number; ``RuntimeError``: too few pages or sequences) changes nothing."""
 
     def __init__(self, pages: int, page: int, sequences: int):
         self._lib = _lib.lib()
@@ -52,7 +58,7 @@ class PageTable:
 
     @staticmethod
     def _ids(seqs) -> np.ndarray:
-        ids = np.asarray(list(seqs), dtype=np.int64)
+        ids = _whole(seqs)
         if ids.size and (ids.min() < 0 or ids.max() >= 1 << 31):
             raise ValueError("PagedKVCache: no such sequence")
         return ids.astype(np.int32)
@@ -60,10 +66,12 @@ class PageTable:
     @staticmethod
     def _counts(n, many: int) -> np.ndarray:
         """One number for each of ``many``, or that many of them."""
-        c = np.asarray(n, dtype=np.int64)
-        if c.ndim and c.shape != (many,):
+        if not np.iterable(n):
+            return np.full(many, operator.index(n), np.int64)
+        c = _whole(n)
+        if len(c) != many:
             raise ValueError(f"PagedKVCache: {many} counts are needed")
-        return np.ascontiguousarray(np.broadcast_to(c, (many,)))
+        return c
 
     @property
     def available(self) -> int:
@@ -76,7 +84,7 @@ class PageTable:
         return n
 
     def add(self, lengths) -> list[int]:
-        n = np.asarray(list(lengths), dtype=np.int64)
+        n = _whole(lengths)
         ids = np.empty(len(n), np.int32)
         self._call("add", _p(n), len(n), _p(ids))
         return ids.tolist()
@@ -87,6 +95,7 @@ class PageTable:
 
     def fork(self, seqs, copies: int) -> list[int]:
         ids = self._ids(seqs)
+        copies = operator.index(copies)
         if not 0 <= copies < 1 << 31:
             raise ValueError("PagedKVCache: counts must be >= 0")
         if len(ids) * copies >= 1 << 24:
@@ -97,7 +106,7 @@ class PageTable:
 
     def compact(self, seqs, starts, paths) -> None:
         ids = self._ids(seqs)
-        paths = [np.asarray(list(p), dtype=np.int64) for p in paths]
+        paths = [_whole(p) for p in paths]
         if len(paths) != len(ids):
             raise ValueError("PagedKVCache: one path per sequence")
         flat = np.concatenate(paths) if paths else np.zeros(0, np.int64)

@@ -1,6 +1,7 @@
 """The paged KV cache (decoding.paged_kv): its bookkeeping on the CPU against a plain model of
 it (who holds which page, lowest page first, full pages shared), and on the GPU its rows after
 random runs of add, extend, write, fork, compact, trim and free against plain tensors."""
+import ctypes
 import random
 
 import numpy as np
@@ -125,6 +126,27 @@ def test_failures_change_nothing():
     for bad in (dict(pages=0), dict(page=3), dict(pages=1 << 28), dict(head_dim=12), dict(layers=0), dict(sequences=0)):
         with pytest.raises(ValueError):
             PagedKVCache(**{**dict(layers=1, kv_heads=1, head_dim=8, pages=4, page=16, device="cpu"), **bad})
+
+
+def test_numbers_that_are_not_whole_are_refused():
+    """Fractions are refused, not cut; whole numbers of any kind are taken."""
+    t = _table(12, 4)
+    a, b = t.add(np.array([7, 9], np.int16))
+    before = t.table([a, b])[0].tolist()
+    for call in (lambda: t.add([1.5]), lambda: t.extend([a], 1.9), lambda: t.extend([a, b], [1, 1.0]), lambda: t.extend([0.9], 1),
+                 lambda: t.fork([0.9], 1), lambda: t.fork([a], 1.5), lambda: t.compact([a], 1.7, [[0]]),
+                 lambda: t.compact([a], 1, [[0.2, 1.9]]), lambda: t.trim([0.9]), lambda: t.free([0.9]), lambda: t.table([0.9]),
+                 lambda: t.slots([a], 0.5, 1), lambda: t.slots([a], 0, 1.5), lambda: t.length(0.9), lambda: t.extend(["0"], 1),
+                 lambda: t.extend([a], np.array(1.5)), lambda: t.extend([a], np.array([1.5])), lambda: t.extend([a], None),
+                 lambda: t.extend([a], torch.tensor([1.5]))):
+        with pytest.raises((TypeError, ctypes.ArgumentError)):
+            call()
+        assert t.table([a, b])[0].tolist() == before and (t.length(a), t.length(b), t.available) == (7, 9, 7)
+    t.extend(torch.tensor([a, b]), np.array(1))
+    t.extend((a, b), torch.tensor([1, 2]))
+    t.extend(iter([a]), np.int32(1))
+    t.compact(np.array([a]), np.array([2]), [range(1, 3)])
+    assert (t.length(a), t.length(b)) == (4, 12) and t.slots([a], torch.tensor(0), 4).tolist() == [0, 1, 2, 3]
 
 
 def test_random_bookkeeping_keeps_count():
