@@ -35,7 +35,9 @@ class PageTable:
 
     def __init__(self, pages: int, page: int, sequences: int):
         self._lib = _lib.lib()
-        self.handle = self._lib.rspx_pages_new(pages, page, sequences)
+        self.handle = None
+        if all(0 < operator.index(n) < 1 << 31 for n in (pages, page, sequences)):   # what 32 bits hold
+            self.handle = self._lib.rspx_pages_new(pages, page, sequences)
         if not self.handle:
             raise ValueError("PagedKVCache: pages and sequences >= 1, page a power of two, pages * page below 2^31")
 

@@ -149,6 +149,14 @@ def test_numbers_that_are_not_whole_are_refused():
     assert (t.length(a), t.length(b)) == (4, 12) and t.slots([a], torch.tensor(0), 4).tolist() == [0, 1, 2, 3]
 
 
+def test_sizes_past_32_bits_are_refused():
+    for sizes in ((1 << 32 | 5, 4, 8), (5, 1 << 32 | 4, 8), (5, 4, 1 << 32 | 8), (5, 4, 1 << 31), (-5, 4, 8), (5 - (1 << 32), 4, 8)):
+        with pytest.raises(ValueError):
+            _table(*sizes)
+    with pytest.raises(TypeError):
+        _table(5.5, 4, 8)
+
+
 def test_random_bookkeeping_keeps_count():
     """Random calls: every page is held by as many as the count says, and never written by a move
     that another sequence's rows depend on."""
