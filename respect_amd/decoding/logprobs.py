@@ -2,6 +2,8 @@
 choice of ``acceptance`` and over the same scores.  No counterpart in the reference."""
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from .. import _lib
@@ -29,6 +31,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
         raise ValueError(f"token_logprobs: V {V}, top {top} (0 to {MAX_TOP})")
     if logits.stride(0) < V:   # rows that overlap
         logits = logits.clone(memory_format=torch.contiguous_format)
+    # Past the vocabulary or below 0 one number is as good as another: 32 bits hold these.
+    offset, size = (min(max(operator.index(x), -1), V) for x in (offset, size))
     tokens = tokens.contiguous()
     dev, n = logits.device, min(top, V)
     given, entropy = torch.empty((2, M), dtype=torch.float32, device=dev)
@@ -38,7 +42,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
     with torch.cuda.device(dev):
         # Of this call alone: torch hands it to the stream, or to the graph being captured.
         ws = torch.empty(L.rspx_token_logprobs_workspace_bytes(M, V, n), dtype=torch.uint8, device=dev)
-        rc = L.rspx_token_logprobs(logits.data_ptr(), logits.stride(0), M, V, int(offset), int(size), tokens.data_ptr(),
+        rc = L.rspx_token_logprobs(logits.data_ptr(), logits.stride(0), M, V, offset, size, tokens.data_ptr(),
                                    n, given.data_ptr(), entropy.data_ptr(), values.data_ptr(), ids.data_ptr(),
                                    ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
     _lib.check("rspx_token_logprobs", rc)

@@ -172,6 +172,25 @@ def test_rows_do_not_depend_on_the_batch_and_agree_with_greedy():
 
 
 @pytest.mark.gpu
+def test_excluded_ranges_past_32_bits():
+    """Offsets and sizes that 32 bits do not hold mean what they say; fractions are refused."""
+    from respect_amd.decoding.logprobs import token_logprobs
+    x, t = _logits(3, 500, seed=11)
+    t[0] = 100
+    g = (x.cuda(), t.cuda())
+    for off, size in ((40, (1 << 32) + 5), (40, 1 << 62), (1 << 32, 60), ((1 << 33) + 7, 1 << 32), (499, 1 << 31)):
+        _check(token_logprobs(*g, top=9, offset=off, size=size), _exact(x, t, 9, min(off, 500), size))
+    all_ = token_logprobs(*g, top=2, size=1 << 32)
+    assert (all_[0] == -math.inf).all() and (all_[1] == 0).all()
+    for off, size in ((-(1 << 32), 5), (0, -(1 << 32)), (-1, 1 << 40)):
+        with pytest.raises(RuntimeError):
+            token_logprobs(*g, offset=off, size=size)
+    for off, size in ((1.9, 5), (1, 5.0)):
+        with pytest.raises(TypeError):
+            token_logprobs(*g, offset=off, size=size)
+
+
+@pytest.mark.gpu
 def test_gpu_refusals_and_empty():
     from respect_amd.decoding.logprobs import token_logprobs
     x, t = (a.cuda() for a in _logits(2, 100))
