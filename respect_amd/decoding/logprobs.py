@@ -7,6 +7,7 @@ import operator
 import torch
 
 from .. import _lib
+from ..kernels._tensor import fits_32_bits
 
 MAX_TOP = 64   # alternatives rspx_token_logprobs gives at most
 
@@ -29,6 +30,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
         raise TypeError(f"token_logprobs: tokens must be int64 [{M}] on the GPU of the logits")
     if V == 0 or not 0 <= top <= MAX_TOP:
         raise ValueError(f"token_logprobs: V {V}, top {top} (0 to {MAX_TOP})")
+    fits_32_bits("token_logprobs", M, V)
     if logits.stride(0) < V:   # rows that overlap
         logits = logits.clone(memory_format=torch.contiguous_format)
     # Past the vocabulary or below 0 one number is as good as another: 32 bits hold these.

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from ..kernels._tensor import as_kernel_input
+from ..kernels._tensor import as_kernel_input, fits_32_bits
 
 
 def _p(a: np.ndarray) -> int:
@@ -307,6 +307,7 @@ class PagedKVCache:
         T = k.shape[0]
         if tuple(k.shape) != (T, self.HK, self.D) or v.shape != k.shape or tuple(slots.shape) != (T,):
             raise ValueError(f"PagedKVCache: k and v must be [T, {self.HK}, {self.D}], slots [T]")
+        fits_32_bits("PagedKVCache.write", T)
         if slots.dtype != torch.int32:
             raise TypeError("PagedKVCache: slots must be int32")
         k, v, slots = as_kernel_input(k, "k"), as_kernel_input(v, "v"), slots.contiguous()

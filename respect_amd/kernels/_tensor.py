@@ -4,6 +4,12 @@ from __future__ import annotations
 import torch
 
 
+def fits_32_bits(what: str, *sizes: int) -> None:
+    """Refuse sizes that the C ABI's 32-bit arguments do not hold (ctypes would cut them)."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{what}: sizes must be below 2^31")
+
+
 def _aligned(t: torch.Tensor, inner_contig: bool = True) -> bool:
     if t.data_ptr() % 16 != 0:
         return False

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._tensor import as_kernel_input
+from ._tensor import as_kernel_input, fits_32_bits
 
 
 def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None):
@@ -33,6 +33,7 @@ def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None):
         raise ValueError(f"paged_attn: {slots} slots are no whole pages of {page}")
     if table.dim() != 2 or table.shape[0] != B or tuple(lens.shape) != (B,):
         raise ValueError(f"paged_attn: table must be [{B}, width] and lens [{B}]")
+    fits_32_bits("paged_attn", B, H, HK, slots, page, table.shape[1])
     if table.dtype != torch.int32 or lens.dtype != torch.int32:
         raise TypeError("paged_attn: table and lens must be int32")
     for name, t in (("kc", kc), ("vc", vc)):                     # a cache is never copied

@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from .. import _lib
-from ._tensor import as_kernel_input
+from ._tensor import as_kernel_input, fits_32_bits
 
 TILE_ROWS = (32, 64, 128)   # what rspx_prompt_attn_tile_rows gives
 
@@ -67,6 +67,7 @@ def prompt_attn(q, k, v, plan: PackedPrompts, sm_scale=None, out=None):
     Tk, HK, _ = k.shape
     if T != plan.Tq or Tk != plan.Tk:
         raise ValueError(f"prompt_attn: the plan packs {plan.Tq} rows and {plan.Tk} keys, not {T} and {Tk}")
+    fits_32_bits("prompt_attn", H, HK)
     if HK == 0 or H % HK:
         raise ValueError(f"prompt_attn: {H} heads over {HK} kv heads")
     q, k, v = (as_kernel_input(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v")))

@@ -191,6 +191,19 @@ def test_excluded_ranges_past_32_bits():
 
 
 @pytest.mark.gpu
+def test_sizes_past_32_bits_are_refused():
+    from respect_amd.decoding.logprobs import token_logprobs
+    x, t = torch.zeros(1, 1, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        token_logprobs(x.expand((1 << 32) + 1, 1), t.expand((1 << 32) + 1))
+    wide = torch.empty(1, (1 << 32) + 5, device="cuda")   # 17 GB
+    with pytest.raises(ValueError):
+        token_logprobs(wide, t)
+    with pytest.raises((ValueError, RuntimeError)):
+        token_logprobs(wide[:, :(1 << 30) + 1], t)
+
+
+@pytest.mark.gpu
 def test_gpu_refusals_and_empty():
     from respect_amd.decoding.logprobs import token_logprobs
     x, t = (a.cuda() for a in _logits(2, 100))

@@ -19,6 +19,32 @@ def test_calls_leaves_what_it_does_not_take():
     assert c.token_logprobs(f, f, 1.5, None, "a") is None
 
 
+def test_sizes_past_32_bits_are_refused():
+    """Tensors of one element seen 2^32 times over: their sizes are refused, not cut to 32 bits."""
+    from respect_amd import _lib
+    from respect_amd.decoding.paged_kv import PagedKVCache
+    from respect_amd.kernels.paged_attention import paged_attn
+    from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    big = 1 << 32
+    q, kc, table, lens = (torch.zeros(1, 4, 64, dtype=BF), torch.zeros(2, 64, 64, dtype=BF),
+                          torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    for args in ((q.expand(1, -1, -1), kc[:, :1].expand(2, big + 64, 64), table),
+                 (q, kc[:1].expand(big + 2, 64, 64), table), (q[:, :1].expand(1, big + 4, 64), kc, table),
+                 (q, kc, table[:, :1].expand(1, big + 4))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            paged_attn(args[0], args[1], args[1], args[2], lens, 16)
+    x = torch.zeros(4, 1, 64, dtype=BF)
+    for h, hk in ((big + 4, 2), (4, big + 2)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            prompt_attn(x.expand(4, h, 64), x.expand(4, hk, 64), x.expand(4, hk, 64), PackedPrompts([4], device="cpu"))
+    c = PagedKVCache(1, 1, 8, pages=4, page=4, device="cpu")
+    row = torch.zeros(1, 1, 8, dtype=BF).expand(big + 1, 1, 8)
+    with pytest.raises(ValueError, match="2\\^31"):
+        c.write(0, row, row, torch.zeros(1, dtype=torch.int32).expand(big + 1))
+
+
 @pytest.mark.gpu
 def test_calls_equal_the_wrappers_own_path(monkeypatch):
     from respect_amd import _lib
