@@ -8,6 +8,8 @@ order: its bits do not depend on what else is packed beside it.
 """
 from __future__ import annotations
 
+import operator
+
 import numpy as np
 import torch
 
@@ -25,9 +27,9 @@ class PackedPrompts:
     and get zeros."""
 
     def __init__(self, rows, keys=None, device="cuda"):
-        r = np.asarray(list(rows), dtype=np.int64)
-        k = r if keys is None else np.asarray(list(keys), dtype=np.int64)
-        if r.ndim != 1 or r.shape != k.shape or (r < 0).any() or (k < 0).any():
+        r = np.array([operator.index(n) for n in rows], dtype=np.int64)
+        k = r if keys is None else np.array([operator.index(n) for n in keys], dtype=np.int64)
+        if r.shape != k.shape or (r < 0).any() or (k < 0).any():
             raise ValueError("PackedPrompts: rows and keys must be equally many lengths >= 0")
         self.rows, self.keys = r.tolist(), k.tolist()
         self.Tq, self.Tk = sum(self.rows), sum(self.keys)

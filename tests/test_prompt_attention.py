@@ -117,6 +117,18 @@ def test_refusals():
     assert L.rspx_prompt_attn_tile_rows(3, 2) == -1 and L.rspx_prompt_attn_tile_rows(0, 1) == -1
 
 
+def test_lengths_that_are_not_whole_are_refused():
+    from respect_amd import _lib
+    from respect_amd.kernels.prompt_attention import PackedPrompts
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("librespect_amd.so not built")
+    for bad in (([1.9], None), ([2, 1.0], None), ([2], [2.5]), (np.array([1.5]), None), (["3"], None), ([[1, 2]], None)):
+        with pytest.raises(TypeError):
+            PackedPrompts(*bad, device="cpu")
+    plan = PackedPrompts(np.array([3, 1], np.int16), torch.tensor([5, 1]), device="cpu")
+    assert plan.rows == [3, 1] and plan.keys == [5, 1]
+
+
 SHAPES = [(8, 2, 128), (4, 2, 64), (3, 1, 128), (16, 2, 64), (4, 1, 32), (4, 1, 256), (2, 2, 256), (6, 2, 64)]
 PACKS = [([1], None), ([77], None), ([64, 65, 1, 0, 130], None), ([33, 5], [97, 5]), ([40, 7, 3], [10, 7, 0]),
          ([129], [323])]
