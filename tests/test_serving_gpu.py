@@ -218,3 +218,22 @@ def test_refusals(model):
         model.prefill_batch([torch.tensor([1, 2, 3])], cache)
     assert cache.free_pages == 63
     assert cache.length(seqs[0]) == 3
+
+
+def test_the_documented_run(model):
+    """Prompts answered four times each, as the documentation shows it: every page is free again."""
+    from respect_amd.decoding.logprobs import token_logprobs
+    cache = _cache(pages=200)
+    first, logits = model.prefill_batch(_prompts(), cache)
+    others = cache.fork(first)
+    want = model.step_batch(torch.tensor([3, 4, 5, 6], device="cuda"), cache, others)
+    seqs = cache.fork(first, 4)
+    cache.free(first)
+    logits = logits.repeat_interleave(4, 0)
+    tokens = torch.tensor([3, 4, 5, 6], device="cuda").repeat_interleave(4)
+    given, entropy, values, ids = token_logprobs(logits, tokens, top=5)
+    assert given.shape == entropy.shape == (16,) and values.shape == ids.shape == (16, 5)
+    got = model.step_batch(tokens, cache, seqs)
+    assert torch.equal(got, want.repeat_interleave(4, 0))
+    cache.free(seqs + others)
+    assert cache.free_pages == 200
