@@ -172,6 +172,42 @@ def test_rows_do_not_depend_on_the_batch_and_agree_with_greedy():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("where", ["spread", "early", "late", "rising", "equal"])
+def test_more_alternatives_than_the_join_holds_at_once(where):
+    """74 parts of 64 pairs a row, more than the 4096 that the join takes at once: the best of them
+    in the parts it takes first, in those it takes last, in both."""
+    from respect_amd.decoding.logprobs import token_logprobs
+    V, top = 300001, 64
+    x, t = _logits(2, V, seed=12)
+    if where == "rising":
+        x = torch.arange(2 * V).view(2, V) * 2e-4
+    elif where == "equal":
+        x = torch.zeros(2, V)
+    elif where != "spread":
+        at = slice(0, 100) if where == "early" else slice(V - 100, V)
+        x[:, at] = 20 + torch.arange(100) % 7
+    _check(token_logprobs(x.cuda(), t.cuda(), top=top), _exact(x, t, top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,top", [(17, 0), (17, 3), (4100, 2)])
+def test_more_rows_than_a_launch_takes(V, top):
+    """65540 rows, launched 65535 at a time: rows on both sides of the border against 64 bits, the
+    last ones the bits of a call for them alone."""
+    from respect_amd.decoding.logprobs import token_logprobs
+    M = 65540
+    g = torch.Generator(device="cuda")
+    g.manual_seed(13)
+    x = torch.randn(M, V, generator=g, device="cuda") * 2
+    t = torch.randint(0, V, (M,), generator=g, device="cuda")
+    got = token_logprobs(x, t, top=top, offset=2, size=3)
+    some = torch.tensor([0, 1, 40000, 65533, 65534, 65535, 65536, 65539], device="cuda")
+    _check([a[some] for a in got], _exact(x[some].cpu(), t[some].cpu(), top, 2, 3))
+    alone = token_logprobs(x[65000:], t[65000:], top=top, offset=2, size=3)
+    assert all(torch.equal(a, b[65000:]) for a, b in zip(alone, got))
+
+
+@pytest.mark.gpu
 def test_excluded_ranges_past_32_bits():
     """Offsets and sizes that 32 bits do not hold mean what they say; fractions are refused."""
     from respect_amd.decoding.logprobs import token_logprobs

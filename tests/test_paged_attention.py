@@ -252,3 +252,23 @@ def test_gpu_refusals_and_empty():
         paged_attn(q, kc[:, :48], vc[:, :48], table, n, 24)      # no power of two
     assert paged_attn(q[:0], kc, vc, table[:0], n[:0], 16).shape == (0, 4, 64)
     assert (paged_attn(q, kc, vc, table[:, :0], _i32([0]), 16) == 0).all()
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_a_launch_takes():
+    """1030 and 2060 sequences, launched 1024 at a time: rows on both sides of the borders against
+    64 bits, every row the bits of the same sequence in a small batch."""
+    from respect_amd.kernels.paged_attention import paged_attn
+    H, HK, D, page = 4, 2, 64, 16
+    for B in (1030, 2060):
+        lens = [(7 * b) % 40 for b in range(B)]
+        for b, n in ((0, 600), (1023, 700), (1024, 900), (1029, 513), (B - 2, 1300), (B - 1, 257)):
+            lens[b] = n
+        kc, vc, table, rows = _cache(lens, page, HK, D, seed=B)
+        q, kc, vc, table = _q(B, H, D, seed=B).cuda(), kc.cuda(), vc.cuda(), table.cuda()
+        got = paged_attn(q, kc, vc, table, _i32(lens), page)
+        some = [0, 1, 1022, 1023, 1024, 1025, 1028, 1029, B - 3, B - 2, B - 1]
+        _check(got[some], *_exact(q[some].cpu(), [rows[b] for b in some]))
+        for a in range(0, B, 200):
+            part = paged_attn(q[a:a + 200], kc, vc, table[a:a + 200], _i32(lens[a:a + 200]), page)
+            assert torch.equal(part, got[a:a + 200]), a
