@@ -354,12 +354,13 @@ class Decoder:
         in proportion to all tokens (98 KB each at the 8B sizes), which goes back to torch with
         its end."""
         self._check_paged(cache)
+        prompts = list(prompts)
         rows = [int(p.shape[0]) for p in prompts]
         if not rows or min(rows) < 1:
             raise ValueError("prefill_batch: prompts must be one or more, none empty")
         cfg, dev, T = self.cfg, self.device, sum(rows)
         plan = PackedPrompts(rows, device=dev)
-        ids = torch.cat(list(prompts))
+        ids = torch.cat(prompts)
         positions = torch.cat([torch.arange(n, device=dev) for n in rows])
         seqs = cache.add(rows)
         try:

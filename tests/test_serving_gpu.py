@@ -220,6 +220,13 @@ def test_refusals(model):
     assert cache.length(seqs[0]) == 3
 
 
+def test_prompts_from_a_generator(model):
+    a, b = _cache(), _cache()
+    _, want = model.prefill_batch(_prompts(), a)
+    seqs, got = model.prefill_batch((p for p in _prompts()), b)
+    assert torch.equal(got, want) and [b.length(s) for s in seqs] == LENS
+
+
 def test_the_documented_run(model):
     """Prompts answered four times each, as the documentation shows it: every page is free again."""
     from respect_amd.decoding.logprobs import token_logprobs
