@@ -57,7 +57,7 @@ class PackedPrompts:
 def prompt_attn(q, k, v, plan: PackedPrompts, sm_scale=None, out=None):
     """q [Tq, H, D], k / v [Tk, HK, D] bf16, packed as ``plan`` says -> [Tq, H, D] bf16.
     ``sm_scale``: default D ** -0.5.  ``out``: written in place if given (any strides with
-    D contiguous, multiples of 8 elements; no memory of k's or v's).  Scores up to 5e8 in
+    D contiguous, multiples of 8 elements; no memory of k's or v's, of q's only as q itself).  Scores up to 5e8 in
     magnitude: past that the softmax's exponents lose their fp32 range and NaN may come."""
     if out is None and isinstance(plan, PackedPrompts):
         y = _lib.calls().prompt_attn(q, k, v, plan.Tq, plan.Tk, *plan._lists, sm_scale)

@@ -326,6 +326,17 @@ def test_values_that_are_not_finite_in_whole_and_partial_steps(what, H, HK, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,HK,D", [(8, 2, 128), (2, 2, 64), (4, 2, 256)])
+def test_result_in_place_of_q(H, HK, D):
+    from respect_amd.kernels.prompt_attention import PackedPrompts, prompt_attn
+    rows = [300, 1, 77]
+    q, k, v = (t.cuda() for t in _inputs(rows, rows, H, HK, D, seed=17))
+    plan = PackedPrompts(rows)
+    want = prompt_attn(q, k, v, plan)
+    assert prompt_attn(q, k, v, plan, out=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.gpu
 def test_more_workgroups_than_a_grid_holds():
     """32900 one-token sequences of 512 heads: 16.8 M workgroups, more than the 2^32 threads of a grid
     dimension, whose count would start again at 0; every result is its one value."""
