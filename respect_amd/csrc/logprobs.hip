@@ -19,7 +19,7 @@
 //
 // What bounds it: the read of the scores, where there are many (1500 rows of 151936, top 5:
 // 911 MB in 190 us, 4.8 TB/s; torch's sum over them reads 4.0); for one row two launches and
-// the selection's dependent steps (6.5 us without alternatives, 10.0 with one, 14.2 with 20).
+// the selection's dependent steps (kernels 6.0 us without alternatives, 9.6 with one, 13.4 with 20).
 #include "common.h"
 #include "respect_amd.h"
 
@@ -394,8 +394,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogArgs A) {
 
 // Workgroups per row: about 4096 in all, 2048 where the lists are long, at most one per chunk.
 // A workgroup that takes more steps has its lists filled once for all of them (1000 rows, top
-// 50: 324 us with 8192 workgroups, 256 with 4096, 220 with 2048; 1500 rows, top 5: 215, 195,
-// 198), fewer of them fill the device less evenly (64 rows, top 20: 34, 34, 39).
+// 50: 303 us with 8192 workgroups, 242 with 4096, 210 with 2048; 1500 rows, top 5: 192, 187,
+// 194), fewer of them fill the device less evenly (64 rows, top 20: 26.5, 26.5, 33.9).
 int parts_of(int M, int chunks, int top) {
   const int total = top > 24 ? 2048 : 4096;
   const int want = (total + M - 1) / M;
