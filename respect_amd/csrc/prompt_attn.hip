@@ -22,10 +22,11 @@
 // tile it falls in or on later rows.
 //
 // What bounds it: in long prompts the power budget (16384 tokens, 32 / 8 heads of 128: 1.86 to
-// 1.97 ms by the card, 1.12 to 1.18 PFLOP/s, where a large library product reaches 1.41; the clock is down to 1.7 GHz, the
-// MFMAs are busy 65 % of it, VALU half; the LDS reads, 128 KB per step and workgroup, take half
-// as long as the MFMAs, without bank conflicts); in short ones and few heads what one wave per
-// SIMD issues in a step (0.87 us at D = 128, of which the MFMAs are 0.48; memory has no part
+// 1.97 ms by the card, 1.12 to 1.18 PFLOP/s, where a large library product reaches 1.41; the
+// clock is down to 1.7 GHz, the MFMAs are busy 65 % of it, VALU half; the LDS reads, 128 KB per
+// step and workgroup, take half as long as the MFMAs, without bank conflicts); in packed prompts
+// besides it the starts and ends of the workgroups; in short ones and few heads what one wave
+// per SIMD issues in a step (0.87 us at D = 128, of which the MFMAs are 0.48; memory has no part
 // in it: keys that all lie in one row take as long).  The order of the whole steps, held by
 // scheduling barriers, took 3 % off the long cases (the compiler's own: 1.93 ms beside 1.87, 24
 // packed prompts 278 us beside 270) and nothing off the short; addresses worked out once and
