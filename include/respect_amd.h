@@ -33,6 +33,9 @@
  *   rspx_prompt_attn    causal attention over whole prompts, packed
  *   rspx_paged_attn     attention of one new token per sequence over a paged cache
  *   rspx_kv_move, rspx_kv_write   rows of a paged cache moved and written
+ *   rspx_kv_write_mx, rspx_kv_read, rspx_kv_move_mx   the same for rows of 8 or 4 bits; rows read back
+ *   rspx_paged_attn_mx, rspx_paged_attn_shared        attention over such rows; over beginnings
+ *                       that sequences share
  *   rspx_pages_*        who holds which page of it (host code)
  *   rspx_token_logprobs log probabilities, entropy and best alternatives per row
  */
@@ -77,7 +80,7 @@ const char* rspx_strerror(int code);
 
 /* Library version.  The last number goes up with every change of a signature in this
  * header: code compiled against another one compares it before its first call. */
-#define RSPX_VERSION "respect_amd 0.1.0 gfx950 abi 2"
+#define RSPX_VERSION "respect_amd 0.1.0 gfx950 abi 3"
 const char* rspx_version(void);
 
 /* ---------------------------------------------------------------- attention
@@ -502,6 +505,64 @@ int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int
                     int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages, int page, int width,
                     float sm_scale, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- formats of a cache's rows
+ * RSPX_BF16: D bf16.  RSPX_MXFP8 / RSPX_MXFP4: D codes of 8 bits (e4m3, no infinities, up to
+ * 448) or 4 (e2m1, up to 6; element 2 i in the low half of byte i), and in a pool of its own a
+ * byte e for each 32 consecutive ones, whose values are the codes' times 2^(e - 127); e = 255:
+ * NaN.  A format's number is its bits per element.  Strides are in elements of the pool: bf16,
+ * or bytes; codes need 16-byte aligned bases and strides, scales none (their bytes lie together).
+ * rspx_kv_write_mx: rows k / v [T, HK, D] bf16 to slots[t] of one layer's pools, slots as in
+ * rspx_kv_write: e the smallest that no element of the 32 outgrows and >= 10, codes rounded to
+ * nearest, ties to even; 32 elements with an infinity or a NaN among them become NaN.
+ * rspx_kv_read: rows slots[t] of one layer's pools of any format to k / v [T, HK, D] bf16, exact
+ * (2^128, to which numbers next to bf16's largest round, becomes an infinity);
+ * a slot outside [0, cap) gives a row of NaN.  Scales are not read for RSPX_BF16.
+ * D a multiple of 32 (of 8 for RSPX_BF16) and <= 2048; HK <= 65535.
+ */
+#define RSPX_BF16 16
+#define RSPX_MXFP8 8
+#define RSPX_MXFP4 4
+int rspx_kv_write_mx(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh, const int32_t* slots,
+                     int T, int cap, void* k_codes, int64_t skch, int64_t skcn, void* k_scales, int64_t sksh, int64_t sksn,
+                     void* v_codes, int64_t svch, int64_t svcn, void* v_scales, int64_t svsh, int64_t svsn, int HK, int D,
+                     int format, void* stream);
+int rspx_kv_read(const void* k_codes, int64_t skch, int64_t skcn, const void* k_scales, int64_t sksh, int64_t sksn,
+                 const void* v_codes, int64_t svch, int64_t svcn, const void* v_scales, int64_t svsh, int64_t svsn,
+                 const int32_t* slots, int T, int cap, void* k, int64_t skt, int64_t skh, void* v, int64_t svt, int64_t svh,
+                 int HK, int D, int format, void* stream);
+
+/* ---------------------------------------------------------------- paged attention, other caches
+ * rspx_paged_attn_mx: rspx_paged_attn over pools of codes and scales (not RSPX_BF16), with the
+ * same workspace.
+ * rspx_paged_attn_shared: the same over pools of any format for a batch with groups of
+ * consecutive sequences that begin with the same keys, which are read once for the group.
+ * rspx_shared_plan: for n groups of members[i] sequences (all of the batch, in order), whose first
+ * keys[i] keys are the same rows, with `group` = H / HK <= 16: prefix [B] int32, the keys of
+ * each sequence that are taken together (keys[i] rounded down to whole steps of 64; 0 for a
+ * group of one), and tiles [count][8] int32; returns count (prefix and tiles, host memory, may be
+ * NULL).  Both go to the device as they are; longest: the largest of prefix.
+ * Which pages a group's shared keys lie in is read from the table row of its first sequence.
+ * A sequence of fewer keys than its prefix goes through all of its own by itself.  Lengths,
+ * pages and refusals as for rspx_paged_attn (a bad page among the shared ones: NaN for all who
+ * read it).  The shared part rounds probabilities to bf16, half a step each, and sums them as
+ * rounded.  A sequence's bits depend on its own keys and length and on its prefix alone.
+ * workspace: rspx_paged_attn_shared_workspace_bytes, as for rspx_paged_attn.
+ */
+int rspx_paged_attn_mx(const void* q, int64_t sqb, int64_t sqh, const void* k_codes, int64_t skch, int64_t skcn,
+                       const void* k_scales, int64_t sksh, int64_t sksn, const void* v_codes, int64_t svch, int64_t svcn,
+                       const void* v_scales, int64_t svsh, int64_t svsn, const int32_t* table, int64_t stb,
+                       const int32_t* lens, void* out, int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages,
+                       int page, int width, float sm_scale, int format, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+int64_t rspx_shared_plan(const int64_t* members, const int64_t* keys, int n, int group, int32_t* prefix, int32_t* tiles);
+int64_t rspx_paged_attn_shared_workspace_bytes(int B, int H, int D, int page, int width, int longest);
+int rspx_paged_attn_shared(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn,
+                           const void* k_scales, int64_t sksh, int64_t sksn, const void* vc, int64_t svh, int64_t svn,
+                           const void* v_scales, int64_t svsh, int64_t svsn, const int32_t* table, int64_t stb,
+                           const int32_t* lens, const int32_t* prefix, const int32_t* tiles, int n_tiles, int longest,
+                           void* out, int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages, int page, int width,
+                           float sm_scale, int format, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- rows of a paged cache
  * rspx_kv_move: for each of n_tensors pools (device array `bases` of base addresses,
  * each [HK][cap][D] bf16, 16-byte aligned, head stride sh, slot stride sn) and each head, the moves
@@ -513,6 +574,8 @@ int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int
  * rspx_kv_move_values: the same for lists in host memory of at most RSPX_VALUES
  * numbers in all (n_groups + 1 + 2 n_moves; RSPX_EUNSUPPORTED past it), which go with the
  * launch: read before the call returns.
+ * rspx_kv_move_mx, rspx_kv_move_mx_values: the same for n_tensors pools of codes, whose bases come
+ * first, and as many of their scales, in the same order (8-byte aligned), strides in bytes.
  * rspx_values: up to RSPX_VALUES numbers of host memory to out, likewise (tables, slots).
  * rspx_kv_write: rows k / v [T, HK, D] of one layer to slots[t] of its pools; a slot
  * outside [0, cap) is skipped; slots differ.
@@ -522,6 +585,11 @@ int rspx_kv_move(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh
 #define RSPX_VALUES 960
 int rspx_kv_move_values(const uint64_t* bases, int n_tensors, int HK, int D, int64_t sh, int64_t sn, int cap,
                         const int32_t* groups, int n_groups, const int32_t* moves, int n_moves, void* stream);
+int rspx_kv_move_mx(const uint64_t* bases, int n_tensors, int HK, int D, int format, int64_t sch, int64_t scn, int64_t ssh,
+                    int64_t ssn, int cap, const int32_t* groups, int n_groups, const int32_t* moves, int n_moves, void* stream);
+int rspx_kv_move_mx_values(const uint64_t* bases, int n_tensors, int HK, int D, int format, int64_t sch, int64_t scn,
+                           int64_t ssh, int64_t ssn, int cap, const int32_t* groups, int n_groups, const int32_t* moves,
+                           int n_moves, void* stream);
 int rspx_values(const int32_t* values, int n, int32_t* out, void* stream);
 int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_t svt, int64_t svh,
                   const int32_t* slots, int T, int cap, void* cache_k, int64_t sckh, int64_t sckn, void* cache_v,
@@ -548,6 +616,9 @@ int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_
  *   width    the most pages that one of ids holds;  table: [n][width] page numbers, -1 past
  *            a sequence's pages, and lens [n], as rspx_paged_attn takes them
  *   slots    pool rows of rows first[i] .. first[i] + counts[i] - 1, one sequence after another
+ *   shared   the batch ids cut into groups of consecutive sequences that begin with the same full
+ *            pages, so that most keys are shared: writes members and keys (of each group; n of
+ *            room) and returns their number.  Fewer than `least` keys count as none
  */
 typedef struct rspx_pages rspx_pages;
 rspx_pages* rspx_pages_new(int pages, int page, int sequences); /* NULL: bad sizes or no memory */
@@ -567,6 +638,7 @@ int rspx_pages_copy_moves(const rspx_pages* p, int32_t* out);
 int rspx_pages_width(rspx_pages* p, const int32_t* ids, int n);
 int rspx_pages_table(rspx_pages* p, const int32_t* ids, int n, int width, int32_t* table, int32_t* lens);
 int rspx_pages_slots(rspx_pages* p, const int32_t* ids, int n, const int64_t* first, const int64_t* counts, int32_t* out);
+int rspx_pages_shared(rspx_pages* p, const int32_t* ids, int n, int64_t least, int64_t* members, int64_t* keys);
 
 /* ---------------------------------------------------------------- scores of given tokens
  * Per row of logits [M, V] (fp32, row stride sl, any 4-byte alignment), with columns

@@ -94,6 +94,24 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_paged_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
     "rspx_paged_attn": (_i32, [_c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _c_p, _c_p, _i64, _i64,
                                _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _c_p, _i64, _c_p]),
+    "rspx_paged_attn_mx": (_i32, [
+        _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64,   # q; k, v codes and scales
+        _c_p, _i64, _c_p, _c_p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _c_p, _i64, _c_p]),
+    "rspx_shared_plan": (_i64, [_c_p, _c_p, _i32, _i32, _c_p, _c_p]),
+    "rspx_paged_attn_shared_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "rspx_paged_attn_shared": (_i32, [
+        _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64,   # q; k, v rows and scales
+        _c_p, _i64, _c_p, _c_p, _c_p, _i32, _i32, _c_p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
+        _c_p, _i64, _c_p]),
+    "rspx_kv_write_mx": (_i32, [
+        _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i32, _i32,                                       # k, v, slots
+        _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _i32, _i32, _i32, _c_p]),
+    "rspx_kv_read": (_i32, [
+        _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i32, _i32,
+        _c_p, _i64, _i64, _c_p, _i64, _i64, _i32, _i32, _i32, _c_p]),
+    "rspx_kv_move_mx": (_i32, [_c_p, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
+    "rspx_kv_move_mx_values": (_i32, [_c_p, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32,
+                                      _c_p]),
     "rspx_kv_move": (_i32, [_c_p, _i32, _i32, _i32, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
     "rspx_kv_move_values": (_i32, [_c_p, _i32, _i32, _i32, _i64, _i64, _i32, _c_p, _i32, _c_p, _i32, _c_p]),
     "rspx_values": (_i32, [_c_p, _i32, _c_p, _c_p]),
@@ -115,6 +133,7 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_pages_width": (_i32, [_c_p, _c_p, _i32]),
     "rspx_pages_table": (_i32, [_c_p, _c_p, _i32, _i32, _c_p, _c_p]),
     "rspx_pages_slots": (_i32, [_c_p, _c_p, _i32, _c_p, _c_p, _c_p]),
+    "rspx_pages_shared": (_i32, [_c_p, _c_p, _i32, _i64, _c_p, _c_p]),
     "rspx_token_logprobs_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "rspx_token_logprobs": (_i32, [_c_p, _i64, _i32, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _i64,
                                    _c_p]),

@@ -463,6 +463,143 @@ PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// One layer's pool in any format: rows [HK, slots, D] bf16, or uint8 codes with their scales.
+struct CachePool {
+  const Tensor *rows = nullptr, *scales = nullptr;
+  int64_t HK, slots, D;
+  bool read(PyObject* r, PyObject* s, int64_t bits) {
+    if (bits == RSPX_BF16) {
+      rows = input(r);
+      if (!rows || rows->dim() != 3 || s != Py_None) return false;
+    } else {
+      rows = plain(r, at::kByte);
+      scales = plain(s, at::kByte);
+      if (!rows || !scales || rows->dim() != 3 || scales->dim() != 3 || rows->stride(2) != 1 ||
+          (scales->size(2) > 1 && scales->stride(2) != 1) || scales->size(0) != rows->size(0) ||
+          scales->size(1) != rows->size(1) || rows->size(2) != 4 * bits * scales->size(2) || scales->device() != rows->device())
+        return false;
+    }
+    HK = rows->size(0), slots = rows->size(1);
+    D = bits == RSPX_BF16 ? rows->size(2) : 32 * scales->size(2);
+    return fits_int(HK) && fits_int(slots) && fits_int(D);
+  }
+  bool like(const CachePool& o) const {
+    return HK == o.HK && slots == o.slots && D == o.D && rows->device() == o.rows->device();
+  }
+  const void* scale_ptr() const { return scales ? ptr(*scales) : nullptr; }
+  int64_t ssh() const { return scales ? scales->stride(0) : 0; }
+  int64_t ssn() const { return scales ? scales->stride(1) : 0; }
+};
+
+bool format_of(PyObject* o, int64_t& bits) { return integer(o, bits) && (bits == RSPX_BF16 || bits == RSPX_MXFP8 || bits == RSPX_MXFP4); }
+
+// int32 numbers of the pool's device, contiguous.
+const Tensor* numbers(PyObject* o, const Tensor& like) {
+  const Tensor* t = plain(o, at::kInt);
+  return t && t->device() == like.device() && t->is_contiguous() ? t : nullptr;
+}
+
+// paged_attn_any(q, k, k_scales, v, v_scales, bits, table, lens, page, sm_scale, prefix, tiles, longest,
+// group): over a cache of any format (no scales: None); prefix None: no sequences begin alike
+PyObject* paged_attn_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 14) NOT_TAKEN;
+  int64_t bits, page, longest = 0, group = 0;
+  CachePool k, v;
+  const Tensor *q = input(a[0]), *t = plain(a[6], at::kInt);
+  if (!q || !t || !format_of(a[5], bits) || !k.read(a[1], a[2], bits) || !v.read(a[3], a[4], bits) || !k.like(v) ||
+      q->dim() != 3 || q->device() != k.rows->device() || t->dim() != 2 || t->device() != q->device())
+    NOT_TAKEN;
+  const Tensor* l = numbers(a[7], *q);
+  const int64_t B = q->size(0), H = q->size(1), D = q->size(2), width = t->size(1);
+  double scale;
+  if (!l || l->dim() != 1 || D != k.D || !integer(a[8], page) || page < 1 || k.slots % page || t->size(0) != B ||
+      l->size(0) != B || (width > 1 && t->stride(1) != 1) || !softmax_scale(a[9], D, scale))
+    NOT_TAKEN;
+  for (int64_t x : {B, H, width, page})
+    if (!fits_int(x)) NOT_TAKEN;
+  const bool shared = a[10] != Py_None;
+  const Tensor *prefix = nullptr, *tiles = nullptr;
+  if (shared) {
+    prefix = numbers(a[10], *q), tiles = numbers(a[11], *q);
+    if (!prefix || !tiles || !integer(a[12], longest) || !integer(a[13], group) || prefix->numel() != B || longest < 0 ||
+        longest > width * page || !fits_int(longest) || !fits_int(tiles->numel()) || H != k.HK * group)
+      NOT_TAKEN;
+  }
+  const int64_t need = std::max<int64_t>(
+      0, rspx_paged_attn_shared_workspace_bytes((int)B, (int)H, (int)D, (int)page, (int)width, (int)longest));
+  const c10::DeviceGuard guard(q->device());
+  Tensor y = empty_like_of(*q, {B, H, D}), ws;
+  if (need) ws = empty_like_of(*q, {need}, at::kByte);
+  void* w = need ? ws.data_ptr() : nullptr;
+  const int rc = call([&] {
+    const int pages = (int)(k.slots / page);
+    if (shared)
+      return rspx_paged_attn_shared(ptr(*q), q->stride(0), q->stride(1), ptr(*k.rows), k.rows->stride(0), k.rows->stride(1),
+                                    k.scale_ptr(), k.ssh(), k.ssn(), ptr(*v.rows), v.rows->stride(0), v.rows->stride(1),
+                                    v.scale_ptr(), v.ssh(), v.ssn(), t->const_data_ptr<int>(), t->stride(0),
+                                    l->const_data_ptr<int>(), prefix->const_data_ptr<int>(), tiles->const_data_ptr<int>(),
+                                    (int)(tiles->numel() / 8), (int)longest, y.data_ptr(), H * D, D, (int)B, (int)H, (int)k.HK,
+                                    (int)D, pages, (int)page, (int)width, (float)scale, (int)bits, w, need, stream_of(*q));
+    return rspx_paged_attn_mx(ptr(*q), q->stride(0), q->stride(1), ptr(*k.rows), k.rows->stride(0), k.rows->stride(1),
+                              k.scale_ptr(), k.ssh(), k.ssn(), ptr(*v.rows), v.rows->stride(0), v.rows->stride(1),
+                              v.scale_ptr(), v.ssh(), v.ssn(), t->const_data_ptr<int>(), t->stride(0), l->const_data_ptr<int>(),
+                              y.data_ptr(), H * D, D, (int)B, (int)H, (int)k.HK, (int)D, pages, (int)page, (int)width,
+                              (float)scale, (int)bits, w, need, stream_of(*q));
+  });
+  STATUS(rc);
+  return wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_write_mx(k, v, k_codes, k_scales, v_codes, v_scales, slots, bits) -> True
+PyObject* kv_write_mx(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t bits;
+  CachePool ck, cv;
+  if (n != 8 || !format_of(a[7], bits) || bits == RSPX_BF16 || !ck.read(a[2], a[3], bits) || !cv.read(a[4], a[5], bits) ||
+      !ck.like(cv))
+    NOT_TAKEN;
+  const Tensor *k = input(a[0]), *v = input(a[1]), *slots = numbers(a[6], *ck.rows);
+  if (!k || !v || !slots || k->dim() != 3 || v->sizes() != k->sizes() || k->device() != ck.rows->device() ||
+      v->device() != k->device() || slots->dim() != 1 || k->size(0) != slots->size(0) || k->size(1) != ck.HK || k->size(2) != ck.D ||
+      !fits_int(k->size(0)))
+    NOT_TAKEN;
+  const c10::DeviceGuard guard(k->device());
+  const int rc = call([&] {
+    return rspx_kv_write_mx(ptr(*k), k->stride(0), k->stride(1), ptr(*v), v->stride(0), v->stride(1), slots->const_data_ptr<int>(),
+                            (int)k->size(0), (int)ck.slots, const_cast<void*>(ptr(*ck.rows)), ck.rows->stride(0),
+                            ck.rows->stride(1), const_cast<void*>(ck.scale_ptr()), ck.ssh(), ck.ssn(),
+                            const_cast<void*>(ptr(*cv.rows)), cv.rows->stride(0), cv.rows->stride(1),
+                            const_cast<void*>(cv.scale_ptr()), cv.ssh(), cv.ssn(), (int)ck.HK, (int)ck.D, (int)bits, stream_of(*k));
+  });
+  STATUS(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv_read(k, k_scales, v, v_scales, slots, bits) -> (k, v)
+PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t bits;
+  CachePool ck, cv;
+  if (n != 6 || !format_of(a[5], bits) || !ck.read(a[0], a[1], bits) || !cv.read(a[2], a[3], bits) || !ck.like(cv)) NOT_TAKEN;
+  const Tensor* slots = numbers(a[4], *ck.rows);
+  if (!slots || slots->dim() != 1 || !fits_int(slots->size(0))) NOT_TAKEN;
+  const int64_t T = slots->size(0);
+  const c10::DeviceGuard guard(slots->device());
+  Tensor k = empty_like_of(*slots, {T, ck.HK, ck.D}, at::kBFloat16), v = empty_like_of(*slots, {T, ck.HK, ck.D}, at::kBFloat16);
+  const int rc = call([&] {
+    return rspx_kv_read(ptr(*ck.rows), ck.rows->stride(0), ck.rows->stride(1), ck.scale_ptr(), ck.ssh(), ck.ssn(), ptr(*cv.rows),
+                        cv.rows->stride(0), cv.rows->stride(1), cv.scale_ptr(), cv.ssh(), cv.ssn(), slots->const_data_ptr<int>(),
+                        (int)T, (int)ck.slots, k.data_ptr(), ck.HK * ck.D, ck.D, v.data_ptr(), ck.HK * ck.D, ck.D, (int)ck.HK,
+                        (int)ck.D, (int)bits, stream_of(*slots));
+  });
+  STATUS(rc);
+  return Py_BuildValue("(NN)", wrap(std::move(k)), wrap(std::move(v)));
+  END_HANDLE_TH_ERRORS
+}
+
 // token_logprobs(logits, tokens, top, offset, size)
 PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -492,7 +629,8 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------ pages of a paged cache
-// handle: the rspx_pages*; bases, HK, D, sh, sn, cap: the pools as rspx_kv_move takes them.
+// handle: the rspx_pages*; bases, HK, D, sh, sn, cap: the pools as rspx_kv_move takes them, or with
+// bits, ssh, ssn behind them as rspx_kv_move_mx does.
 
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
@@ -523,9 +661,13 @@ bool counts_of(PyObject* o, size_t n, std::vector<int64_t>& v) {
 struct Pool {
   rspx_pages* pages;
   const Tensor* bases;
-  int64_t HK, D, sh, sn, cap;
+  int64_t HK, D, sh, sn, cap, bits = RSPX_BF16, ssh = 0, ssn = 0;
   bool read(PyObject* handle, PyObject* const* a, Py_ssize_t n) {
     int64_t h;
+    if (n == 9) {
+      if (!format_of(a[6], bits) || bits == RSPX_BF16 || !integer(a[7], ssh) || !integer(a[8], ssn)) return false;
+      n = 6;
+    }
     if (n != 6 || !integer(handle, h) || h == 0 || !(bases = plain(a[0], at::kLong))) return false;
     pages = reinterpret_cast<rspx_pages*>(h);
     return integer(a[1], HK) && integer(a[2], D) && integer(a[3], sh) && integer(a[4], sn) && integer(a[5], cap);
@@ -557,6 +699,10 @@ int enqueue_moves(const Pool& p) {
     int32_t lists[RSPX_VALUES];
     rspx_pages_copy_moves(p.pages, lists);
     return call([&] {
+      if (p.bits != RSPX_BF16)
+        return rspx_kv_move_mx_values(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel() / 2, (int)p.HK, (int)p.D,
+                                      (int)p.bits, p.sh, p.sn, p.ssh, p.ssn, (int)p.cap, lists, groups, lists + groups + 1, moves,
+                                      stream_of(*p.bases));
       return rspx_kv_move_values(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel(), (int)p.HK, (int)p.D, p.sh,
                                  p.sn, (int)p.cap, lists, groups, lists + groups + 1, moves, stream_of(*p.bases));
     });
@@ -564,6 +710,9 @@ int enqueue_moves(const Pool& p) {
   Tensor t = uploaded(*p.bases, (int64_t)groups + 1 + 2 * (int64_t)moves, [&](int* out) { rspx_pages_copy_moves(p.pages, out); });
   return call([&] {
     const int32_t* d = t.const_data_ptr<int>();
+    if (p.bits != RSPX_BF16)
+      return rspx_kv_move_mx(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel() / 2, (int)p.HK, (int)p.D,
+                             (int)p.bits, p.sh, p.sn, p.ssh, p.ssn, (int)p.cap, d, groups, d + groups + 1, moves, stream_of(*p.bases));
     return rspx_kv_move(static_cast<const uint64_t*>(ptr(*p.bases)), (int)p.bases->numel(), (int)p.HK, (int)p.D, p.sh, p.sn,
                         (int)p.cap, d, groups, d + groups + 1, moves, stream_of(*p.bases));
   });
@@ -601,7 +750,7 @@ PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pool p;
   std::vector<int32_t> ids;
   int64_t copies;
-  if (n != 9 || !p.read(a[0], a + 3, 6) || !integers(a[1], ids) || !integer(a[2], copies) || !fits_int(copies)) NOT_TAKEN;
+  if (n < 9 || !p.read(a[0], a + 3, n - 3) || !integers(a[1], ids) || !integer(a[2], copies) || !fits_int(copies)) NOT_TAKEN;
   const c10::DeviceGuard guard(p.bases->device());
   if (capturing() || (int64_t)ids.size() * copies > 1 << 24) NOT_TAKEN;
   std::vector<int32_t> out(ids.size() * copies);
@@ -619,7 +768,7 @@ PyObject* pages_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pool p;
   std::vector<int32_t> ids;
   std::vector<int64_t> counts;
-  if (n != 9 || !p.read(a[0], a + 3, 6) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), counts)) NOT_TAKEN;
+  if (n < 9 || !p.read(a[0], a + 3, n - 3) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), counts)) NOT_TAKEN;
   const c10::DeviceGuard guard(p.bases->device());
   if (capturing()) NOT_TAKEN;
   STATUS(rspx_pages_extend(p.pages, ids.data(), (int)ids.size(), counts.data()));
@@ -634,7 +783,7 @@ PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pool p;
   std::vector<int32_t> ids;
   std::vector<int64_t> starts, paths, ends;
-  if (n != 10 || !p.read(a[0], a + 4, 6) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), starts) ||
+  if (n < 10 || !p.read(a[0], a + 4, n - 4) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), starts) ||
       !PyList_CheckExact(a[3]) || PyList_GET_SIZE(a[3]) != (Py_ssize_t)ids.size())
     NOT_TAKEN;
   for (size_t i = 0; i < ids.size(); ++i) {
@@ -665,7 +814,7 @@ PyObject* pages_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pool p;
   std::vector<int32_t> ids;
-  if (n != 8 || !p.read(a[0], a + 2, 6) || !integers(a[1], ids)) NOT_TAKEN;
+  if (n < 8 || !p.read(a[0], a + 2, n - 2) || !integers(a[1], ids)) NOT_TAKEN;
   const c10::DeviceGuard guard(p.bases->device());
   if (capturing()) NOT_TAKEN;
   const int64_t B = (int64_t)ids.size(), width = rspx_pages_width(p.pages, ids.data(), (int)B);
@@ -683,7 +832,7 @@ PyObject* pages_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pool p;
   std::vector<int32_t> ids;
   std::vector<int64_t> first, counts;
-  if (n != 10 || !p.read(a[0], a + 4, 6) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), first) ||
+  if (n < 10 || !p.read(a[0], a + 4, n - 4) || !integers(a[1], ids) || !counts_of(a[2], ids.size(), first) ||
       !counts_of(a[3], ids.size(), counts))
     NOT_TAKEN;
   const c10::DeviceGuard guard(p.bases->device());
@@ -706,7 +855,7 @@ PyObject* pages_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {FAST(silu_mul), FAST(rmsnorm), FAST(qk_norm_rope), FAST(rmsnorm_qk_norm_rope),
                          FAST(rope),     FAST(add_sq),  FAST(norm_apply),   FAST(rope_vision),
                          FAST(linear),   FAST(trie_attn), FAST(prompt_attn), FAST(paged_attn),
-                         FAST(token_logprobs), FAST(pages_fork), FAST(pages_extend), FAST(pages_compact),
+                         FAST(token_logprobs), FAST(paged_attn_any), FAST(kv_write_mx), FAST(kv_read), FAST(pages_fork), FAST(pages_extend), FAST(pages_compact),
                          FAST(pages_tables),   FAST(pages_slots), FAST(pages_free), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -38,6 +38,8 @@ namespace {
 
 using Pages = rspx_pages;
 
+constexpr int kMostMembers = 4096;    // of a group of sequences that begin alike: bounds the search
+
 int64_t pages_for(const Pages& p, int64_t rows) { return (rows + p.page - 1) / p.page; }
 
 int check_ids(Pages& p, const int32_t* ids, int n, bool distinct) {
@@ -417,4 +419,41 @@ extern "C" int rspx_pages_slots(rspx_pages* p, const int32_t* ids, int n, const 
   for (int i = 0; i < n; ++i)
     for (int64_t r = first[i]; r < first[i] + counts[i]; ++r) *out++ = slot(*p, p->held[ids[i]], r);
   return RSPX_OK;
+}
+
+extern "C" int rspx_pages_shared(rspx_pages* p, const int32_t* ids, int n, int64_t least, int64_t* members, int64_t* keys) {
+  if (!p || least < 0) return RSPX_EINVAL;
+  if (const int rc = check_ids(*p, ids, n, false)) return rc;
+  if (n > 0 && (!members || !keys)) return RSPX_EINVAL;
+  return guarded([&] {
+    // alike[i]: the full pages that sequences i - 1 and i begin with alike.
+    std::vector<int64_t> alike(n, 0), best(n + 1, 0);
+    std::vector<int32_t> from(n + 1, 0);
+    for (int i = 1; i < n; ++i) {
+      const std::vector<int32_t>&a = p->held[ids[i - 1]], &b = p->held[ids[i]];
+      const int64_t most = std::min(p->len[ids[i - 1]], p->len[ids[i]]) / p->page;
+      int64_t& k = alike[i];
+      while (k < most && a[k] == b[k]) ++k;
+    }
+    // best[j]: the most keys that need not be read again, of the sequences before j.
+    for (int j = 1; j <= n; ++j) {
+      best[j] = best[j - 1], from[j] = j - 1;
+      int64_t common = INT64_MAX;
+      for (int i = j - 2; i >= 0 && j - i <= kMostMembers; --i) {
+        common = std::min(common, alike[i + 1]);
+        if (common == 0) break;
+        const int64_t saved = common * p->page * (j - i - 1);
+        if (common * p->page >= least && best[i] + saved > best[j]) best[j] = best[i] + saved, from[j] = i;
+      }
+    }
+    int groups = 0;
+    for (int j = n; j > 0; j = from[j]) ++groups;
+    int at = groups;
+    for (int j = n; j > 0; j = from[j]) {
+      int64_t common = j - from[j] > 1 ? INT64_MAX : 0;
+      for (int i = from[j] + 1; i < j; ++i) common = std::min(common, alike[i]);
+      members[--at] = j - from[j], keys[at] = common * p->page;
+    }
+    return groups;
+  });
 }

@@ -1,4 +1,5 @@
-// Attention of one new token per sequence over a paged KV cache, for gfx950.
+// Attention of one new token per sequence over a paged KV cache, for gfx950, whose rows are
+// bf16 or hold codes of 8 or 4 bits (mx.h), and whose sequences may begin alike.
 //
 //   o[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j,   j < lens[b],
 //
@@ -30,15 +31,15 @@
 // 17 MB take 3.3 of them).  Splits of 128 keys: 67 us instead of 64 for the batch, of 512: 17
 // instead of 13 for the one; at most 64 splits, or two tiles per wave requested at once: no
 // difference.
-#include "common.h"
+#include <algorithm>
+
+#include "keys64.h"
+#include "mx.h"
 #include "respect_amd.h"
 
 namespace rspx {
 
 namespace {
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kTile = 32;            // keys of a wave's step
 constexpr int kWaves = 4;
@@ -46,9 +47,13 @@ constexpr int kSplitKeys = 256;      // the shortest split
 constexpr int kMaxSplits = 32;       // a longer cache gets longer splits
 constexpr int kSeqs = 1024;          // sequences of a launch
 constexpr int kCUs = 256;
-constexpr float kTau = 8.0f;         // log2 headroom before the reference maximum moves
 constexpr float kTiny = 1.17549435e-38f;   // the smallest normal number
-constexpr float kNone = -1e30f;      // reference maximum before the first key
+
+// Shared beginnings: whole steps of kKeys keys, in splits of their own.
+constexpr int kPrefixSplitKeys = 256;
+constexpr int kMaxPrefixSplits = 16;
+constexpr int kPrefixRows = 32 * kWaves;   // rows (sequences by heads of a group) of a workgroup
+constexpr int kTileInts = 8;               // first sequence, rows, first row, first key, end, split
 
 // Keys per split of a sequence of n keys: a multiple of kSplitKeys.
 __host__ __device__ __forceinline__ int split_keys(int n) {
@@ -62,20 +67,47 @@ __host__ __device__ __forceinline__ int split_count(int n) {
 // The most splits that any length up to n gives.
 __host__ __forceinline__ int split_bound(int64_t n) { return n >= (int64_t)kSplitKeys * kMaxSplits ? kMaxSplits : split_count((int)n); }
 
+// The same for n shared keys, a multiple of kKeys.
+__host__ __device__ __forceinline__ int prefix_split_keys(int n) {
+  const unsigned per = ((unsigned)n + kMaxPrefixSplits - 1) / kMaxPrefixSplits;
+  return per <= kPrefixSplitKeys ? kPrefixSplitKeys : (int)((per + kKeys - 1) / kKeys * kKeys);
+}
+__host__ __device__ __forceinline__ int prefix_splits(int n) {
+  const unsigned k = (unsigned)prefix_split_keys(n);
+  return (int)(((unsigned)n + k - 1) / k);
+}
+__host__ __forceinline__ int prefix_split_bound(int n) { return n >= kPrefixSplitKeys * kMaxPrefixSplits ? kMaxPrefixSplits : prefix_splits(n); }
+
 struct PagedArgs {
-  const uint16_t *q, *k, *v;
+  const uint16_t* q;
+  const char *k, *v;           // pools, strides in bytes
+  const uint8_t *ks, *vs;      // their scales
   const int *table, *lens;
+  const int *prefix, *tiles;   // keys that a sequence shares; what to compute of them
   uint16_t* out;
-  float* po;                   // [B][H][smax][D]: a split's sums
+  float* po;                   // [B][H][smax][D]: a split's sums, the shared keys' splits first
   f32x2* pml;                  // [B][H][smax]: its m and l
-  int64_t sqb, sqh, skh, skn, svh, svn, stb, sob, soh;
-  int B, HK, G, pages, shift, width, smax;
+  int64_t sqb, sqh, skh, skn, svh, svn, sksh, sksn, svsh, svsn, stb, sob, soh;
+  int B, HK, G, pages, shift, width, smax, n_tiles, longest;
   float c;                     // scale * log2(e)
 };
 
+// Of sequence b, of n keys: those that the launch's tiles compute, 0 where it is too short for
+// them and goes through all of its own.
+template <bool SHARED>
+__device__ __forceinline__ int shared_keys(const PagedArgs& A, int b, int n) {
+  if constexpr (!SHARED) return 0;
+  const int p = A.prefix[b];
+  return p > 0 && p <= A.longest && p <= n && n <= ((int64_t)A.width << A.shift) ? p : 0;
+}
+
 // first[b]: the splits of sequences before b (one for a sequence without any, whose rows
 // are written too), length[b]: lens[b]; returns the number of splits.  All 256 threads call it.
-__device__ __forceinline__ int list_items(const int* lens, int B, int64_t cap, int* first, int* length) {
+// The keys that from[b] says are shared have splits elsewhere.
+template <bool SHARED>
+__device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* first, int* length, int* from) {
+  const int* lens = A.lens;
+  const int B = A.B;
   __shared__ int waves[4];
   constexpr int kPer = kSeqs / 256;
   int cnt[kPer], sum = 0;
@@ -87,6 +119,10 @@ __device__ __forceinline__ int list_items(const int* lens, int B, int64_t cap, i
       const int n = lens[b];
       length[b] = n;
       cnt[i] = n <= 0 || n > cap ? 1 : split_count(n);
+      if constexpr (SHARED) {
+        const int p = from[b] = shared_keys<true>(A, b, n);
+        if (p > 0) cnt[i] = split_count(n - p);
+      }
     }
     sum += cnt[i];
   }
@@ -122,26 +158,13 @@ __device__ __forceinline__ int find_seq(const int* first, int B, int i) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-__device__ __forceinline__ s16x4 tr_read(const lds_char* __restrict__ p) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-}
-
 // 16-byte unit swizzle of a staged V row: four consecutive keys' pairs of units lie in
 // different banks for the transposing reads.
 template <int D>
-__device__ __forceinline__ int vswizzle(int key) {
+__device__ __forceinline__ int tile_vswizzle(int key) {
   constexpr int U = D / 8;
   if constexpr (U >= 16) return 2 * (key % 8);
   else return 2 * ((key / (16 / U)) % (U / 2));
-}
-
-// A barrier that does not wait for the loads in flight.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 __device__ __forceinline__ float max4(float x) { return fmaxf(fmaxf(x, shfl_xor(x, 16)), fmaxf(shfl_xor(x, 32), shfl_xor(x, 48))); }
@@ -157,23 +180,33 @@ struct PagedGeom {
 
 // One split of one sequence for one kv head.
 struct Item {
-  int g, b, n, split, splits;
+  int g, b, from, n, split, splits;   // keys from .. from + n - 1
   int t, tend;                 // this wave's first tile, and the end of the split's
 };
 
-template <int D>
-__global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(PagedArgs A) {
+template <int D, bool SHARED>
+struct PagedLds {
+  char stage[kWaves][kTile * D * 2];
+  float sm[kWaves][16], sl[kWaves][16];
+  int first[kSeqs + 1], length[kSeqs], from[SHARED ? kSeqs : 1];
+};
+
+// Workgroup `block` of `blocks`: splits of the sequences' own keys.
+template <int D, int BITS, bool SHARED>
+__device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int blocks, char (*stage)[kTile * D * 2],
+                                            float (*sm)[16], float (*sl)[16], int* first, int* length, int* from) {
   constexpr int NQ = D / 32, DT = D / 16, U = D / 8;
-  constexpr int VL = kTile * U / 64;                       // 16-byte loads of a V tile per lane
-  __shared__ __align__(16) char stage[kWaves][kTile * D * 2];
-  __shared__ float sm[kWaves][16], sl[kWaves][16];
-  __shared__ int first[kSeqs + 1], length[kSeqs];
+  constexpr int RB = D * BITS / 8;                         // bytes of a row
+  // K: lane (key, r4) takes KN loads of KW bytes, KF operands each; V: a tile is VL loads of VW
+  // bytes per lane, VF units of the stage each.
+  constexpr int KW = RB / 4 < 16 ? RB / 4 : 16, KN = RB / 4 / KW, KE = KW * 8 / BITS, KF = KE / 8;
+  constexpr int VW = RB / 2 < 16 ? RB / 2 : 16, VU = RB / VW, VL = kTile * VU / 64, VE = VW * 8 / BITS, VF = VE / 8;
 
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, c16 = lane & 15, r4 = lane >> 4;
   const int64_t cap = (int64_t)A.width << A.shift;
-  const int items = list_items(A.lens, A.B, cap, first, length) * A.HK;
-  if ((int)blockIdx.x >= items) return;
+  const int items = list_items<SHARED>(A, cap, first, length, from) * A.HK;
+  if (block >= items) return;
 
   auto decode = [&](int i) {
     Item x;
@@ -181,8 +214,12 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
     x.b = find_seq(first, A.B, i / A.HK);
     x.split = i / A.HK - __builtin_amdgcn_readfirstlane(first[x.b]);
     x.n = __builtin_amdgcn_readfirstlane(length[x.b]);
-    x.splits = x.t = x.tend = 0;
+    x.splits = x.t = x.tend = x.from = 0;
     if (x.n > 0 && x.n <= cap) {
+      if constexpr (SHARED) {
+        x.from = __builtin_amdgcn_readfirstlane(from[x.b]);
+        x.n -= x.from;
+      }
       const int per = split_keys(x.n);
       x.splits = split_count(x.n);
       x.t = x.split * (per / kTile) + w;
@@ -193,49 +230,56 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
   // The pool slot of key 32 t + lane % 32; keys past the end give the last one's.  -1: the
   // page is none, and nothing of it is read.
   auto slot_of = [&](const Item& x, int t) {
-    const int key = min(t * kTile + (lane & 31), x.n - 1);
+    const int key = x.from + min(t * kTile + (lane & 31), x.n - 1);
     const int p = A.table[x.b * A.stb + (key >> A.shift)];
     return (unsigned)p < (unsigned)A.pages ? (p << A.shift) + (key & ((1 << A.shift) - 1)) : -1;
   };
-  u32x4 kf[2][NQ], vf[VL];
+  Words<KW> kf[2][KN];
+  Words<VW> vf[VL];
+  uint32_t kscale[2][KN], vscale[VL];
   auto load = [&](const Item& x, int slot) {
     slot = max(slot, 0);
-    const uint16_t* kb = A.k + x.g * A.skh;
-    const uint16_t* vb = A.v + x.g * A.svh;
+    const char* kb = A.k + x.g * A.skh;
+    const char* vb = A.v + x.g * A.svh;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint16_t* p = kb + shfl_idx_i(slot, 16 * j + c16) * A.skn + 8 * r4;
+      const int row = shfl_idx_i(slot, 16 * j + c16);
+      const char* p = kb + row * A.skn + KW * r4;
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) kf[j][i] = *reinterpret_cast<const u32x4*>(p + 32 * i);
+      for (int i = 0; i < KN; ++i) {
+        kf[j][i] = load_words<KW>(p + 4 * KW * i);
+        if constexpr (BITS < 16) kscale[j][i] = A.ks[x.g * A.sksh + row * A.sksn + KE * (4 * i + r4) / kGroup];
+      }
     }
 #pragma unroll
     for (int j = 0; j < VL; ++j) {
-      const int u = 64 * j + lane;
-      vf[j] = *reinterpret_cast<const u32x4*>(vb + shfl_idx_i(slot, u / U) * A.svn + 8 * (u % U));
+      const int u = 64 * j + lane, row = shfl_idx_i(slot, u / VU);
+      vf[j] = load_words<VW>(vb + row * A.svn + VW * (u % VU));
+      if constexpr (BITS < 16) vscale[j] = A.vs[x.g * A.svsh + row * A.svsn + VE * (u % VU) / kGroup];
     }
   };
-  // B operand of the scores: lane (c16, r4) holds head c16, head_dim 32 i + 8 r4 .. + 7.
+  // B operand of the scores: lane (c16, r4) holds head c16, the head_dims of the lane's keys.
   bf16x8 qf[NQ];
   auto load_q = [&](const Item& x) {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       u32x4 y = {0, 0, 0, 0};
       if (c16 < A.G)
-        y = *reinterpret_cast<const u32x4*>(A.q + x.b * A.sqb + (int64_t)(x.g * A.G + c16) * A.sqh + 32 * i + 8 * r4);
+        y = *reinterpret_cast<const u32x4*>(A.q + x.b * A.sqb + (int64_t)(x.g * A.G + c16) * A.sqh + KE * (4 * (i / KF) + r4) + 8 * (i % KF));
       qf[i] = __builtin_bit_cast(bf16x8, y);
     }
   };
 
   lds_char* st = (lds_char*)stage[w];
-  Item cur = decode(blockIdx.x);
+  Item cur = decode(block);
   int slot = -1;                                           // of the tile in kf and vf
   if (cur.t < cur.tend) {
     slot = slot_of(cur, cur.t);
     load_q(cur);
     load(cur, slot);
   }
-  for (int item = blockIdx.x;;) {
-    const int after = item + gridDim.x;
+  for (int item = block;;) {
+    const int after = item + blocks;
     Item nxt = cur;
     nxt.t = nxt.tend = 0;
     if (after < items) nxt = decode(after);
@@ -255,20 +299,24 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
         s[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-          s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[j][i]), qf[i], s[j], 0, 0, 0);
+          s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8, eight<BITS>(kf[j][i / KF], i % KF, mx_scale(BITS < 16 ? kscale[j][i / KF] : 0))), qf[i], s[j], 0, 0, 0);
       }
       const int left = cur.n - t * kTile;                  // keys of the tile that exist
       if (left < kTile) {   // the repeated last row: its p of 0 times inf would be NaN
 #pragma unroll
         for (int j = 0; j < VL; ++j)
-          if ((64 * j + lane) / U >= left) vf[j] = u32x4{0, 0, 0, 0};
+          if ((64 * j + lane) / VU >= left) vf[j] = Words<VW>{}, vscale[j] = kLeastScale;
       }
       // The stage belongs to this wave, whose LDS operations keep their order: the reads of
       // the tile before are done before these writes land.
 #pragma unroll
       for (int j = 0; j < VL; ++j) {
-        const int u = 64 * j + lane, key = u / U;
-        *(__attribute__((address_space(3))) u32x4*)(st + 16 * (key * U + ((u % U) ^ vswizzle<D>(key)))) = vf[j];
+        const int u = 64 * j + lane, key = u / VU;
+#pragma unroll
+        for (int i = 0; i < VF; ++i)
+          *(__attribute__((address_space(3))) u32x4*)(st + 16 * (key * U + ((u % VU * VF + i) ^ tile_vswizzle<D>(key)))) =
+              eight<BITS>(vf[j], i, mx_scale(BITS < 16 ? vscale[j] : 0));
       }
       if (t + kWaves < cur.tend) {
         bad |= ahead < 0;
@@ -311,7 +359,7 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const int key = 16 * z + 4 * r4 + (c16 >> 2), u = 2 * j + ((c16 & 3) >> 1);
-          h[z] = tr_read(st + 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (c16 & 1));
+          h[z] = tr_read(st + 16 * (key * U + (u ^ tile_vswizzle<D>(key))) + 8 * (c16 & 1));
         }
         const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, ph, acc[j], 0, 0, 0);
@@ -349,10 +397,10 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
           l = __builtin_fmaf(sl[k][h], a, l);
           o = __builtin_fmaf(so[(k * 16 + h) * D + d], a, o);
         }
-        if (cur.splits == 1) {
+        if (cur.splits == 1 && cur.from == 0) {
           orow[h * A.soh + d] = f32_to_bf16_rne(o / l);
         } else {
-          const int64_t p = (((int64_t)cur.b * A.HK + cur.g) * A.G + h) * A.smax + cur.split;
+          const int64_t p = (((int64_t)cur.b * A.HK + cur.g) * A.G + h) * A.smax + (SHARED ? prefix_splits(cur.from) : 0) + cur.split;
           A.po[p * D + d] = o;
           if (d == 0) A.pml[p] = f32x2{m, l};
         }
@@ -366,24 +414,225 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
   }
 }
 
+// What a tile says of shared keys: for up to kPrefixRows rows (sequence b0 + r / G, head r % G of
+// kv head g) and keys [key0, end), whole steps, the sums of a split.  Four waves of 32 rows; K and
+// V of a step go through registers, where they become bf16, into one of two slots of LDS while
+// the other one is read.  S^T = K Q^T by v_mfma_f32_32x32x16_bf16 leaves a row's scores in one
+// lane and its neighbour of the other half; the probabilities, rounded to bf16 (half a step each)
+// and summed as rounded, are used in place.  Every row sees all keys: there is no mask.
+template <int D, int BITS>
+__device__ __forceinline__ void prefix_tile(const PagedArgs& A, int total, int psmax, int index, char* lds) {
+  constexpr int U = D / 8, NS = D / 16, DT = D / 32;
+  constexpr int RB = D * BITS / 8, W = RB / 4 < 16 ? RB / 4 : 16, UR = RB / W, UL = kKeys * UR / 256;   // loads of a row, of a thread
+  constexpr int E = W * 8 / BITS, EU = E / 8;
+  constexpr int kBytes = kKeys * D * 2;                    // K or V of one step
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int g = index % A.HK;
+  const int* T = A.tiles + (int64_t)(index / A.HK) * kTileInts;
+  const int b0 = T[0], row0 = T[2], key0 = T[3], split = T[5];
+  const int64_t cap = (int64_t)A.width << A.shift;
+  if (b0 < 0 || b0 >= total || row0 < 0 || key0 < 0 || split < 0 || split >= psmax) return;
+  const int rows = (int)min((int64_t)min(T[1], kPrefixRows), (int64_t)(total - b0) * A.G - row0);
+  const int steps = (int)(min((int64_t)T[4], cap) - key0) / kKeys;
+  if (rows <= 0 || steps <= 0) return;
+  const bool active = 32 * w < rows;                       // this wave has rows
+  const int row = row0 + min(32 * w + col, rows - 1);
+  const int64_t bh = (int64_t)(b0 + row / A.G) * A.HK * A.G + g * A.G + row % A.G;
+  // A sequence that goes through all of its keys by itself has its own splits where these would be.
+  const bool stored = 32 * w + col < rows && shared_keys<true>(A, b0 + row / A.G, A.lens[b0 + row / A.G]) > 0;
+
+  // B operand of the scores: lane (col, half) holds row col, head_dim 16 i + 8 half .. + 7.
+  bf16x8 qf[NS];
+  if (active) {
+    const uint16_t* q = A.q + (b0 + row / A.G) * A.sqb + (int64_t)(g * A.G + row % A.G) * A.sqh + 8 * half;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) qf[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 16 * i));
+  }
+
+  // Load j of this thread: bytes W (u % UR) of key u / UR, u = 256 j + thread, of K and of V.
+  const int* table = A.table + b0 * A.stb;
+  bool bad = false;
+  auto lookup = [&](int t, int (&slot)[UL]) {
+#pragma unroll
+    for (int j = 0; j < UL; ++j) {
+      const int key = key0 + t * kKeys + (256 * j + (int)threadIdx.x) / UR;
+      const int p = table[key >> A.shift];
+      const bool ok = (unsigned)p < (unsigned)A.pages;
+      bad |= !ok;
+      slot[j] = ok ? (p << A.shift) + (key & ((1 << A.shift) - 1)) : 0;
+    }
+  };
+  Words<W> rk[UL], rv[UL];
+  uint32_t sk[UL], sv[UL];
+  const char* kb = A.k + g * A.skh;
+  const char* vb = A.v + g * A.svh;
+  auto fetch = [&](const int (&slot)[UL]) {
+#pragma unroll
+    for (int j = 0; j < UL; ++j) {
+      const int c = (256 * j + (int)threadIdx.x) % UR;
+      rk[j] = load_words<W>(kb + slot[j] * A.skn + W * c);
+      rv[j] = load_words<W>(vb + slot[j] * A.svn + W * c);
+      if constexpr (BITS < 16) {
+        sk[j] = A.ks[g * A.sksh + slot[j] * A.sksn + E * c / kGroup];
+        sv[j] = A.vs[g * A.svsh + slot[j] * A.svsn + E * c / kGroup];
+      }
+    }
+  };
+  auto put = [&](int t) {
+    lds_char* dk = (lds_char*)lds + kBytes * (t & 1);
+    lds_char* dv = (lds_char*)lds + kBytes * (2 + (t & 1));
+#pragma unroll
+    for (int j = 0; j < UL; ++j) {
+      const int u = 256 * j + (int)threadIdx.x, key = u / UR;
+#pragma unroll
+      for (int i = 0; i < EU; ++i) {
+        const int c = u % UR * EU + i;
+        *(__attribute__((address_space(3))) u32x4*)(dk + 16 * (key * U + (c ^ kswizzle<D>(key)))) =
+            eight<BITS>(rk[j], i, mx_scale(BITS < 16 ? sk[j] : 0));
+        *(__attribute__((address_space(3))) u32x4*)(dv + 16 * (key * U + (c ^ vswizzle<D>(key)))) =
+            eight<BITS>(rv[j], i, mx_scale(BITS < 16 ? sv[j] : 0));
+      }
+    }
+  };
+
+  int k_at = 16 * (col * U + (half ^ kswizzle<D>(col)));
+  int v_at;
+  {
+    const int l16 = lane & 15, key = 4 * half + (l16 >> 2), u = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    v_at = 16 * (key * U + (u ^ vswizzle<D>(key))) + 8 * (l16 & 1);
+  }
+  asm("" : "+v"(k_at), "+v"(v_at));
+
+  float mref = kNone, lsum = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int j = 0; j < DT; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+
+  int slot[UL];
+  lookup(0, slot);
+  fetch(slot);
+  if (steps > 1) lookup(1, slot);
+  put(0);
+  for (int t = 0; t < steps; ++t) {
+    lds_barrier();                                         // step t is in place, step t - 1 has been read
+    if (t + 1 < steps) fetch(slot);
+    if (t + 2 < steps) lookup(t + 2, slot);
+    if (active) {
+      const lds_char* dk = (const lds_char*)lds + kBytes * (t & 1);
+      const lds_char* dv = (const lds_char*)lds + kBytes * (2 + (t & 1));
+      // Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
+      f32x16 s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, read16(dk + (k_at ^ (32 * i)) + 16 * 32 * U * kb)), qf[i], s[kb], 0, 0, 0);
+      float mx = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+      if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
+        const float top = fmaxf(mx, shfl_xor(mx, 32)) * A.c;
+        const float mn = top > mref + kTau ? top : mref;   // rows that stay get a factor of exactly 1
+        const float alpha = fexp2(mref - mn);
+        lsum = lsum * alpha;
+        mref = mn;
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
+      }
+      u32x4 p[4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float a = fexp2(__builtin_fmaf(s[i / 8][2 * i % 16], A.c, -mref));
+        const float b = fexp2(__builtin_fmaf(s[i / 8][2 * i % 16 + 1], A.c, -mref));
+        p[i / 4][i % 4] = pack_bf16x2(a, b);
+        lsum = dot2(p[i / 4][i % 4], lsum);
+      }
+      // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
+      // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+          s16x4 h[2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) h[z] = tr_read(dv + (v_at ^ (64 * j)) + 16 * U * (16 * i + 8 * z));
+          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7)),
+              __builtin_bit_cast(bf16x8, p[i]), acc[j], 0, 0, 0);
+        }
+    }
+    if (t + 1 < steps) put(t + 1);
+  }
+  // A page that is none spoils every row that reads it.
+  int* flag = reinterpret_cast<int*>(lds);
+  lds_barrier();
+  if (threadIdx.x == 0) *flag = 0;
+  lds_barrier();
+  if (bad) *flag = 1;
+  lds_barrier();
+  lsum = lsum + shfl_xor(lsum, 32);
+  if (!stored) return;
+  if (*flag) lsum = __builtin_nanf("");
+  const int64_t at = bh * A.smax + split;
+#pragma unroll
+  for (int j = 0; j < DT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<f32x4*>(A.po + at * D + 32 * j + 8 * e + 4 * half) =
+          f32x4{acc[j][4 * e], acc[j][4 * e + 1], acc[j][4 * e + 2], acc[j][4 * e + 3]};
+  if (half == 0) A.pml[at] = f32x2{mref, lsum};
+}
+
+template <int D, int BITS>
+__global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(PagedArgs A) {
+  __shared__ __align__(16) char stage[kWaves][kTile * D * 2];
+  __shared__ float sm[kWaves][16], sl[kWaves][16];
+  __shared__ int first[kSeqs + 1], length[kSeqs];
+  paged_items<D, BITS, false>(A, blockIdx.x, gridDim.x, stage, sm, sl, first, length, nullptr);
+}
+
+// The first `tiles` workgroups take the shared keys, the rest the sequences' own.
+template <int D, int BITS>
+__global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void shared_attn_kernel(PagedArgs A, int total, int psmax, int tiles) {
+  constexpr int kPrefixBytes = 4 * kKeys * D * 2;
+  __shared__ __align__(16) char lds[sizeof(PagedLds<D, true>) > kPrefixBytes ? sizeof(PagedLds<D, true>) : kPrefixBytes];
+  if ((int)blockIdx.x < tiles) {
+    prefix_tile<D, BITS>(A, total, psmax, blockIdx.x, lds);
+  } else {
+    auto& x = *reinterpret_cast<PagedLds<D, true>*>(lds);
+    paged_items<D, BITS, true>(A, blockIdx.x - tiles, gridDim.x - tiles, x.stage, x.sm, x.sl, x.first, x.length, x.from);
+  }
+}
+
 // One workgroup per (query head, sequence).  Every wave takes the splits' weights, lane s
 // that of split s; then lanes of four columns each sum every (256 / (D / 4))-th split, and
 // those sums are added in order.
-template <int D>
+template <int D, bool SHARED>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
-  constexpr int L = D / 4, P = 256 / L;
-  __shared__ float wt[kMaxSplits];
+  constexpr int L = D / 4, P = 256 / L, kMost = kMaxSplits + (SHARED ? kMaxPrefixSplits : 0);
+  __shared__ float wt[kMost];
   __shared__ __align__(16) f32x4 sums[P][L];
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63;
   const int64_t p = ((int64_t)b * A.HK * A.G + h) * A.smax;
   const f32x2 held = lane < A.smax ? A.pml[p + lane] : f32x2{kNone, 0.f};   // beside the length
   const int n = A.lens[b];
   if (n <= 0 || n > ((int64_t)A.width << A.shift)) return;
-  const int splits = split_count(n);
-  if (splits == 1) return;
+  const int from = shared_keys<SHARED>(A, b, n);
+  const int splits = (from > 0 ? prefix_splits(from) : 0) + split_count(n - from);
+  if (splits == 1 && from == 0) return;
   const f32x2 ml = lane < splits ? held : f32x2{kNone, 0.f};
   const int c = threadIdx.x % L, part = threadIdx.x / L;
-  constexpr int N = (kMaxSplits + P - 1) / P;
+  constexpr int N = (kMost + P - 1) / P;
   f32x4 x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -396,7 +645,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
   const float a = fexp2(ml[0] - m);
   float l = ml[1] * a;
   for (int k = 32; k >= 1; k >>= 1) l = l + __shfl_xor(l, k);
-  if (threadIdx.x < kMaxSplits) wt[threadIdx.x] = a;
+  if (threadIdx.x < kMost) wt[threadIdx.x] = a;
   __syncthreads();
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -415,24 +664,110 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
   }
 }
 
-template <int D>
+template <int D, int BITS, bool SHARED>
 int launch(PagedArgs A, int B, hipStream_t s) {
+  const int psmax = SHARED ? prefix_split_bound(A.longest) : 0;
   for (int b0 = 0; b0 < B; b0 += kSeqs) {
     A.B = B - b0 < kSeqs ? B - b0 : kSeqs;
-    const int64_t items = (int64_t)A.B * A.smax * A.HK;
-    hipLaunchKernelGGL(paged_attn_kernel<D>, dim3((unsigned)(items < kCUs * PagedGeom<D>::kPerCU ? items : kCUs * PagedGeom<D>::kPerCU)), dim3(256), 0, s, A);
-    if (A.smax > 1) hipLaunchKernelGGL(paged_join_kernel<D>, dim3(A.HK * A.G, A.B), dim3(256), 0, s, A);
+    const int64_t items = (int64_t)A.B * (A.smax - psmax) * A.HK, most = kCUs * PagedGeom<D>::kPerCU;
+    const unsigned blocks = (unsigned)(items < most ? items : most);
+    if constexpr (SHARED) {
+      const int tiles = b0 == 0 ? A.n_tiles * A.HK : 0;    // of all sequences
+      hipLaunchKernelGGL((shared_attn_kernel<D, BITS>), dim3(tiles + blocks), dim3(256), 0, s, A, B, psmax, tiles);
+    } else {
+      hipLaunchKernelGGL((paged_attn_kernel<D, BITS>), dim3(blocks), dim3(256), 0, s, A);
+    }
+    if (A.smax > 1) hipLaunchKernelGGL((paged_join_kernel<D, SHARED>), dim3(A.HK * A.G, A.B), dim3(256), 0, s, A);
     A.q += A.B * A.sqb;
     A.out += A.B * A.sob;
     A.table += A.B * A.stb;
     A.lens += A.B;
+    if constexpr (SHARED) A.prefix += A.B;
     A.po += (int64_t)A.B * A.HK * A.G * A.smax * D;
     A.pml += (int64_t)A.B * A.HK * A.G * A.smax;
   }
   return hipGetLastError() == hipSuccess ? RSPX_OK : RSPX_ELAUNCH;
 }
 
+template <int BITS, bool SHARED>
+int launch_for(int D, const PagedArgs& A, int B, hipStream_t s) {
+  switch (D) {
+    case 32: return launch<32, BITS, SHARED>(A, B, s);
+    case 64: return launch<64, BITS, SHARED>(A, B, s);
+    case 128: return launch<128, BITS, SHARED>(A, B, s);
+    default: return launch<256, BITS, SHARED>(A, B, s);
+  }
+}
+
 bool head_dim_ok(int D) { return D == 32 || D == 64 || D == 128 || D == 256; }
+
+int64_t workspace(int B, int H, int D, int page, int width, int psmax) {
+  if (B < 0 || H < 1 || page < 1 || width < 0 || !head_dim_ok(D)) return -1;
+  const int smax = split_bound((int64_t)width * page) + psmax;
+  return smax <= 1 ? 0 : (int64_t)B * H * smax * (D + 2) * 4;
+}
+
+// A pool as the C ABI names it: strides in its elements.
+struct PoolArg {
+  const void* rows;
+  int64_t sh, sn;
+  const void* scales;
+  int64_t ssh, ssn;
+};
+
+int attend(const void* q, int64_t sqb, int64_t sqh, const PoolArg& k, const PoolArg& v, int bits, const int32_t* table,
+           int64_t stb, const int32_t* lens, bool shared, const int32_t* prefix, const int32_t* tiles, int n_tiles, int longest,
+           void* out, int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages, int page, int width, float sm_scale,
+           void* ws, int64_t ws_bytes, void* stream) {
+  if (B < 0 || H < 1 || HK < 1 || H % HK || pages < 1 || page < 1 || (page & (page - 1)) || width < 0) return RSPX_EINVAL;
+  if (!(sm_scale > 0.f) || sm_scale > 3e38f) return RSPX_EINVAL;
+  if ((int64_t)pages * page > INT32_MAX || (int64_t)width * page > INT32_MAX - 4096) return RSPX_EINVAL;
+  if (n_tiles < 0 || longest < 0 || longest > (int64_t)width * page) return RSPX_EINVAL;
+  if (bits != 16 && bits != 8 && bits != 4) return RSPX_EUNSUPPORTED;
+  if (!head_dim_ok(D) || H / HK > 16 || HK > 4096) return RSPX_EUNSUPPORTED;   // items of a launch are counted in 32 bits
+  if ((int64_t)n_tiles * HK > (1 << 23)) return RSPX_EUNSUPPORTED;             // a grid dimension holds 2^32 threads
+  if (B == 0) return RSPX_OK;
+  if (!q || !k.rows || !v.rows || !lens || !out || (width && !table)) return RSPX_EINVAL;
+  if (bits < 16 && (!k.scales || !v.scales)) return RSPX_EINVAL;
+  if (shared && (!prefix || (n_tiles && !tiles))) return RSPX_EINVAL;
+  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  if (reinterpret_cast<uintptr_t>(out) & 1u) return RSPX_EALIGN;
+  const int unit = bits == 16 ? 8 : 16;
+  if (!al(q) || !al(k.rows) || !al(v.rows) || sqb % 8 || sqh % 8 || k.sh % unit || k.sn % unit || v.sh % unit || v.sn % unit)
+    return RSPX_EALIGN;
+  const int psmax = shared ? prefix_split_bound(longest) : 0;
+  const int64_t need = workspace(B, H, D, page, width, psmax);
+  if (need > 0 && (!ws || ws_bytes < need)) return RSPX_EWORKSPACE;
+  if (need > 0 && !al(ws)) return RSPX_EALIGN;
+  const int64_t e = bits == 16 ? 2 : 1;
+  PagedArgs A;
+  A.q = static_cast<const uint16_t*>(q);
+  A.k = static_cast<const char*>(k.rows);
+  A.v = static_cast<const char*>(v.rows);
+  A.ks = static_cast<const uint8_t*>(k.scales);
+  A.vs = static_cast<const uint8_t*>(v.scales);
+  A.table = table;
+  A.lens = lens;
+  A.prefix = prefix, A.tiles = tiles, A.n_tiles = n_tiles, A.longest = longest;
+  A.out = static_cast<uint16_t*>(out);
+  A.po = static_cast<float*>(ws);
+  A.sqb = sqb, A.sqh = sqh, A.stb = stb, A.sob = sob, A.soh = soh;
+  A.skh = k.sh * e, A.skn = k.sn * e, A.svh = v.sh * e, A.svn = v.sn * e;
+  A.sksh = k.ssh, A.sksn = k.ssn, A.svsh = v.ssh, A.svsn = v.ssn;
+  A.HK = HK, A.G = H / HK, A.pages = pages, A.width = width;
+  A.shift = __builtin_ctz((unsigned)page);
+  const int smax = split_bound((int64_t)width * page);
+  A.smax = (smax < 1 ? 1 : smax) + psmax;
+  A.pml = reinterpret_cast<f32x2*>(A.po + (int64_t)B * H * A.smax * D);
+  A.c = sm_scale * 1.44269504088896340736f;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (shared) {
+    if (bits == 16) return launch_for<16, true>(D, A, B, s);
+    return bits == 8 ? launch_for<8, true>(D, A, B, s) : launch_for<4, true>(D, A, B, s);
+  }
+  if (bits == 16) return launch_for<16, false>(D, A, B, s);
+  return bits == 8 ? launch_for<8, false>(D, A, B, s) : launch_for<4, false>(D, A, B, s);
+}
 
 }  // namespace
 
@@ -441,9 +776,7 @@ bool head_dim_ok(int D) { return D == 32 || D == 64 || D == 128 || D == 256; }
 using namespace rspx;
 
 extern "C" int64_t rspx_paged_attn_workspace_bytes(int B, int H, int D, int page, int width) {
-  if (B < 0 || H < 1 || page < 1 || width < 0 || !head_dim_ok(D)) return -1;
-  const int smax = split_bound((int64_t)width * page);
-  return smax <= 1 ? 0 : (int64_t)B * H * smax * (D + 2) * 4;
+  return workspace(B, H, D, page, width, 0);
 }
 
 extern "C" int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn,
@@ -451,38 +784,59 @@ extern "C" int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const vo
                                const int32_t* lens, void* out, int64_t sob, int64_t soh, int B, int H, int HK, int D,
                                int pages, int page, int width, float sm_scale, void* workspace,
                                int64_t workspace_bytes, void* stream) {
-  if (B < 0 || H < 1 || HK < 1 || H % HK || pages < 1 || page < 1 || (page & (page - 1)) || width < 0) return RSPX_EINVAL;
-  if (!(sm_scale > 0.f) || sm_scale > 3e38f) return RSPX_EINVAL;
-  if ((int64_t)pages * page > INT32_MAX || (int64_t)width * page > INT32_MAX - 4096) return RSPX_EINVAL;
-  if (!head_dim_ok(D) || H / HK > 16 || HK > 4096) return RSPX_EUNSUPPORTED;   // items of a launch are counted in 32 bits
-  if (B == 0) return RSPX_OK;
-  if (!q || !kc || !vc || !lens || !out || (width && !table)) return RSPX_EINVAL;
-  auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  if (reinterpret_cast<uintptr_t>(out) & 1u) return RSPX_EALIGN;
-  if (!al(q) || !al(kc) || !al(vc) || sqb % 8 || sqh % 8 || skh % 8 || skn % 8 || svh % 8 || svn % 8) return RSPX_EALIGN;
-  const int64_t need = rspx_paged_attn_workspace_bytes(B, H, D, page, width);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return RSPX_EWORKSPACE;
-  if (need > 0 && !al(workspace)) return RSPX_EALIGN;
-  PagedArgs A;
-  A.q = static_cast<const uint16_t*>(q);
-  A.k = static_cast<const uint16_t*>(kc);
-  A.v = static_cast<const uint16_t*>(vc);
-  A.table = table;
-  A.lens = lens;
-  A.out = static_cast<uint16_t*>(out);
-  A.po = static_cast<float*>(workspace);
-  A.sqb = sqb, A.sqh = sqh, A.skh = skh, A.skn = skn, A.svh = svh, A.svn = svn, A.stb = stb, A.sob = sob, A.soh = soh;
-  A.HK = HK, A.G = H / HK, A.pages = pages, A.width = width;
-  A.shift = __builtin_ctz((unsigned)page);
-  const int smax = split_bound((int64_t)width * page);
-  A.smax = smax < 1 ? 1 : smax;
-  A.pml = reinterpret_cast<f32x2*>(A.po + (int64_t)B * H * A.smax * D);
-  A.c = sm_scale * 1.44269504088896340736f;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (D) {
-    case 32: return launch<32>(A, B, s);
-    case 64: return launch<64>(A, B, s);
-    case 128: return launch<128>(A, B, s);
-    default: return launch<256>(A, B, s);
+  return attend(q, sqb, sqh, PoolArg{kc, skh, skn, nullptr, 0, 0}, PoolArg{vc, svh, svn, nullptr, 0, 0}, RSPX_BF16, table, stb,
+                lens, false, nullptr, nullptr, 0, 0, out, sob, soh, B, H, HK, D, pages, page, width, sm_scale, workspace,
+                workspace_bytes, stream);
+}
+
+extern "C" int rspx_paged_attn_mx(const void* q, int64_t sqb, int64_t sqh, const void* k_codes, int64_t skch, int64_t skcn,
+                                  const void* k_scales, int64_t sksh, int64_t sksn, const void* v_codes, int64_t svch,
+                                  int64_t svcn, const void* v_scales, int64_t svsh, int64_t svsn, const int32_t* table,
+                                  int64_t stb, const int32_t* lens, void* out, int64_t sob, int64_t soh, int B, int H, int HK,
+                                  int D, int pages, int page, int width, float sm_scale, int format, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  if (format == RSPX_BF16) return RSPX_EUNSUPPORTED;   // rspx_paged_attn
+  return attend(q, sqb, sqh, PoolArg{k_codes, skch, skcn, k_scales, sksh, sksn}, PoolArg{v_codes, svch, svcn, v_scales, svsh, svsn},
+                format, table, stb, lens, false, nullptr, nullptr, 0, 0, out, sob, soh, B, H, HK, D, pages, page, width, sm_scale,
+                workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t rspx_shared_plan(const int64_t* members, const int64_t* keys, int n, int group, int32_t* prefix,
+                                    int32_t* tiles) {
+  if (n < 0 || group < 1 || group > 16 || (n > 0 && (!members || !keys))) return RSPX_EINVAL;
+  int64_t b = 0, count = 0;
+  for (int i = 0; i < n; ++i) {
+    if (members[i] < 0 || keys[i] < 0 || members[i] > INT32_MAX || keys[i] > INT32_MAX) return RSPX_EINVAL;
+    // One sequence alone shares nothing; a begun step is left to the sequences themselves.
+    const int p = members[i] < 2 ? 0 : (int)(keys[i] / kKeys * kKeys);
+    if (b + members[i] > INT32_MAX / 16) return RSPX_EINVAL;
+    if (prefix) std::fill(prefix + b, prefix + b + members[i], p);
+    const int per = prefix_split_keys(p), rows = (int)members[i] * group;
+    // The row blocks of a split beside one another: they read the same keys.
+    for (int64_t k = 0, split = 0; k < p; k += per, ++split)
+      for (int r = 0; r < rows; r += kPrefixRows, ++count)
+        if (tiles) {
+          int32_t* t = tiles + count * kTileInts;
+          t[0] = (int32_t)b, t[1] = std::min(rows - r, kPrefixRows), t[2] = r, t[3] = (int32_t)k;
+          t[4] = (int32_t)std::min<int64_t>(k + per, p), t[5] = (int32_t)split, t[6] = t[7] = 0;
+        }
+    b += members[i];
   }
+  return count;
+}
+
+extern "C" int64_t rspx_paged_attn_shared_workspace_bytes(int B, int H, int D, int page, int width, int longest) {
+  return longest < 0 ? -1 : workspace(B, H, D, page, width, prefix_split_bound(longest));
+}
+
+extern "C" int rspx_paged_attn_shared(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn,
+                                      const void* k_scales, int64_t sksh, int64_t sksn, const void* vc, int64_t svh, int64_t svn,
+                                      const void* v_scales, int64_t svsh, int64_t svsn, const int32_t* table, int64_t stb,
+                                      const int32_t* lens, const int32_t* prefix, const int32_t* tiles, int n_tiles, int longest,
+                                      void* out, int64_t sob, int64_t soh, int B, int H, int HK, int D, int pages, int page,
+                                      int width, float sm_scale, int format, void* workspace, int64_t workspace_bytes,
+                                      void* stream) {
+  return attend(q, sqb, sqh, PoolArg{kc, skh, skn, k_scales, sksh, sksn}, PoolArg{vc, svh, svn, v_scales, svsh, svsn}, format,
+                table, stb, lens, true, prefix, tiles, n_tiles, longest, out, sob, soh, B, H, HK, D, pages, page, width, sm_scale,
+                workspace, workspace_bytes, stream);
 }

@@ -39,23 +39,16 @@
 // the middle of a step, operands of the next one requested before its end (0 to 2 %).
 #include <algorithm>
 
-#include "common.h"
+#include "keys64.h"
 #include "respect_amd.h"
 
 namespace rspx {
 
 namespace {
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kKeys = 64;            // keys of a step
 constexpr int kRows = 32;            // rows of a wave
-constexpr float kTau = 8.0f;         // log2 headroom before the reference maximum moves
-constexpr float kNone = -1e30f;      // reference maximum before the first key
 
 constexpr int kGroups = 1 << 23;     // workgroups of a launch: a grid dimension holds 2^32 threads
 constexpr int kEdges = 8;            // more than the steps that some row of a tile sees in part
@@ -77,49 +70,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint32_
 }
 __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t r, int voff, lds_char* dst) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, 0, 0, 0);
-}
-__device__ __forceinline__ s16x4 tr_read(const lds_char* __restrict__ p) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-}
-
-typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
-// c + both bf16 of x, rounded to nearest (measured: 63 of 64 sums as one rounding, none by more
-// than 0.52 of a step).
-__device__ __forceinline__ float dot2(uint32_t x, float c) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b16x2, x), __builtin_bit_cast(b16x2, 0x3f803f80u), c, false);
-}
-// LDS reads of what is in place (its loads waited for, the barrier passed).  __restrict__:
-// without alias information the compiler waits for every load to LDS in flight, the next
-// steps' included, ahead of the first read.
-__device__ __forceinline__ u32x4 read16(const lds_char* __restrict__ p) {
-  return *(const __attribute__((address_space(3))) u32x4*)p;
-}
-
-// A barrier that does not wait for the loads in flight.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// 16-byte unit swizzles of a staged row of U units, 256 bytes of banks: sixteen consecutive
-// keys' units of one column lie in different banks (K); so do four keys' four units, and
-// eight keys' two (V).
-template <int D>
-__device__ __forceinline__ int kswizzle(int key) {
-  constexpr int U = D / 8;
-  if constexpr (U >= 16) return key % 16;
-  else return (key / (16 / U)) % U;
-}
-template <int D>
-__device__ __forceinline__ int vswizzle(int key) {
-  constexpr int U = D / 8;
-  const int odd = 2 * ((key >> 2) & 1);
-  if constexpr (U >= 16) return 4 * (key % 4) + odd;
-  else if constexpr (U == 8) return 4 * ((key >> 1) & 1) + odd;
-  else return odd;
 }
 
 // HW heads and RW = 4 / HW row blocks of 32 rows per workgroup.

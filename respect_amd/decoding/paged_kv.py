@@ -1,7 +1,8 @@
 """KV cache of many sequences in pages: taken, shared, copied, compacted and given back.
 
 No counterpart in the reference, whose buffer holds one request (kv_buffer.py here).
-Per layer one bf16 pool [HK, pages * page, D] for K and one for V; row j of a sequence is
+Per layer one pool [HK, pages * page, D] for K and one for V, bf16 or in a microscaled format
+of 8 or 4 bits (``kernels.mx``); row j of a sequence is
 pool row ``table[j // page] * page + j % page``.  Who holds which page is kept on the
 host (rspx_pages_*: pages are counted, so that forks share the full ones); the rows move on
 the GPU, all layers and sequences in one launch (rspx_kv_move).  ``paged_attn`` reads the
@@ -17,6 +18,8 @@ import torch
 
 from .. import _lib
 from ..kernels._tensor import as_kernel_input, fits_32_bits
+from ..kernels.mx import BITS, MXRows, read_rows, write_rows
+from ..kernels.paged_attention import SharedPrefix
 
 
 def _p(a: np.ndarray) -> int:
@@ -146,6 +149,16 @@ class PageTable:
         self._call("table", _p(ids), len(ids), width, _p(table), _p(lens))
         return table, lens
 
+    def shared(self, seqs, least: int) -> tuple[list[int], list[int]]:
+        """(members, keys): ``seqs`` cut into groups of consecutive sequences that begin with the
+        same full pages, so that most keys are shared; fewer than ``least`` keys count as none."""
+        ids = self._ids(seqs)
+        members, keys = np.empty(len(ids), np.int64), np.empty(len(ids), np.int64)
+        n = self._lib.rspx_pages_shared(self.handle, _p(ids), len(ids), least, _p(members), _p(keys))
+        if n < 0:
+            self.refuse("shared", n)
+        return members[:n].tolist(), keys[:n].tolist()
+
     def slots(self, seqs, first, count) -> np.ndarray:
         ids = self._ids(seqs)
         lo, n = self._counts(first, len(ids)), self._counts(count, len(ids))
@@ -163,21 +176,40 @@ class PagedKVCache:
     cannot be captured into a graph.  Pages given back are taken again at once: calls that
     still read them have to be on the same stream, or waited for.  A call that is refused
     (``ValueError``; ``RuntimeError`` for too few pages or sequences) or whose copies cannot be
-    enqueued changes nothing.  One thread at a time."""
+    enqueued changes nothing.  One thread at a time.
+
+    ``dtype``: "bf16", or "mxfp8" or "mxfp4" (head_dim a multiple of 32), whose rows take 33 / 64
+    and 17 / 64 of the bytes: ``k[layer]`` and ``v[layer]`` are then ``MXRows``, ``write``
+    quantises, and ``read`` and ``paged_attn`` see the values that the codes stand for."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page: int = 64, device="cuda",
-                 sequences: int = 1024):
+                 sequences: int = 1024, dtype: str = "bf16"):
         if layers < 1 or kv_heads < 1 or head_dim < 8 or head_dim % 8:
             raise ValueError("PagedKVCache: layers and kv_heads >= 1 and head_dim a multiple of 8")
+        if dtype != "bf16" and (dtype not in BITS or head_dim % 32):
+            raise ValueError("PagedKVCache: dtype bf16, mxfp8 or mxfp4, the latter with head_dim a multiple of 32")
         self._t = PageTable(pages, page, sequences)
         self.layers, self.HK, self.D, self.page, self.pages = layers, kv_heads, head_dim, page, pages
+        self.dtype = dtype
         shape = (kv_heads, pages * page, head_dim)
-        self.k = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
-        self.v = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
+
+        def pools():
+            if dtype == "bf16":
+                return [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(layers)]
+            return [MXRows.empty(*shape, dtype, device=device) for _ in range(layers)]
+        self.k, self.v = pools(), pools()
         self.device = self.k[0].device
-        bases = torch.tensor([t.data_ptr() for kv in zip(self.k, self.v) for t in kv], dtype=torch.int64).to(self.device)
         k0 = self.k[0]
-        self._pool = (bases, kv_heads, head_dim, k0.stride(0), k0.stride(1), pages * page)
+        pairs = [t for kv in zip(self.k, self.v) for t in kv]
+        if dtype == "bf16":
+            tensors, strides = pairs, (k0.stride(0), k0.stride(1))
+        else:
+            tensors = [t.codes for t in pairs] + [t.scales for t in pairs]
+            strides = (k0.codes.stride(0), k0.codes.stride(1))
+        bases = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64).to(self.device)
+        self._pool = (bases, kv_heads, head_dim, *strides, pages * page)
+        if dtype != "bf16":
+            self._pool += (k0.bits, k0.scales.stride(0), k0.scales.stride(1))
 
     @property
     def free_pages(self) -> int:
@@ -220,12 +252,17 @@ class PagedKVCache:
         if len(groups) == 1:
             return
         flat = self._upload(groups, moves)
-        bases, HK, D, sh, sn, cap = self._pool
+        bases, HK, D, sh, sn, cap, *scales = self._pool
+        lists = (flat.data_ptr(), len(groups) - 1, flat.data_ptr() + 4 * len(groups), len(moves))
         with torch.cuda.device(self.device):
-            rc = _lib.lib().rspx_kv_move(bases.data_ptr(), bases.numel(), HK, D, sh, sn, cap, flat.data_ptr(),
-                                         len(groups) - 1, flat.data_ptr() + 4 * len(groups), len(moves),
-                                         _lib.stream_ptr(bases.device))
-        _lib.check("rspx_kv_move", rc)
+            stream = _lib.stream_ptr(bases.device)
+            if scales:
+                bits, ssh, ssn = scales
+                rc = _lib.lib().rspx_kv_move_mx(bases.data_ptr(), bases.numel() // 2, HK, D, bits, sh, sn, ssh, ssn, cap,
+                                                *lists, stream)
+            else:
+                rc = _lib.lib().rspx_kv_move(bases.data_ptr(), bases.numel(), HK, D, sh, sn, cap, *lists, stream)
+        _lib.check("rspx_kv_move_mx" if scales else "rspx_kv_move", rc)
 
     # ------------------------------------------------------------------ sequences
 
@@ -301,9 +338,26 @@ class PagedKVCache:
         self._check_capture()
         return self._upload(self._t.slots(seqs, first, count))
 
+    def shared(self, seqs, heads: int, least: int = 256) -> SharedPrefix:
+        """The plan by which ``paged_attn`` and ``Decoder.step_batch`` take the pages that
+        consecutive ones of ``seqs`` begin with in common once, for ``heads`` query heads: forks
+        stand side by side.  Groups that share fewer than ``least`` keys are none.  It holds while
+        the sequences grow, and until one of them is compacted into those pages or freed."""
+        heads = operator.index(heads)
+        if heads < 1 or heads % self.HK:
+            raise ValueError(f"PagedKVCache.shared: {heads} heads over {self.HK} kv heads")
+        return SharedPrefix(*self._t.shared(seqs, least), heads // self.HK, device=self.device)
+
+    def read(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) [T, HK, D] bf16: the pool rows ``slots`` [T] (device int32) of one layer, as
+        attention sees them.  Can be captured."""
+        return read_rows(self.k[layer], self.v[layer], slots)
+
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """k / v [T, HK, D] bf16 of one layer to the pool rows ``slots`` [T] (device int32, as
         ``slots`` gives them; one named twice keeps parts of either row).  Can be captured."""
+        if self.dtype != "bf16":
+            return write_rows(k, v, self.k[layer], self.v[layer], slots)
         T = k.shape[0]
         if tuple(k.shape) != (T, self.HK, self.D) or v.shape != k.shape or tuple(slots.shape) != (T,):
             raise ValueError(f"PagedKVCache: k and v must be [T, {self.HK}, {self.D}], slots [T]")
