@@ -34,8 +34,9 @@ so a token verified inside a trie gets the same logits and KV bits as when it
 is decoded alone -- the property the reference's verification relies on
 (respect/decoding/verify.py:12-46, respect/decoding/sequential.py:17-42).
 
-``prefill_batch`` and ``step_batch`` run the same layers for several sequences at once
-over a PagedKVCache, with rspx_prompt_attn and rspx_paged_attn as the attention.
+``prefill_batch``, ``append_batch`` and ``step_batch`` run the same layers for several sequences
+at once over a PagedKVCache, with rspx_prompt_attn and rspx_paged_attn (or, over rows of 8 and 4
+bits and beginnings that sequences share, its other forms) as the attention.
 """
 from __future__ import annotations
 
@@ -350,9 +351,10 @@ class Decoder:
         """New sequences of the PagedKVCache ``cache`` holding ``prompts`` (1-D token tensors on the
         GPU, none empty), all in one pass.  Returns (sequences, logits [B, V] of each prompt's
         last token).  A prompt's results do not depend on the others; its attention runs in
-        ``prompt_attn``'s order, so its bits are not those of ``prefill``.  The pass takes scratch
-        in proportion to all tokens (98 KB each at the 8B sizes), which goes back to torch with
-        its end."""
+        ``prompt_attn``'s order, so its bits are not those of ``prefill``.  Over a cache of few bits
+        the prompt's own attention sees K and V as they are before they are quantised.  The pass
+        takes scratch in proportion to all tokens (98 KB each at the 8B sizes), which goes back to
+        torch with its end."""
         self._check_paged(cache)
         prompts = list(prompts)
         rows = [int(p.shape[0]) for p in prompts]
@@ -377,21 +379,67 @@ class Decoder:
             scratch = _CallScratch(dev)
             y = self._stack(ids, torch.arange(T, dtype=torch.int32, device=dev), positions, _reach(max(rows)),
                             lambda li: (k, v, T), attend, scratch)
-            # the last rows of the tiled rows (RSPX_TILED): elements 32 b + 8 g + e at [b, g, e]
-            m = torch.tensor(rows, device=dev).cumsum(0) - 1
-            last = y.view(-1, cfg.hidden // 32, 4, 4, 16, 8)[m // 64, :, m % 64 // 16, :, m % 16].reshape(len(rows), -1)
-            return seqs, self._linear(last.data_ptr(), last.stride(0), len(rows), self.t_lm_head, out_dtype=torch.float32,
-                                      scratch=scratch)
+            return seqs, self._last_logits(y, rows, scratch)
         except BaseException:
             cache.free(seqs)
             raise
 
+    def _last_logits(self, y, rows: list[int], scratch) -> torch.Tensor:
+        """Logits [B, V] of the last of each ``rows[s]`` consecutive ones of the tiled rows y (RSPX_TILED):
+        elements 32 b + 8 g + e at [b, g, e]."""
+        m = torch.tensor(rows, device=self.device).cumsum(0) - 1
+        last = y.view(-1, self.cfg.hidden // 32, 4, 4, 16, 8)[m // 64, :, m % 64 // 16, :, m % 16].reshape(len(rows), -1)
+        return self._linear(last.data_ptr(), last.stride(0), len(rows), self.t_lm_head, out_dtype=torch.float32, scratch=scratch)
+
     @torch.no_grad()
-    def step_batch(self, ids: torch.Tensor, cache, seqs) -> torch.Tensor:
+    def append_batch(self, prompts, cache, seqs) -> torch.Tensor:
+        """Further tokens ``prompts[i]`` (1-D on the GPU, none empty) of each of the different sequences
+        ``seqs`` of ``cache``, all in one pass: the next turn of conversations, the questions about a
+        document that was forked.  Returns logits [B, V] of each one's last token.  Attention reads
+        the sequences' rows back from the cache (``cache.read``), the new ones among them, and runs
+        as in ``prefill_batch``.  A sequence's results do not depend on the others.  A pass that
+        fails leaves the sequences and the free pages as they were."""
+        self._check_paged(cache)
+        prompts, seqs = list(prompts), list(seqs)
+        rows = [int(p.shape[0]) for p in prompts]
+        if not rows or min(rows) < 1 or len(seqs) != len(rows) or len(set(seqs)) != len(seqs):
+            raise ValueError("append_batch: one prompt for each of the different sequences, at least one, none empty")
+        cache.extend(seqs, rows)
+        try:
+            return self._append_batch(prompts, cache, seqs, rows, [cache.length(s) for s in seqs])
+        except BaseException:
+            cache._t.undo()   # the extension: nothing else has changed the books since
+            raise
+
+    def _append_batch(self, prompts, cache, seqs, rows: list[int], n: list[int]) -> torch.Tensor:
+        """append_batch for sequences that have been extended to ``n`` rows."""
+        cfg, dev, T = self.cfg, self.device, sum(rows)
+        plan = PackedPrompts(rows, n, device=dev)
+        ids = torch.cat(prompts)
+        positions = torch.cat([torch.arange(m - r, m, device=dev) for r, m in zip(rows, n)])
+        slots = cache.slots(seqs, [m - r for r, m in zip(rows, n)], rows)
+        every = cache.slots(seqs, 0, n)
+        k, v = torch.empty((2, cfg.kv_heads, T, cfg.head_dim), dtype=torch.bfloat16, device=dev)
+        att = torch.empty((T, cfg.heads, cfg.head_dim), dtype=torch.bfloat16, device=dev)
+
+        def attend(li, qo):
+            cache.write(li, k.transpose(0, 1), v.transpose(0, 1), slots)
+            prompt_attn(qo, *cache.read(li, every), plan, self.sm_scale, out=att)
+            return att.data_ptr(), cfg.heads * cfg.head_dim
+
+        scratch = _CallScratch(dev)
+        y = self._stack(ids, torch.arange(T, dtype=torch.int32, device=dev), positions, _reach(max(n)), lambda li: (k, v, T),
+                        attend, scratch)
+        return self._last_logits(y, rows, scratch)
+
+    @torch.no_grad()
+    def step_batch(self, ids: torch.Tensor, cache, seqs, shared=None) -> torch.Tensor:
         """One token (``ids`` [B] on the GPU) of each of the sequences ``seqs`` of the PagedKVCache
         ``cache``, appended to them.  Returns fp32 logits [B, V].  A sequence's results do not
-        depend on the others.  A step that fails leaves the sequences and the free pages as
-        they were."""
+        depend on the others.  ``shared``: ``cache.shared(seqs, heads)``, made once for these
+        sequences in this order and used for all their steps: rows that they begin with alike are
+        then read once.  A step that fails leaves the sequences and the free pages as they
+        were."""
         self._check_paged(cache)
         seqs = list(seqs)
         if tuple(ids.shape) != (len(seqs),) or not seqs:
@@ -399,25 +447,31 @@ class Decoder:
         cache.extend(seqs, 1)
         n = [cache.length(s) for s in seqs]
         try:
-            return self._step_batch(ids, cache, seqs, n)
+            return self._step_batch(ids, cache, seqs, n, shared)
         except BaseException:
             cache._t.undo()   # the extension: nothing else has changed the books since
             raise
 
-    def _step_batch(self, ids, cache, seqs, n: list[int]) -> torch.Tensor:
+    def _step_batch(self, ids, cache, seqs, n: list[int], shared) -> torch.Tensor:
         """step_batch for sequences that have been extended to ``n`` rows."""
         cfg, B = self.cfg, len(seqs)
         slots = cache.slots(seqs, [m - 1 for m in n], 1)
         table, lens = cache.tables(seqs)
         att = torch.empty((B, cfg.heads, cfg.head_dim), dtype=torch.bfloat16, device=self.device)
+        if cache.dtype == "bf16":
+            into, kv = slots, lambda li: (cache.k[li], cache.v[li], cache.pages * cache.page)
+        else:   # the new rows as bf16, to be quantised from there
+            k, v = torch.empty((2, cfg.kv_heads, B, cfg.head_dim), dtype=torch.bfloat16, device=self.device)
+            into, kv = torch.arange(B, dtype=torch.int32, device=self.device), lambda li: (k, v, B)
 
         def attend(li, qo):
-            paged_attn(qo, cache.k[li], cache.v[li], table, lens, cache.page, self.sm_scale, out=att)
+            if cache.dtype != "bf16":
+                cache.write(li, k.transpose(0, 1), v.transpose(0, 1), slots)
+            paged_attn(qo, cache.k[li], cache.v[li], table, lens, cache.page, self.sm_scale, out=att, shared=shared)
             return att.data_ptr(), cfg.heads * cfg.head_dim
 
         scratch = _CallScratch(self.device)
-        y = self._stack(ids, slots, lens - 1, _reach(max(n)), lambda li: (cache.k[li], cache.v[li], cache.pages * cache.page),
-                        attend, scratch)
+        y = self._stack(ids, into, lens - 1, _reach(max(n)), kv, attend, scratch)
         return self._linear(y.data_ptr(), _lib.RSPX_TILED, B, self.t_lm_head, out_dtype=torch.float32, scratch=scratch)
 
     def _check_paged(self, cache) -> None:
