@@ -555,7 +555,7 @@ int rspx_paged_attn_mx(const void* q, int64_t sqb, int64_t sqh, const void* k_co
                        int page, int width, float sm_scale, int format, void* workspace, int64_t workspace_bytes,
                        void* stream);
 int64_t rspx_shared_plan(const int64_t* members, const int64_t* keys, int n, int group, int32_t* prefix, int32_t* tiles);
-int64_t rspx_paged_attn_shared_workspace_bytes(int B, int H, int D, int page, int width, int longest);
+int64_t rspx_paged_attn_shared_workspace_bytes(int B, int H, int D, int page, int width, int longest, int format);
 int rspx_paged_attn_shared(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn,
                            const void* k_scales, int64_t sksh, int64_t sksn, const void* vc, int64_t svh, int64_t svn,
                            const void* v_scales, int64_t svsh, int64_t svsn, const int32_t* table, int64_t stb,

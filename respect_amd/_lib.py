@@ -98,7 +98,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64,   # q; k, v codes and scales
         _c_p, _i64, _c_p, _c_p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _c_p, _i64, _c_p]),
     "rspx_shared_plan": (_i64, [_c_p, _c_p, _i32, _i32, _c_p, _c_p]),
-    "rspx_paged_attn_shared_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "rspx_paged_attn_shared_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "rspx_paged_attn_shared": (_i32, [
         _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _i64,   # q; k, v rows and scales
         _c_p, _i64, _c_p, _c_p, _c_p, _i32, _i32, _c_p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,

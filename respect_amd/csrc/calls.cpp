@@ -527,7 +527,7 @@ PyObject* paged_attn_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
       NOT_TAKEN;
   }
   const int64_t need = std::max<int64_t>(
-      0, rspx_paged_attn_shared_workspace_bytes((int)B, (int)H, (int)D, (int)page, (int)width, (int)longest));
+      0, rspx_paged_attn_shared_workspace_bytes((int)B, (int)H, (int)D, (int)page, (int)width, (int)longest, (int)bits));
   const c10::DeviceGuard guard(q->device());
   Tensor y = empty_like_of(*q, {B, H, D}), ws;
   if (need) ws = empty_like_of(*q, {need}, at::kByte);

@@ -17,6 +17,24 @@ constexpr int kLeastScale = 10;      // 2^-117: e4m3's smallest code then stands
 
 __device__ __forceinline__ float mx_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
+// The scales of up to 128 elements as a word, the first ones in its low byte; any alignment.
+template <int D>
+__device__ __forceinline__ uint32_t load_scales(const uint8_t* p) {
+  if constexpr (D >= 128) {
+    uint32_t w;
+    __builtin_memcpy(&w, p, 4);
+    return w;
+  } else if constexpr (D == 64) {
+    uint16_t w;
+    __builtin_memcpy(&w, p, 2);
+    return w;
+  } else {
+    return *p;
+  }
+}
+// Scale i of a row, from the word that holds it.
+__device__ __forceinline__ float scale_in(uint32_t w, int i) { return mx_scale(__builtin_amdgcn_ubfe(w, 8 * (i & 3), 8)); }
+
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 // Non-template wrappers: the host pass rejects these builtins inside templates.

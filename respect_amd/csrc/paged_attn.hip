@@ -44,39 +44,51 @@ namespace {
 constexpr int kTile = 32;            // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kSplitKeys = 256;      // the shortest split
-constexpr int kMaxSplits = 32;       // a longer cache gets longer splits
+// A longer cache gets longer splits.  Rows of few bits are bound by the waves that take them
+// before they are by their bytes: twice the splits (131072 keys in 4 bits: SPLIT64).
+constexpr int most_splits(int bits) { return bits < 16 ? 64 : 32; }
 constexpr int kSeqs = 1024;          // sequences of a launch
 constexpr int kCUs = 256;
 constexpr float kTiny = 1.17549435e-38f;   // the smallest normal number
 
-// Shared beginnings: whole steps of kKeys keys, in splits of their own.
-constexpr int kPrefixSplitKeys = 256;
-constexpr int kMaxPrefixSplits = 16;
+// Shared beginnings: multiples of kKeys keys, in splits of their own.
+constexpr int kMaxPrefixSplits = 64;
 constexpr int kPrefixRows = 32 * kWaves;   // rows (sequences by heads of a group) of a workgroup
-constexpr int kTileInts = 8;               // first sequence, rows, first row, first key, end, split
+constexpr int kTileInts = 8;               // first sequence, rows, first row, first split, splits, keys
 
 // Keys per split of a sequence of n keys: a multiple of kSplitKeys.
+template <int BITS>
 __host__ __device__ __forceinline__ int split_keys(int n) {
-  const unsigned per = ((unsigned)n + kMaxSplits - 1) / kMaxSplits;
+  constexpr unsigned kMost = most_splits(BITS);
+  const unsigned per = ((unsigned)n + kMost - 1) / kMost;
   return per <= kSplitKeys ? kSplitKeys : (int)((per + kSplitKeys - 1) / kSplitKeys * kSplitKeys);
 }
+template <int BITS>
 __host__ __device__ __forceinline__ int split_count(int n) {
-  const unsigned k = (unsigned)split_keys(n);
+  const unsigned k = (unsigned)split_keys<BITS>(n);
   return (int)(((unsigned)n + k - 1) / k);
 }
 // The most splits that any length up to n gives.
-__host__ __forceinline__ int split_bound(int64_t n) { return n >= (int64_t)kSplitKeys * kMaxSplits ? kMaxSplits : split_count((int)n); }
+__host__ __forceinline__ int split_bound(int64_t n, int bits) {
+  const int most = most_splits(bits);
+  return n >= (int64_t)kSplitKeys * most ? most : (int)((n + kSplitKeys - 1) / kSplitKeys);
+}
 
-// The same for n shared keys, a multiple of kKeys.
+// The same for n shared keys: 32 splits of 128 to 512 keys, past that 64.
 __host__ __device__ __forceinline__ int prefix_split_keys(int n) {
-  const unsigned per = ((unsigned)n + kMaxPrefixSplits - 1) / kMaxPrefixSplits;
-  return per <= kPrefixSplitKeys ? kPrefixSplitKeys : (int)((per + kKeys - 1) / kKeys * kKeys);
+  auto parts = [&](unsigned m) { return ((unsigned)n + m * kKeys - 1) / (m * kKeys) * kKeys; };
+  const unsigned per = parts(32);
+  return per <= 128 ? 128 : per <= 512 ? (int)per : parts(64) <= 512 ? 512 : (int)parts(64);
 }
 __host__ __device__ __forceinline__ int prefix_splits(int n) {
   const unsigned k = (unsigned)prefix_split_keys(n);
   return (int)(((unsigned)n + k - 1) / k);
 }
-__host__ __forceinline__ int prefix_split_bound(int n) { return n >= kPrefixSplitKeys * kMaxPrefixSplits ? kMaxPrefixSplits : prefix_splits(n); }
+// The most splits that any n up to this one gives.
+__host__ __forceinline__ int prefix_split_bound(int n) {
+  const unsigned some = ((unsigned)n + 127) / 128, many = ((unsigned)n + 511) / 512;
+  return (int)std::min<unsigned>(kMaxPrefixSplits, std::max<unsigned>(std::min<unsigned>(some, 32), many));
+}
 
 struct PagedArgs {
   const uint16_t* q;
@@ -104,7 +116,7 @@ __device__ __forceinline__ int shared_keys(const PagedArgs& A, int b, int n) {
 // first[b]: the splits of sequences before b (one for a sequence without any, whose rows
 // are written too), length[b]: lens[b]; returns the number of splits.  All 256 threads call it.
 // The keys that from[b] says are shared have splits elsewhere.
-template <bool SHARED>
+template <int BITS, bool SHARED>
 __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* first, int* length, int* from) {
   const int* lens = A.lens;
   const int B = A.B;
@@ -118,10 +130,10 @@ __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* 
     if (b < B) {
       const int n = lens[b];
       length[b] = n;
-      cnt[i] = n <= 0 || n > cap ? 1 : split_count(n);
+      cnt[i] = n <= 0 || n > cap ? 1 : split_count<BITS>(n);
       if constexpr (SHARED) {
         const int p = from[b] = shared_keys<true>(A, b, n);
-        if (p > 0) cnt[i] = split_count(n - p);
+        if (p > 0) cnt[i] = split_count<BITS>(n - p);
       }
     }
     sum += cnt[i];
@@ -147,15 +159,14 @@ __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* 
   return __builtin_amdgcn_readfirstlane(first[kSeqs]);
 }
 
-// The sequence that split number i belongs to.
-__device__ __forceinline__ int find_seq(const int* first, int B, int i) {
-  int lo = 0, hi = B;                                      // first[lo] <= i < first[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (first[mid] <= i) lo = mid;
-    else hi = mid;
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
+// The sequence that split number i belongs to: the last one with first[b] <= i, by the counts of
+// those up to i among every 16th and then among 16 (two reads of LDS one after the other, where a
+// binary search makes ten).
+__device__ __forceinline__ int find_seq(const int* first, int i) {
+  static_assert(kSeqs == 64 * 16, "a lane holds 16");
+  const int lane = threadIdx.x & 63;
+  const int b = 16 * (__builtin_popcountll(__builtin_amdgcn_ballot_w64(first[16 * lane] <= i)) - 1);
+  return b + __builtin_popcountll(__builtin_amdgcn_ballot_w64(first[b + (lane & 15)] <= i)) / 4 - 1;
 }
 
 // 16-byte unit swizzle of a staged V row: four consecutive keys' pairs of units lie in
@@ -167,15 +178,24 @@ __device__ __forceinline__ int tile_vswizzle(int key) {
   else return 2 * ((key / (16 / U)) % (U / 2));
 }
 
+// The byte offset of a row; the products of 64 bits are for strides of 4 GB and more, which the
+// newer calls refuse.
+template <bool WIDE>
+__device__ __forceinline__ int64_t row_at(int row, int64_t stride) {
+  return WIDE ? row * stride : (int64_t)((uint64_t)(uint32_t)row * (uint32_t)stride);
+}
+
 __device__ __forceinline__ float max4(float x) { return fmaxf(fmaxf(x, shfl_xor(x, 16)), fmaxf(shfl_xor(x, 32), shfl_xor(x, 48))); }
 __device__ __forceinline__ float sum4(float x) {
   x = x + shfl_xor(x, 16);
   return x + shfl_xor(x, 32);
 }
 
-template <int D>
+// Workgroups resident on a CU, by registers and LDS.
+template <int D, int BITS>
 struct PagedGeom {
-  static constexpr int kPerCU = D >= 256 ? 1 : D >= 128 ? 2 : D >= 64 ? 3 : 4;   // resident workgroups
+  static constexpr int kPerCU = BITS < 16 ? (D >= 256 ? (BITS == 8 ? 1 : 2) : D >= 128 ? 3 : 4) : D >= 256 ? 1 : D >= 128 ? 2 : D >= 64 ? 3 : 4;
+  static constexpr int kSharedPerCU = D >= 256 ? 1 : D >= 128 ? 2 : 3;
 };
 
 // One split of one sequence for one kv head.
@@ -205,13 +225,13 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, c16 = lane & 15, r4 = lane >> 4;
   const int64_t cap = (int64_t)A.width << A.shift;
-  const int items = list_items<SHARED>(A, cap, first, length, from) * A.HK;
+  const int items = list_items<BITS, SHARED>(A, cap, first, length, from) * A.HK;
   if (block >= items) return;
 
   auto decode = [&](int i) {
     Item x;
     x.g = i % A.HK;
-    x.b = find_seq(first, A.B, i / A.HK);
+    x.b = find_seq(first, i / A.HK);
     x.split = i / A.HK - __builtin_amdgcn_readfirstlane(first[x.b]);
     x.n = __builtin_amdgcn_readfirstlane(length[x.b]);
     x.splits = x.t = x.tend = x.from = 0;
@@ -220,42 +240,58 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
         x.from = __builtin_amdgcn_readfirstlane(from[x.b]);
         x.n -= x.from;
       }
-      const int per = split_keys(x.n);
-      x.splits = split_count(x.n);
+      const int per = split_keys<BITS>(x.n);
+      x.splits = split_count<BITS>(x.n);
       x.t = x.split * (per / kTile) + w;
       x.tend = ((int)min((int64_t)x.n, (int64_t)(x.split + 1) * per) + kTile - 1) / kTile;
     }
     return x;
   };
-  // The pool slot of key 32 t + lane % 32; keys past the end give the last one's.  -1: the
-  // page is none, and nothing of it is read.
-  auto slot_of = [&](const Item& x, int t) {
-    const int key = x.from + min(t * kTile + (lane & 31), x.n - 1);
-    const int p = A.table[x.b * A.stb + (key >> A.shift)];
-    return (unsigned)p < (unsigned)A.pages ? (p << A.shift) + (key & ((1 << A.shift) - 1)) : -1;
+  // Key 32 t + lane % 32 (past the end: the last one): its page as the table has it, and its pool
+  // slot, once that has come.  -1: the page is none, and nothing of it is read; or the wave has no
+  // tile t.  No branch around the load: past one, all loads in flight would be waited for.
+  auto page_of = [&](const Item& x, int t) {
+    const bool on = t < x.tend;
+    const int* row = on ? A.table + x.b * A.stb : A.lens;
+    return row[on ? (x.from + min(t * kTile + (lane & 31), x.n - 1)) >> A.shift : 0];
   };
+  auto slot_of = [&](const Item& x, int t, int p) {
+    const int key = x.from + min(t * kTile + (lane & 31), x.n - 1);
+    return t < x.tend && (unsigned)p < (unsigned)A.pages ? (p << A.shift) + (key & ((1 << A.shift) - 1)) : -1;
+  };
+  auto at = [&](int row, int64_t stride) { return row_at<BITS == 16 && !SHARED>(row, stride); };
   Words<KW> kf[2][KN];
   Words<VW> vf[VL];
-  uint32_t kscale[2][KN], vscale[VL];
-  auto load = [&](const Item& x, int slot) {
+  // Scales by the word (of a shorter row: all of them).  As bytes the compiler extends them where
+  // paths meet, behind a wait for loads that have just begun.
+  constexpr int KS = D >= 128 ? D / 128 : 1;
+  uint32_t kscale[2][KS], vscale[VL];
+  const int kfirst = KE * r4 / kGroup, vfirst = VE * (lane % VU) / kGroup;
+  auto kscale_of = [&](int j, int i) {                     // of load i: KE elements from 4 KE i + KE r4 on
+    return BITS < 16 ? scale_in(kscale[j][D >= 128 ? KE * i / kGroup : 0], kfirst + 4 * KE * i / kGroup) : 0.f;
+  };
+  auto vscale_of = [&](int j) { return BITS < 16 ? scale_in(vscale[j], vfirst) : 0.f; };
+  auto load = [&](int g, int slot) {
     slot = max(slot, 0);
-    const char* kb = A.k + x.g * A.skh;
-    const char* vb = A.v + x.g * A.svh;
+    const char* kb = A.k + g * A.skh;
+    const char* vb = A.v + g * A.svh;
+    const uint8_t *ks = A.ks + g * A.sksh, *vs = A.vs + g * A.svsh;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = shfl_idx_i(slot, 16 * j + c16);
-      const char* p = kb + row * A.skn + KW * r4;
+      const char* p = kb + at(row, A.skn) + KW * r4;
 #pragma unroll
-      for (int i = 0; i < KN; ++i) {
-        kf[j][i] = load_words<KW>(p + 4 * KW * i);
-        if constexpr (BITS < 16) kscale[j][i] = A.ks[x.g * A.sksh + row * A.sksn + KE * (4 * i + r4) / kGroup];
+      for (int i = 0; i < KN; ++i) kf[j][i] = load_words<KW>(p + 4 * KW * i);
+      if constexpr (BITS < 16) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) kscale[j][i] = load_scales<D>(ks + at(row, A.sksn) + 4 * i);
       }
     }
 #pragma unroll
     for (int j = 0; j < VL; ++j) {
       const int u = 64 * j + lane, row = shfl_idx_i(slot, u / VU);
-      vf[j] = load_words<VW>(vb + row * A.svn + VW * (u % VU));
-      if constexpr (BITS < 16) vscale[j] = A.vs[x.g * A.svsh + row * A.svsn + VE * (u % VU) / kGroup];
+      vf[j] = load_words<VW>(vb + at(row, A.svn) + VW * (u % VU));
+      if constexpr (BITS < 16) vscale[j] = load_scales<D>(vs + at(row, A.svsn) + vfirst / 4 * 4);
     }
   };
   // B operand of the scores: lane (c16, r4) holds head c16, the head_dims of the lane's keys.
@@ -272,18 +308,17 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 
   lds_char* st = (lds_char*)stage[w];
   Item cur = decode(block);
-  int slot = -1;                                           // of the tile in kf and vf
-  if (cur.t < cur.tend) {
-    slot = slot_of(cur, cur.t);
-    load_q(cur);
-    load(cur, slot);
-  }
+  const int page = page_of(cur, cur.t);
+  load_q(cur);
+  int slot = slot_of(cur, cur.t, page);                    // of the tile in kf and vf
+  load(cur.g, slot);
   for (int item = block;;) {
     const int after = item + blocks;
     Item nxt = cur;
     nxt.t = nxt.tend = 0;
     if (after < items) nxt = decode(after);
-    const int nslot = nxt.t < nxt.tend ? slot_of(nxt, nxt.t) : -1;
+    const int npage = page_of(nxt, nxt.t);
+    int ahead = page_of(cur, cur.t + kWaves);              // the page of this item's next tile
     uint16_t* orow = A.out + cur.b * A.sob + (int64_t)cur.g * A.G * A.soh;
 
     float mref = kNone, lsum = 0.f;
@@ -291,7 +326,10 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 #pragma unroll
     for (int j = 0; j < DT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     bool bad = cur.t < cur.tend && slot < 0;
-    int ahead = cur.t + kWaves < cur.tend ? slot_of(cur, cur.t + kWaves) : -1;
+    if (cur.t >= cur.tend) {
+      slot = slot_of(nxt, nxt.t, npage);
+      load(nxt.g, slot);
+    }
     for (int t = cur.t; t < cur.tend; t += kWaves) {
       f32x4 s[2];
 #pragma unroll
@@ -300,13 +338,13 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
           s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8, eight<BITS>(kf[j][i / KF], i % KF, mx_scale(BITS < 16 ? kscale[j][i / KF] : 0))), qf[i], s[j], 0, 0, 0);
+              __builtin_bit_cast(bf16x8, eight<BITS>(kf[j][i / KF], i % KF, kscale_of(j, i / KF))), qf[i], s[j], 0, 0, 0);
       }
       const int left = cur.n - t * kTile;                  // keys of the tile that exist
       if (left < kTile) {   // the repeated last row: its p of 0 times inf would be NaN
 #pragma unroll
         for (int j = 0; j < VL; ++j)
-          if ((64 * j + lane) / VU >= left) vf[j] = Words<VW>{}, vscale[j] = kLeastScale;
+          if ((64 * j + lane) / VU >= left) vf[j] = Words<VW>{}, vscale[j] = 0x01010101u * kLeastScale;
       }
       // The stage belongs to this wave, whose LDS operations keep their order: the reads of
       // the tile before are done before these writes land.
@@ -316,22 +354,32 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 #pragma unroll
         for (int i = 0; i < VF; ++i)
           *(__attribute__((address_space(3))) u32x4*)(st + 16 * (key * U + ((u % VU * VF + i) ^ tile_vswizzle<D>(key)))) =
-              eight<BITS>(vf[j], i, mx_scale(BITS < 16 ? vscale[j] : 0));
+              eight<BITS>(vf[j], i, vscale_of(j));
       }
-      if (t + kWaves < cur.tend) {
-        bad |= ahead < 0;
-        load(cur, ahead);
-        ahead = t + 2 * kWaves < cur.tend ? slot_of(cur, t + 2 * kWaves) : -1;
-      }
+      // The next tile, of this item or the first of the next one.  Always some loads (row 0's where
+      // there is none): the compiler counts those in flight the same on every path.
+      const bool more = t + kWaves < cur.tend;
+      int other = npage;
+      asm volatile("" : "+v"(other));    // waited for here, not ahead of the loop
+      const int mine = slot_of(cur, t + kWaves, ahead);
+      bad |= more && mine < 0;
+      slot = more ? mine : slot_of(nxt, nxt.t, other);
+      ahead = page_of(cur, t + 2 * kWaves);
+      load(more ? cur.g : nxt.g, slot);
 
       // Lane (c16, r4): head c16, keys 16 j + 4 r4 + e of the tile.
       float x[8], mx = kNegInf;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         x[i] = s[i / 4][i % 4];
-        if (left < kTile && 16 * (i / 4) + 4 * r4 + i % 4 >= left) x[i] = kNegInf;
-        mx = fmaxf(mx, x[i]);
       }
+      if (left < kTile) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (16 * (i / 4) + 4 * r4 + i % 4 >= left) x[i] = kNegInf;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
       if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
         const float top = max4(mx) * A.c;
         const float mn = top > mref + kTau ? top : mref;   // rows that stay get a factor of exactly 1
@@ -366,10 +414,7 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pl, acc[j], 0, 0, 0);
       }
     }
-    if (nxt.t < nxt.tend) {   // on its way while this item's waves are joined
-      load_q(nxt);
-      load(nxt, nslot);
-    }
+    load_q(nxt);              // on its way while this item's waves are joined
     if (cur.splits == 0) {    // no keys: zeros; a length that does not fit: NaN
       for (int i = threadIdx.x; i < A.G * D; i += 256) orow[(i / D) * A.soh + i % D] = cur.n == 0 ? 0 : 0x7fc0;
     } else {
@@ -410,88 +455,89 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
     if (after >= items) break;
     item = after;
     cur = nxt;
-    slot = nslot;
   }
 }
 
-// What a tile says of shared keys: for up to kPrefixRows rows (sequence b0 + r / G, head r % G of
-// kv head g) and keys [key0, end), whole steps, the sums of a split.  Four waves of 32 rows; K and
-// V of a step go through registers, where they become bf16, into one of two slots of LDS while
-// the other one is read.  S^T = K Q^T by v_mfma_f32_32x32x16_bf16 leaves a row's scores in one
-// lane and its neighbour of the other half; the probabilities, rounded to bf16 (half a step each)
-// and summed as rounded, are used in place.  Every row sees all keys: there is no mask.
-template <int D, int BITS>
-__device__ __forceinline__ void prefix_tile(const PagedArgs& A, int total, int psmax, int index, char* lds) {
+// What a tile says of shared keys: up to kPrefixRows rows (sequence b0 + r / G, head r % G of kv
+// head g) and up to 4 / WR splits of the keys they share.  A wave takes 32 rows through one split,
+// 32 keys a step; WR waves of different rows take the same split, and fetch its K and V together.
+// What a wave computes of a row does not depend on WR, nor on the rows beside it.
+//
+// K and V come through registers, PF steps ahead, where they become bf16, into LDS: where waves
+// share a split, into one of two slots while the other one is read, with one barrier a step.
+// S^T = K Q^T by v_mfma_f32_32x32x16_bf16 leaves a row's scores in one lane and its neighbour of
+// the other half; the probabilities, rounded to bf16 (half a step each) and summed as rounded, are
+// used in place.  Every row sees all keys: there is no mask.
+template <int D, int BITS, int WR>
+__device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const int* T, int g, char* lds) {
   constexpr int U = D / 8, NS = D / 16, DT = D / 32;
-  constexpr int RB = D * BITS / 8, W = RB / 4 < 16 ? RB / 4 : 16, UR = RB / W, UL = kKeys * UR / 256;   // loads of a row, of a thread
+  constexpr int RB = D * BITS / 8, W = RB / 4 < 16 ? RB / 4 : 16, UR = RB / W;   // bytes of a row, of a load; loads of a row
+  constexpr int kTeam = 64 * WR, N = kTile * UR, UL = N > kTeam ? N / kTeam : 1; // loads of a step, of a thread
   constexpr int E = W * 8 / BITS, EU = E / 8;
-  constexpr int kBytes = kKeys * D * 2;                    // K or V of one step
+  constexpr int kRoom = (D >= 128 ? 64 : 32) / (UL * W / 2), PF = kRoom < 1 ? 1 : kRoom > 4 ? 4 : kRoom;   // registers in flight
+  constexpr int NB = WR == 1 ? 1 : 2, kBytes = kTile * D * 2;                    // K or V of a step in LDS
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, half = lane >> 5;
-  const int g = index % A.HK;
-  const int* T = A.tiles + (int64_t)(index / A.HK) * kTileInts;
-  const int b0 = T[0], row0 = T[2], key0 = T[3], split = T[5];
-  const int64_t cap = (int64_t)A.width << A.shift;
-  if (b0 < 0 || b0 >= total || row0 < 0 || key0 < 0 || split < 0 || split >= psmax) return;
-  const int rows = (int)min((int64_t)min(T[1], kPrefixRows), (int64_t)(total - b0) * A.G - row0);
-  const int steps = (int)(min((int64_t)T[4], cap) - key0) / kKeys;
-  if (rows <= 0 || steps <= 0) return;
-  const bool active = 32 * w < rows;                       // this wave has rows
-  const int row = row0 + min(32 * w + col, rows - 1);
-  const int64_t bh = (int64_t)(b0 + row / A.G) * A.HK * A.G + g * A.G + row % A.G;
+  const int col = lane & 31, half = lane >> 5, tid = threadIdx.x % kTeam, team = w / WR;
+  const int b0 = T[0], row0 = T[2], P = T[5], per = prefix_split_keys(P);
+  const int rows = (int)min((int64_t)T[1], (int64_t)(total - b0) * A.G - row0) - 32 * (w % WR);   // from this wave's first on
+  const int split = T[3] + team, key0 = team < T[4] ? split * per : 0;
+  const int steps = team < T[4] ? (min(P - key0, per)) / kTile : 0;
+  const int n = WR == 1 ? steps : (min(P - T[3] * per, per)) / kTile;            // the workgroup's longest
+  if (WR == 1 && steps == 0) return;
+  const bool active = rows > 0;
+  const int row = row0 + 32 * (w % WR) + min(col, max(rows - 1, 0));
+  const int b = b0 + (active ? row / A.G : 0), h = g * A.G + (active ? row % A.G : 0);
   // A sequence that goes through all of its keys by itself has its own splits where these would be.
-  const bool stored = 32 * w + col < rows && shared_keys<true>(A, b0 + row / A.G, A.lens[b0 + row / A.G]) > 0;
+  const bool stored = col < rows && steps > 0 && shared_keys<true>(A, b, A.lens[b]) > 0;
 
   // B operand of the scores: lane (col, half) holds row col, head_dim 16 i + 8 half .. + 7.
   bf16x8 qf[NS];
-  if (active) {
-    const uint16_t* q = A.q + (b0 + row / A.G) * A.sqb + (int64_t)(g * A.G + row % A.G) * A.sqh + 8 * half;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) qf[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 16 * i));
-  }
+  for (int i = 0; i < NS; ++i)
+    qf[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(A.q + b * A.sqb + (int64_t)h * A.sqh + 8 * half + 16 * i));
 
-  // Load j of this thread: bytes W (u % UR) of key u / UR, u = 256 j + thread, of K and of V.
+  // The page of key 32 t + lane % 32 of the split (of a step there is not: of the last one's), and
+  // its slot, once that has come (0 where there is none).
   const int* table = A.table + b0 * A.stb;
   bool bad = false;
-  auto lookup = [&](int t, int (&slot)[UL]) {
-#pragma unroll
-    for (int j = 0; j < UL; ++j) {
-      const int key = key0 + t * kKeys + (256 * j + (int)threadIdx.x) / UR;
-      const int p = table[key >> A.shift];
-      const bool ok = (unsigned)p < (unsigned)A.pages;
-      bad |= !ok;
-      slot[j] = ok ? (p << A.shift) + (key & ((1 << A.shift) - 1)) : 0;
-    }
+  auto key_of = [&](int t) { return (steps > 0 ? key0 + kTile * min(t, steps - 1) : 0) + (lane & 31); };
+  auto page_of = [&](int t) { return table[key_of(t) >> A.shift]; };
+  auto slot_of = [&](int t, int p) {
+    const bool ok = (unsigned)p < (unsigned)A.pages;
+    bad |= t < steps && !ok;
+    return ok && t < steps ? (p << A.shift) + (key_of(t) & ((1 << A.shift) - 1)) : 0;
   };
-  Words<W> rk[UL], rv[UL];
-  uint32_t sk[UL], sv[UL];
-  const char* kb = A.k + g * A.skh;
-  const char* vb = A.v + g * A.svh;
-  auto fetch = [&](const int (&slot)[UL]) {
+
+  // Load j of this thread: bytes W c of key u / UR, u = kTeam j + tid, of K and of V.
+  Words<W> rk[PF][UL], rv[PF][UL];
+  uint32_t sk[PF][UL], sv[PF][UL];
+  const int c = tid % UR, scale = E * c / kGroup;
+  const char *kb = A.k + g * A.skh + W * c, *vb = A.v + g * A.svh + W * c;
+  const uint8_t *ksb = A.ks + g * A.sksh + scale / 4 * 4, *vsb = A.vs + g * A.svsh + scale / 4 * 4;
+  auto fetch = [&](int set, int slot) {
 #pragma unroll
     for (int j = 0; j < UL; ++j) {
-      const int c = (256 * j + (int)threadIdx.x) % UR;
-      rk[j] = load_words<W>(kb + slot[j] * A.skn + W * c);
-      rv[j] = load_words<W>(vb + slot[j] * A.svn + W * c);
+      const int r = shfl_idx_i(slot, (kTeam * j + tid) % N / UR);
+      rk[set][j] = load_words<W>(kb + row_at<false>(r, A.skn));
+      rv[set][j] = load_words<W>(vb + row_at<false>(r, A.svn));
       if constexpr (BITS < 16) {
-        sk[j] = A.ks[g * A.sksh + slot[j] * A.sksn + E * c / kGroup];
-        sv[j] = A.vs[g * A.svsh + slot[j] * A.svsn + E * c / kGroup];
+        sk[set][j] = load_scales<D>(ksb + row_at<false>(r, A.sksn));
+        sv[set][j] = load_scales<D>(vsb + row_at<false>(r, A.svsn));
       }
     }
   };
-  auto put = [&](int t) {
-    lds_char* dk = (lds_char*)lds + kBytes * (t & 1);
-    lds_char* dv = (lds_char*)lds + kBytes * (2 + (t & 1));
+  lds_char* base = (lds_char*)lds + team * (NB * 2 * kBytes);
+  auto put = [&](int set, int slot) {
 #pragma unroll
     for (int j = 0; j < UL; ++j) {
-      const int u = 256 * j + (int)threadIdx.x, key = u / UR;
+      const int key = (kTeam * j + tid) % N / UR;
+      const float fk = BITS < 16 ? scale_in(sk[set][j], scale) : 0.f, fv = BITS < 16 ? scale_in(sv[set][j], scale) : 0.f;
 #pragma unroll
       for (int i = 0; i < EU; ++i) {
-        const int c = u % UR * EU + i;
-        *(__attribute__((address_space(3))) u32x4*)(dk + 16 * (key * U + (c ^ kswizzle<D>(key)))) =
-            eight<BITS>(rk[j], i, mx_scale(BITS < 16 ? sk[j] : 0));
-        *(__attribute__((address_space(3))) u32x4*)(dv + 16 * (key * U + (c ^ vswizzle<D>(key)))) =
-            eight<BITS>(rv[j], i, mx_scale(BITS < 16 ? sv[j] : 0));
+        const int u = c * EU + i;
+        lds_char* d = base + 2 * kBytes * slot + 16 * key * U;
+        *(__attribute__((address_space(3))) u32x4*)(d + 16 * (u ^ kswizzle<D>(key))) = eight<BITS>(rk[set][j], i, fk);
+        *(__attribute__((address_space(3))) u32x4*)(d + kBytes + 16 * (u ^ vswizzle<D>(key))) = eight<BITS>(rv[set][j], i, fv);
       }
     }
   };
@@ -510,80 +556,87 @@ __device__ __forceinline__ void prefix_tile(const PagedArgs& A, int total, int p
   for (int j = 0; j < DT; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
-
-  int slot[UL];
-  lookup(0, slot);
-  fetch(slot);
-  if (steps > 1) lookup(1, slot);
-  put(0);
-  for (int t = 0; t < steps; ++t) {
-    lds_barrier();                                         // step t is in place, step t - 1 has been read
-    if (t + 1 < steps) fetch(slot);
-    if (t + 2 < steps) lookup(t + 2, slot);
-    if (active) {
-      const lds_char* dk = (const lds_char*)lds + kBytes * (t & 1);
-      const lds_char* dv = (const lds_char*)lds + kBytes * (2 + (t & 1));
-      // Lane (col, half): row col, keys 32 kb + 8 (e / 4) + 4 half + e % 4.
-      f32x16 s[2];
+  auto compute = [&](int slot) {
+    const lds_char* dk = base + 2 * kBytes * slot;
+    const lds_char* dv = dk + kBytes;
+    // Lane (col, half): row col, keys 8 (e / 4) + 4 half + e % 4.
+    f32x16 s;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+    for (int i = 0; i < NS; ++i)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, read16(dk + (k_at ^ (32 * i)))), qf[i], s, 0, 0, 0);
+    float mx = s[0];
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
+      const float top = fmaxf(mx, shfl_xor(mx, 32)) * A.c;
+      const float mn = top > mref + kTau ? top : mref;     // rows that stay get a factor of exactly 1
+      const float alpha = fexp2(mref - mn);
+      lsum = lsum * alpha;
+      mref = mn;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, read16(dk + (k_at ^ (32 * i)) + 16 * 32 * U * kb)), qf[i], s[kb], 0, 0, 0);
-      float mx = s[0][0];
+      for (int j = 0; j < DT; ++j)
 #pragma unroll
-      for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
-      if (__builtin_amdgcn_ballot_w64(mx * A.c > mref + kTau) != 0) {
-        const float top = fmaxf(mx, shfl_xor(mx, 32)) * A.c;
-        const float mn = top > mref + kTau ? top : mref;   // rows that stay get a factor of exactly 1
-        const float alpha = fexp2(mref - mn);
-        lsum = lsum * alpha;
-        mref = mn;
-#pragma unroll
-        for (int j = 0; j < DT; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
-      }
-      u32x4 p[4];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float a = fexp2(__builtin_fmaf(s[i / 8][2 * i % 16], A.c, -mref));
-        const float b = fexp2(__builtin_fmaf(s[i / 8][2 * i % 16 + 1], A.c, -mref));
-        p[i / 4][i % 4] = pack_bf16x2(a, b);
-        lsum = dot2(p[i / 4][i % 4], lsum);
-      }
-      // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
-      // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < DT; ++j) {
-          s16x4 h[2];
-#pragma unroll
-          for (int z = 0; z < 2; ++z) h[z] = tr_read(dv + (v_at ^ (64 * j)) + 16 * U * (16 * i + 8 * z));
-          acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7)),
-              __builtin_bit_cast(bf16x8, p[i]), acc[j], 0, 0, 0);
-        }
+        for (int e = 0; e < 16; ++e) acc[j][e] = acc[j][e] * alpha;
     }
-    if (t + 1 < steps) put(t + 1);
+    u32x4 p[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = fexp2(__builtin_fmaf(s[2 * i], A.c, -mref)), y = fexp2(__builtin_fmaf(s[2 * i + 1], A.c, -mref));
+      p[i / 4][i % 4] = pack_bf16x2(x, y);
+      lsum = dot2(p[i / 4][i % 4], lsum);
+    }
+    // A operand of head_dim tile j, 16-key step i: V[key][32 j + lane % 32], k-slots
+    // 8 half + e <-> keys 16 i + 8 (e / 4) + 4 half + e % 4, the order in which the lane holds p.
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < DT; ++j) {
+        s16x4 h[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) h[z] = tr_read(dv + (v_at ^ (64 * j)) + 16 * U * (16 * i + 8 * z));
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7)),
+            __builtin_bit_cast(bf16x8, p[i]), acc[j], 0, 0, 0);
+      }
+  };
+
+  // No branch around the loads: past one, all in flight would be waited for.
+  int page[PF];
+#pragma unroll
+  for (int i = 0; i < PF; ++i) page[i] = page_of(i);
+  auto next = [&](int set, int t) {
+    const int slot = slot_of(t, page[set]);
+    page[set] = page_of(t + PF);
+    fetch(set, slot);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int i = 0; i < PF; ++i) next(i, i);
+  if constexpr (NB == 2) {
+    put(0, 0);
+    next(0, PF);
+    lds_barrier();                                         // step 0 is in place
   }
+  for (int t0 = 0;; t0 += PF) {
+#pragma unroll
+    for (int i = 0; i < PF; ++i) {
+      const int t = t0 + i, set = NB == 2 ? (i + 1) % PF : i, slot = NB == 2 ? t & 1 : 0;
+      put(set, NB == 2 ? slot ^ 1 : 0);                    // step t + 1, where step t - 1 has been read; or step t
+      next(set, t + PF + (NB == 2));
+      asm volatile("" ::: "memory");
+      if (active && t < steps) compute(slot);
+      if constexpr (NB == 2) lds_barrier();
+      if (t + 1 >= n) goto done;
+    }
+  }
+done:
   // A page that is none spoils every row that reads it.
-  int* flag = reinterpret_cast<int*>(lds);
-  lds_barrier();
-  if (threadIdx.x == 0) *flag = 0;
-  lds_barrier();
-  if (bad) *flag = 1;
-  lds_barrier();
   lsum = lsum + shfl_xor(lsum, 32);
+  if (__builtin_amdgcn_ballot_w64(bad) != 0) lsum = __builtin_nanf("");
   if (!stored) return;
-  if (*flag) lsum = __builtin_nanf("");
-  const int64_t at = bh * A.smax + split;
+  const int64_t at = ((int64_t)b * A.HK * A.G + h) * A.smax + split;
 #pragma unroll
   for (int j = 0; j < DT; ++j)
 #pragma unroll
@@ -593,8 +646,24 @@ __device__ __forceinline__ void prefix_tile(const PagedArgs& A, int total, int p
   if (half == 0) A.pml[at] = f32x2{mref, lsum};
 }
 
+// Waves of a tile's rows: they share a split, the others take the next ones.
+__host__ __device__ __forceinline__ int prefix_waves(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
 template <int D, int BITS>
-__global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(PagedArgs A) {
+__device__ __forceinline__ void prefix_tile(const PagedArgs& A, int total, int index, char* lds) {
+  const int g = index % A.HK;
+  const int* T = A.tiles + (int64_t)(index / A.HK) * kTileInts;
+  const int b0 = T[0], rows = T[1], row0 = T[2], split0 = T[3], splits = T[4], P = T[5];
+  if (b0 < 0 || b0 >= total || rows < 1 || rows > kPrefixRows || row0 < 0 || row0 >= (int64_t)(total - b0) * A.G) return;
+  if (P < kKeys || P % kKeys || P > A.longest || P > ((int64_t)A.width << A.shift)) return;
+  if (split0 < 0 || splits < 1 || splits > 4 / prefix_waves(rows) || split0 > prefix_splits(P) - splits) return;
+  if (rows <= 32) prefix_rows<D, BITS, 1>(A, total, T, g, lds);
+  else if (rows <= 64) prefix_rows<D, BITS, 2>(A, total, T, g, lds);
+  else prefix_rows<D, BITS, 4>(A, total, T, g, lds);
+}
+
+template <int D, int BITS>
+__global__ __launch_bounds__(256, (PagedGeom<D, BITS>::kPerCU)) void paged_attn_kernel(PagedArgs A) {
   __shared__ __align__(16) char stage[kWaves][kTile * D * 2];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ int first[kSeqs + 1], length[kSeqs];
@@ -603,11 +672,11 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void paged_attn_kernel(P
 
 // The first `tiles` workgroups take the shared keys, the rest the sequences' own.
 template <int D, int BITS>
-__global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void shared_attn_kernel(PagedArgs A, int total, int psmax, int tiles) {
-  constexpr int kPrefixBytes = 4 * kKeys * D * 2;
+__global__ __launch_bounds__(256, (PagedGeom<D, BITS>::kSharedPerCU)) void shared_attn_kernel(PagedArgs A, int total, int tiles) {
+  constexpr int kPrefixBytes = 2 * kWaves * kTile * D * 2;
   __shared__ __align__(16) char lds[sizeof(PagedLds<D, true>) > kPrefixBytes ? sizeof(PagedLds<D, true>) : kPrefixBytes];
   if ((int)blockIdx.x < tiles) {
-    prefix_tile<D, BITS>(A, total, psmax, blockIdx.x, lds);
+    prefix_tile<D, BITS>(A, total, blockIdx.x, lds);
   } else {
     auto& x = *reinterpret_cast<PagedLds<D, true>*>(lds);
     paged_items<D, BITS, true>(A, blockIdx.x - tiles, gridDim.x - tiles, x.stage, x.sm, x.sl, x.first, x.length, x.from);
@@ -617,20 +686,22 @@ __global__ __launch_bounds__(256, PagedGeom<D>::kPerCU) void shared_attn_kernel(
 // One workgroup per (query head, sequence).  Every wave takes the splits' weights, lane s
 // that of split s; then lanes of four columns each sum every (256 / (D / 4))-th split, and
 // those sums are added in order.
-template <int D, bool SHARED>
+template <int D, int BITS, bool SHARED>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
-  constexpr int L = D / 4, P = 256 / L, kMost = kMaxSplits + (SHARED ? kMaxPrefixSplits : 0);
-  __shared__ float wt[kMost];
+  constexpr int L = D / 4, P = 256 / L, kMost = most_splits(BITS) + (SHARED ? kMaxPrefixSplits : 0);
+  constexpr int R = (kMost + 63) / 64;                     // splits of a lane: lane, lane + 64
+  __shared__ float wt[64 * R];
   __shared__ __align__(16) f32x4 sums[P][L];
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63;
   const int64_t p = ((int64_t)b * A.HK * A.G + h) * A.smax;
-  const f32x2 held = lane < A.smax ? A.pml[p + lane] : f32x2{kNone, 0.f};   // beside the length
+  f32x2 ml[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) ml[i] = lane + 64 * i < A.smax ? A.pml[p + lane + 64 * i] : f32x2{kNone, 0.f};   // beside the length
   const int n = A.lens[b];
   if (n <= 0 || n > ((int64_t)A.width << A.shift)) return;
   const int from = shared_keys<SHARED>(A, b, n);
-  const int splits = (from > 0 ? prefix_splits(from) : 0) + split_count(n - from);
+  const int splits = (from > 0 ? prefix_splits(from) : 0) + split_count<BITS>(n - from);
   if (splits == 1 && from == 0) return;
-  const f32x2 ml = lane < splits ? held : f32x2{kNone, 0.f};
   const int c = threadIdx.x % L, part = threadIdx.x / L;
   constexpr int N = (kMost + P - 1) / P;
   f32x4 x[N];
@@ -640,12 +711,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
     x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (s < splits) x[i] = *reinterpret_cast<const f32x4*>(A.po + (p + s) * D + 4 * c);
   }
-  float m = ml[0];
+  float m = kNone;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (lane + 64 * i >= splits) ml[i] = f32x2{kNone, 0.f};
+    m = fmaxf(m, ml[i][0]);
+  }
   for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-  const float a = fexp2(ml[0] - m);
-  float l = ml[1] * a;
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const float a = fexp2(ml[i][0] - m);
+    l = i == 0 ? ml[i][1] * a : __builtin_fmaf(ml[i][1], a, l);
+    if (threadIdx.x < 64) wt[lane + 64 * i] = a;
+  }
   for (int k = 32; k >= 1; k >>= 1) l = l + __shfl_xor(l, k);
-  if (threadIdx.x < kMost) wt[threadIdx.x] = a;
   __syncthreads();
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -669,15 +749,15 @@ int launch(PagedArgs A, int B, hipStream_t s) {
   const int psmax = SHARED ? prefix_split_bound(A.longest) : 0;
   for (int b0 = 0; b0 < B; b0 += kSeqs) {
     A.B = B - b0 < kSeqs ? B - b0 : kSeqs;
-    const int64_t items = (int64_t)A.B * (A.smax - psmax) * A.HK, most = kCUs * PagedGeom<D>::kPerCU;
+    const int64_t items = (int64_t)A.B * (A.smax - psmax) * A.HK, most = kCUs * (SHARED ? PagedGeom<D, BITS>::kSharedPerCU : PagedGeom<D, BITS>::kPerCU);
     const unsigned blocks = (unsigned)(items < most ? items : most);
     if constexpr (SHARED) {
       const int tiles = b0 == 0 ? A.n_tiles * A.HK : 0;    // of all sequences
-      hipLaunchKernelGGL((shared_attn_kernel<D, BITS>), dim3(tiles + blocks), dim3(256), 0, s, A, B, psmax, tiles);
+      hipLaunchKernelGGL((shared_attn_kernel<D, BITS>), dim3(tiles + blocks), dim3(256), 0, s, A, B, tiles);
     } else {
       hipLaunchKernelGGL((paged_attn_kernel<D, BITS>), dim3(blocks), dim3(256), 0, s, A);
     }
-    if (A.smax > 1) hipLaunchKernelGGL((paged_join_kernel<D, SHARED>), dim3(A.HK * A.G, A.B), dim3(256), 0, s, A);
+    if (A.smax > 1) hipLaunchKernelGGL((paged_join_kernel<D, BITS, SHARED>), dim3(A.HK * A.G, A.B), dim3(256), 0, s, A);
     A.q += A.B * A.sqb;
     A.out += A.B * A.sob;
     A.table += A.B * A.stb;
@@ -701,9 +781,9 @@ int launch_for(int D, const PagedArgs& A, int B, hipStream_t s) {
 
 bool head_dim_ok(int D) { return D == 32 || D == 64 || D == 128 || D == 256; }
 
-int64_t workspace(int B, int H, int D, int page, int width, int psmax) {
+int64_t workspace(int B, int H, int D, int page, int width, int psmax, int bits) {
   if (B < 0 || H < 1 || page < 1 || width < 0 || !head_dim_ok(D)) return -1;
-  const int smax = split_bound((int64_t)width * page) + psmax;
+  const int smax = split_bound((int64_t)width * page, bits) + psmax;
   return smax <= 1 ? 0 : (int64_t)B * H * smax * (D + 2) * 4;
 }
 
@@ -729,6 +809,9 @@ int attend(const void* q, int64_t sqb, int64_t sqh, const PoolArg& k, const Pool
   if (B == 0) return RSPX_OK;
   if (!q || !k.rows || !v.rows || !lens || !out || (width && !table)) return RSPX_EINVAL;
   if (bits < 16 && (!k.scales || !v.scales)) return RSPX_EINVAL;
+  if (bits < 16 || shared)
+    for (const int64_t s : {k.sn, v.sn, bits < 16 ? k.ssn : 0, bits < 16 ? v.ssn : 0})
+      if (s < 0 || s > INT32_MAX) return s < 0 ? RSPX_EINVAL : RSPX_EUNSUPPORTED;
   if (shared && (!prefix || (n_tiles && !tiles))) return RSPX_EINVAL;
   auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   if (reinterpret_cast<uintptr_t>(out) & 1u) return RSPX_EALIGN;
@@ -736,7 +819,7 @@ int attend(const void* q, int64_t sqb, int64_t sqh, const PoolArg& k, const Pool
   if (!al(q) || !al(k.rows) || !al(v.rows) || sqb % 8 || sqh % 8 || k.sh % unit || k.sn % unit || v.sh % unit || v.sn % unit)
     return RSPX_EALIGN;
   const int psmax = shared ? prefix_split_bound(longest) : 0;
-  const int64_t need = workspace(B, H, D, page, width, psmax);
+  const int64_t need = workspace(B, H, D, page, width, psmax, bits);
   if (need > 0 && (!ws || ws_bytes < need)) return RSPX_EWORKSPACE;
   if (need > 0 && !al(ws)) return RSPX_EALIGN;
   const int64_t e = bits == 16 ? 2 : 1;
@@ -756,7 +839,7 @@ int attend(const void* q, int64_t sqb, int64_t sqh, const PoolArg& k, const Pool
   A.sksh = k.ssh, A.sksn = k.ssn, A.svsh = v.ssh, A.svsn = v.ssn;
   A.HK = HK, A.G = H / HK, A.pages = pages, A.width = width;
   A.shift = __builtin_ctz((unsigned)page);
-  const int smax = split_bound((int64_t)width * page);
+  const int smax = split_bound((int64_t)width * page, bits);
   A.smax = (smax < 1 ? 1 : smax) + psmax;
   A.pml = reinterpret_cast<f32x2*>(A.po + (int64_t)B * H * A.smax * D);
   A.c = sm_scale * 1.44269504088896340736f;
@@ -776,7 +859,7 @@ int attend(const void* q, int64_t sqb, int64_t sqh, const PoolArg& k, const Pool
 using namespace rspx;
 
 extern "C" int64_t rspx_paged_attn_workspace_bytes(int B, int H, int D, int page, int width) {
-  return workspace(B, H, D, page, width, 0);
+  return workspace(B, H, D, page, width, 0, RSPX_BF16);
 }
 
 extern "C" int rspx_paged_attn(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn,
@@ -811,22 +894,26 @@ extern "C" int64_t rspx_shared_plan(const int64_t* members, const int64_t* keys,
     const int p = members[i] < 2 ? 0 : (int)(keys[i] / kKeys * kKeys);
     if (b + members[i] > INT32_MAX / 16) return RSPX_EINVAL;
     if (prefix) std::fill(prefix + b, prefix + b + members[i], p);
-    const int per = prefix_split_keys(p), rows = (int)members[i] * group;
+    const int rows = (int)members[i] * group, splits = p ? prefix_splits(p) : 0;
     // The row blocks of a split beside one another: they read the same keys.
-    for (int64_t k = 0, split = 0; k < p; k += per, ++split)
-      for (int r = 0; r < rows; r += kPrefixRows, ++count)
-        if (tiles) {
-          int32_t* t = tiles + count * kTileInts;
-          t[0] = (int32_t)b, t[1] = std::min(rows - r, kPrefixRows), t[2] = r, t[3] = (int32_t)k;
-          t[4] = (int32_t)std::min<int64_t>(k + per, p), t[5] = (int32_t)split, t[6] = t[7] = 0;
-        }
+    for (int split = 0; split < splits; split += 4)
+      for (int r = 0; r < rows; r += kPrefixRows) {
+        const int part = std::min(rows - r, kPrefixRows), each = 4 / prefix_waves(part);
+        for (int k = split; k < std::min(split + 4, splits); k += each, ++count)
+          if (tiles) {
+            int32_t* t = tiles + count * kTileInts;
+            t[0] = (int32_t)b, t[1] = part, t[2] = r, t[3] = k, t[4] = std::min({each, splits - k, split + 4 - k});
+            t[5] = p, t[6] = t[7] = 0;
+          }
+      }
     b += members[i];
   }
   return count;
 }
 
-extern "C" int64_t rspx_paged_attn_shared_workspace_bytes(int B, int H, int D, int page, int width, int longest) {
-  return longest < 0 ? -1 : workspace(B, H, D, page, width, prefix_split_bound(longest));
+extern "C" int64_t rspx_paged_attn_shared_workspace_bytes(int B, int H, int D, int page, int width, int longest, int format) {
+  if (longest < 0 || (format != RSPX_BF16 && format != RSPX_MXFP8 && format != RSPX_MXFP4)) return -1;
+  return workspace(B, H, D, page, width, prefix_split_bound(longest), format);
 }
 
 extern "C" int rspx_paged_attn_shared(const void* q, int64_t sqb, int64_t sqh, const void* kc, int64_t skh, int64_t skn,

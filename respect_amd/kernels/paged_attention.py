@@ -116,7 +116,7 @@ def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None, share
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     with torch.cuda.device(q.device):
         # Of this call alone: torch hands it to the stream, or to the graph being captured.
-        need = max(0, L.rspx_paged_attn_shared_workspace_bytes(B, H, D, page, width, 0 if shared is None else shared.longest))
+        need = max(0, L.rspx_paged_attn_shared_workspace_bytes(B, H, D, page, width, 0 if shared is None else shared.longest, bits))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         rest = (out.data_ptr(), out.stride(0), out.stride(1), B, H, HK, D, slots // page, page, width, scale)
         end = (ws.data_ptr() if need else None, need, _lib.stream_ptr(q.device))

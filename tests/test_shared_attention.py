@@ -120,15 +120,17 @@ def test_plans():
     assert p.B == 46 and p.longest == 960
     assert p.prefix.tolist() == [0] + [128] * 3 + [0] * 2 + [960] * 40
     t = p.tiles.tolist()
-    assert t[0] == [1, 12, 0, 0, 128, 0, 0, 0]
-    assert [x[:6] for x in t[1:3]] == [[6, 128, 0, 0, 256, 0], [6, 32, 128, 0, 256, 0]] and len(t) == 1 + 2 * 4
-    assert t[-1] == [6, 32, 128, 768, 960, 3, 0, 0]
-    long = _plan([2], [1 << 20], 16, device="cpu").tiles
-    assert len(long) == 16 and (long[1:, 3] == long[:-1, 4]).all() and ((long[:, 4] - long[:, 3]) % 64 == 0).all()
-    for keys in (64, 255, 256, 4095, 4096, 4097, 4160, 5000, 70000, 131072):
-        t = _plan([2], [keys], 1, device="cpu").tiles
-        assert len(t) <= 16 and t[0, 3] == 0 and t[-1, 4] == keys // 64 * 64 and (t[1:, 3] == t[:-1, 4]).all()
-        assert t[:, 5].tolist() == list(range(len(t))) and (t[:, 3] < t[:, 4]).all()
+    assert t[0] == [1, 12, 0, 0, 1, 128, 0, 0] and t[1] == [6, 128, 0, 0, 1, 960, 0, 0] and t[5] == [6, 32, 128, 0, 4, 960, 0, 0]
+    for keys in (64, 128, 192, 4095, 4096, 4160, 8000, 16384, 16448, 32768, 32832, 131072, 1 << 30, (1 << 31) - 1):
+        for members, group in ((2, 1), (8, 4), (9, 4), (20, 4), (33, 4), (97, 4), (70, 16)):
+            taken = {}
+            for b0, rows, row0, split, splits, n, _, _ in _plan([members], [keys], group, device="cpu").tiles.tolist():
+                assert b0 == 0 and n == keys // 64 * 64 and row0 % 128 == 0 and rows == min(128, members * group - row0)
+                assert 1 <= splits <= (4 if rows <= 32 else 2 if rows <= 64 else 1)
+                taken.setdefault(row0, []).extend(range(split, split + splits))
+            assert sorted(taken) == list(range(0, members * group, 128))
+            assert all(sorted(x) == list(range(len(x))) == list(range(len(taken[0]))) for x in taken.values())
+            assert len(taken[0]) <= 64 and 128 * len(taken[0]) < keys // 64 * 64 + 128
     e = _plan([], [], 4, device="cpu")
     assert e.B == 0 and e.longest == 0 and len(e.tiles) == 0
     for bad in (([1], [1, 2], 4), ([-1], [5], 4), ([2], [-5], 4), ([2], [5], 0), ([2], [5], 17), ([1 << 28], [64], 16),
@@ -230,15 +232,16 @@ def test_refusals():
         assert call(sh, width=-1) == -1 and call(sh, scale=0.0) == -1 and call(sh, p=0) == -1 and call(sh, lens=0) == -1
         assert call(sh, table=0) == -1 and call(sh, s=0) == -1 and call(sh, pages=1 << 28) == -1
         assert call(sh, D=96) == -2 and call(sh, H=34) == -2 and call(sh, fmt=6) == -2
-        assert call(sh, p=8) == -4 and call(sh, st=72) == -4
+        assert call(sh, p=8) == -4 and call(sh, st=72) == -4 and call(sh, st=1 << 31) == -2 and call(sh, st=-64) == -1
         assert call(sh, width=1024, ws=16) == -3
         assert call(sh, B=0) == 0
     assert call(False, fmt=16) == -2
     assert call(True, prefix=0) == -1 and call(True, tiles=0) == -1 and call(True, n=-1) == -1 and call(True, longest=-1) == -1
     assert call(True, longest=129) == -1 and call(True, n=1 << 23) == -2 and call(True, ws=16) == -3
-    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 64, 16, 8, 0) == 0
-    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 64, 16, 8, 64) == 2 * 4 * 2 * 66 * 4
-    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 96, 16, 8, 64) == -1
+    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 64, 16, 8, 0, 16) == 0
+    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 64, 16, 8, 64, 8) == 2 * 4 * 2 * 66 * 4
+    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 96, 16, 8, 64, 4) == -1
+    assert lib.rspx_paged_attn_shared_workspace_bytes(2, 4, 64, 16, 8, 64, 5) == -1
     assert lib.rspx_shared_plan(None, None, 1, 4, None, None) == -1 and lib.rspx_shared_plan(None, None, 0, 4, None, None) == 0
 
 
