@@ -74,10 +74,10 @@ __host__ __forceinline__ int split_bound(int64_t n, int bits) {
   return n >= (int64_t)kSplitKeys * most ? most : (int)((n + kSplitKeys - 1) / kSplitKeys);
 }
 
-// The same for n shared keys: 32 splits of 128 to 512 keys, past that 64.
+// The same for n shared keys: 20 splits of 128 to 512 keys, past that up to 64.
 __host__ __device__ __forceinline__ int prefix_split_keys(int n) {
   auto parts = [&](unsigned m) { return ((unsigned)n + m * kKeys - 1) / (m * kKeys) * kKeys; };
-  const unsigned per = parts(32);
+  const unsigned per = parts(20);
   return per <= 128 ? 128 : per <= 512 ? (int)per : parts(64) <= 512 ? 512 : (int)parts(64);
 }
 __host__ __device__ __forceinline__ int prefix_splits(int n) {
@@ -87,7 +87,7 @@ __host__ __device__ __forceinline__ int prefix_splits(int n) {
 // The most splits that any n up to this one gives.
 __host__ __forceinline__ int prefix_split_bound(int n) {
   const unsigned some = ((unsigned)n + 127) / 128, many = ((unsigned)n + 511) / 512;
-  return (int)std::min<unsigned>(kMaxPrefixSplits, std::max<unsigned>(std::min<unsigned>(some, 32), many));
+  return (int)std::min<unsigned>(kMaxPrefixSplits, std::max<unsigned>(std::min<unsigned>(some, 20), many));
 }
 
 struct PagedArgs {
@@ -104,18 +104,23 @@ struct PagedArgs {
   float c;                     // scale * log2(e)
 };
 
-// Of sequence b, of n keys: those that the launch's tiles compute, 0 where it is too short for
-// them and goes through all of its own.
-template <bool SHARED>
-__device__ __forceinline__ int shared_keys(const PagedArgs& A, int b, int n) {
-  if constexpr (!SHARED) return 0;
-  const int p = A.prefix[b];
+// Of a sequence of n keys that says it shares p: those that the launch's tiles compute, 0 where it
+// is too short for them and goes through all of its own.
+__device__ __forceinline__ int shared_keys(const PagedArgs& A, int p, int n) {
   return p > 0 && p <= A.longest && p <= n && n <= ((int64_t)A.width << A.shift) ? p : 0;
 }
 
-// first[b]: the splits of sequences before b (one for a sequence without any, whose rows
-// are written too), length[b]: lens[b]; returns the number of splits.  All 256 threads call it.
-// The keys that from[b] says are shared have splits elsewhere.
+// A sequence of n > 0 keys as items, one for each workgroup that takes part: every split for every
+// kv head, or, of no more keys than a wave takes at once, four kv heads (the result is the one that
+// a workgroup's other waves, without keys, would leave as it is).
+template <int BITS>
+__device__ __forceinline__ int item_count(int n, int HK) {
+  return n <= kTile ? (n > 0 ? (HK + kWaves - 1) / kWaves : 0) : split_count<BITS>(n) * HK;
+}
+
+// first[b]: the items of sequences before b (one for each kv head of a sequence without keys,
+// whose rows are written too), length[b]: lens[b]; returns their number.  All 256 threads call it.
+// The keys that from[b] says are shared are items elsewhere.
 template <int BITS, bool SHARED>
 __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* first, int* length, int* from) {
   const int* lens = A.lens;
@@ -130,10 +135,10 @@ __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* 
     if (b < B) {
       const int n = lens[b];
       length[b] = n;
-      cnt[i] = n <= 0 || n > cap ? 1 : split_count<BITS>(n);
+      cnt[i] = n <= 0 || n > cap ? A.HK : item_count<BITS>(n, A.HK);
       if constexpr (SHARED) {
-        const int p = from[b] = shared_keys<true>(A, b, n);
-        if (p > 0) cnt[i] = split_count<BITS>(n - p);
+        const int p = from[b] = shared_keys(A, A.prefix[b], n);
+        if (p > 0) cnt[i] = item_count<BITS>(n - p, A.HK);
       }
     }
     sum += cnt[i];
@@ -159,7 +164,7 @@ __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* 
   return __builtin_amdgcn_readfirstlane(first[kSeqs]);
 }
 
-// The sequence that split number i belongs to: the last one with first[b] <= i, by the counts of
+// The sequence that item i belongs to: the last one with first[b] <= i, by the counts of
 // those up to i among every 16th and then among 16 (two reads of LDS one after the other, where a
 // binary search makes ten).
 __device__ __forceinline__ int find_seq(const int* first, int i) {
@@ -201,6 +206,7 @@ struct PagedGeom {
 // One split of one sequence for one kv head.
 struct Item {
   int g, b, from, n, split, splits;   // keys from .. from + n - 1
+  int heads;                   // kv heads of the workgroup: this one, or one per wave
   int t, tend;                 // this wave's first tile, and the end of the split's
 };
 
@@ -225,25 +231,34 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, c16 = lane & 15, r4 = lane >> 4;
   const int64_t cap = (int64_t)A.width << A.shift;
-  const int items = list_items<BITS, SHARED>(A, cap, first, length, from) * A.HK;
+  const int items = list_items<BITS, SHARED>(A, cap, first, length, from);
   if (block >= items) return;
 
   auto decode = [&](int i) {
     Item x;
-    x.g = i % A.HK;
-    x.b = find_seq(first, i / A.HK);
-    x.split = i / A.HK - __builtin_amdgcn_readfirstlane(first[x.b]);
+    x.b = find_seq(first, i);
+    const int r = i - __builtin_amdgcn_readfirstlane(first[x.b]);
     x.n = __builtin_amdgcn_readfirstlane(length[x.b]);
-    x.splits = x.t = x.tend = x.from = 0;
+    x.g = r;
+    x.split = x.splits = x.t = x.tend = x.from = 0;
+    x.heads = 1;
     if (x.n > 0 && x.n <= cap) {
       if constexpr (SHARED) {
         x.from = __builtin_amdgcn_readfirstlane(from[x.b]);
         x.n -= x.from;
       }
-      const int per = split_keys<BITS>(x.n);
       x.splits = split_count<BITS>(x.n);
-      x.t = x.split * (per / kTile) + w;
-      x.tend = ((int)min((int64_t)x.n, (int64_t)(x.split + 1) * per) + kTile - 1) / kTile;
+      if (x.n <= kTile) {
+        x.heads = kWaves;
+        x.g = min(kWaves * r + w, A.HK - 1);
+        x.tend = kWaves * r + w < A.HK;
+      } else {
+        const int per = split_keys<BITS>(x.n);
+        x.split = r / A.HK;
+        x.g = r - x.split * A.HK;
+        x.t = x.split * (per / kTile) + w;
+        x.tend = ((int)min((int64_t)x.n, (int64_t)(x.split + 1) * per) + kTile - 1) / kTile;
+      }
     }
     return x;
   };
@@ -417,6 +432,24 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
     load_q(nxt);              // on its way while this item's waves are joined
     if (cur.splits == 0) {    // no keys: zeros; a length that does not fit: NaN
       for (int i = threadIdx.x; i < A.G * D; i += 256) orow[(i / D) * A.soh + i % D] = cur.n == 0 ? 0 : 0x7fc0;
+    } else if (cur.heads > 1) {   // this wave's own
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) lsum = __builtin_nanf("");
+      lsum = sum4(lsum);
+      const int64_t p = (((int64_t)cur.b * A.HK + cur.g) * A.G + c16) * A.smax + (SHARED ? prefix_splits(cur.from) : 0);
+      if (cur.tend > 0 && c16 < A.G) {
+#pragma unroll
+        for (int j = 0; j < DT; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + 0.f;   // as joined: no -0
+          if (cur.from == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) orow[c16 * A.soh + 16 * j + 4 * r4 + e] = f32_to_bf16_rne(acc[j][e] / lsum);
+          } else {
+            *reinterpret_cast<f32x4*>(A.po + p * D + 16 * j + 4 * r4) = acc[j];
+          }
+        }
+        if (cur.from != 0 && r4 == 0) A.pml[p] = f32x2{mref, lsum};
+      }
     } else {
       if (__builtin_amdgcn_ballot_w64(bad) != 0) lsum = __builtin_nanf("");
       lsum = sum4(lsum);
@@ -469,12 +502,14 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 // the other half; the probabilities, rounded to bf16 (half a step each) and summed as rounded, are
 // used in place.  Every row sees all keys: there is no mask.
 template <int D, int BITS, int WR>
-__device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const int* T, int g, char* lds) {
+__device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const int (&T)[kTileInts], int g, char* lds) {
   constexpr int U = D / 8, NS = D / 16, DT = D / 32;
-  constexpr int RB = D * BITS / 8, W = RB / 4 < 16 ? RB / 4 : 16, UR = RB / W;   // bytes of a row, of a load; loads of a row
-  constexpr int kTeam = 64 * WR, N = kTile * UR, UL = N > kTeam ? N / kTeam : 1; // loads of a step, of a thread
+  // Bytes of a row and of a load, eight elements or more; loads of a row, of a step, of a thread.
+  constexpr int kTeam = 64 * WR, RB = D * BITS / 8, kShare = kTile * RB / kTeam;
+  constexpr int W = kShare >= 16 ? 16 : kShare > BITS ? kShare : BITS;
+  constexpr int UR = RB / W, N = kTile * UR, UL = N > kTeam ? N / kTeam : 1;
   constexpr int E = W * 8 / BITS, EU = E / 8;
-  constexpr int kRoom = (D >= 128 ? 64 : 32) / (UL * W / 2), PF = kRoom < 1 ? 1 : kRoom > 4 ? 4 : kRoom;   // registers in flight
+  constexpr int kRoom = (D >= 128 ? (WR == 1 ? 64 : 48) : 32) / (UL * W / 2), PF = kRoom < 1 ? 1 : kRoom > 4 ? 4 : kRoom;   // registers in flight
   constexpr int NB = WR == 1 ? 1 : 2, kBytes = kTile * D * 2;                    // K or V of a step in LDS
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5, tid = threadIdx.x % kTeam, team = w / WR;
@@ -487,8 +522,7 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   const bool active = rows > 0;
   const int row = row0 + 32 * (w % WR) + min(col, max(rows - 1, 0));
   const int b = b0 + (active ? row / A.G : 0), h = g * A.G + (active ? row % A.G : 0);
-  // A sequence that goes through all of its keys by itself has its own splits where these would be.
-  const bool stored = col < rows && steps > 0 && shared_keys<true>(A, b, A.lens[b]) > 0;
+  const int keys = A.lens[b], prefix = A.prefix[b];
 
   // B operand of the scores: lane (col, half) holds row col, head_dim 16 i + 8 half .. + 7.
   bf16x8 qf[NS];
@@ -514,10 +548,19 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   const int c = tid % UR, scale = E * c / kGroup;
   const char *kb = A.k + g * A.skh + W * c, *vb = A.v + g * A.svh + W * c;
   const uint8_t *ksb = A.ks + g * A.sksh + scale / 4 * 4, *vsb = A.vs + g * A.svsh + scale / 4 * 4;
-  auto fetch = [&](int set, int slot) {
+  struct RowsOf {
+    int r[UL];
+  };
+  auto rows_of = [&](int slot) {
+    RowsOf x;
+#pragma unroll
+    for (int j = 0; j < UL; ++j) x.r[j] = shfl_idx_i(slot, (kTeam * j + tid) % N / UR);
+    return x;
+  };
+  auto fetch = [&](int set, const RowsOf& x) {
 #pragma unroll
     for (int j = 0; j < UL; ++j) {
-      const int r = shfl_idx_i(slot, (kTeam * j + tid) % N / UR);
+      const int r = x.r[j];
       rk[set][j] = load_words<W>(kb + row_at<false>(r, A.skn));
       rv[set][j] = load_words<W>(vb + row_at<false>(r, A.svn));
       if constexpr (BITS < 16) {
@@ -525,6 +568,7 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
         sv[set][j] = load_scales<D>(vsb + row_at<false>(r, A.svsn));
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
   lds_char* base = (lds_char*)lds + team * (NB * 2 * kBytes);
   auto put = [&](int set, int slot) {
@@ -556,16 +600,20 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   for (int j = 0; j < DT; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+  u32x4 kf[NS];                                            // A operands of the scores
+  auto read_k = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) kf[i] = read16(base + 2 * kBytes * slot + (k_at ^ (32 * i)));
+  };
   auto compute = [&](int slot) {
-    const lds_char* dk = base + 2 * kBytes * slot;
-    const lds_char* dv = dk + kBytes;
+    const lds_char* dv = base + 2 * kBytes * slot + kBytes;
     // Lane (col, half): row col, keys 8 (e / 4) + 4 half + e % 4.
     f32x16 s;
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, read16(dk + (k_at ^ (32 * i)))), qf[i], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf[i]), qf[i], s, 0, 0, 0);
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
@@ -607,10 +655,9 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
 #pragma unroll
   for (int i = 0; i < PF; ++i) page[i] = page_of(i);
   auto next = [&](int set, int t) {
-    const int slot = slot_of(t, page[set]);
+    const RowsOf x = rows_of(slot_of(t, page[set]));
     page[set] = page_of(t + PF);
-    fetch(set, slot);
-    __builtin_amdgcn_sched_barrier(0);
+    fetch(set, x);
   };
 #pragma unroll
   for (int i = 0; i < PF; ++i) next(i, i);
@@ -622,10 +669,14 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   for (int t0 = 0;; t0 += PF) {
 #pragma unroll
     for (int i = 0; i < PF; ++i) {
-      const int t = t0 + i, set = NB == 2 ? (i + 1) % PF : i, slot = NB == 2 ? t & 1 : 0;
+      const int t = t0 + i, set = NB == 2 ? (i + 1) % PF : i, slot = NB == 2 ? t & 1 : 0, ahead = t + PF + (NB == 2);
+      if constexpr (NB == 2) read_k(slot);
+      const RowsOf x = rows_of(slot_of(ahead, page[set]));
+      page[set] = page_of(ahead + PF);
       put(set, NB == 2 ? slot ^ 1 : 0);                    // step t + 1, where step t - 1 has been read; or step t
-      next(set, t + PF + (NB == 2));
+      fetch(set, x);
       asm volatile("" ::: "memory");
+      if constexpr (NB == 1) read_k(0);
       if (active && t < steps) compute(slot);
       if constexpr (NB == 2) lds_barrier();
       if (t + 1 >= n) goto done;
@@ -635,7 +686,8 @@ done:
   // A page that is none spoils every row that reads it.
   lsum = lsum + shfl_xor(lsum, 32);
   if (__builtin_amdgcn_ballot_w64(bad) != 0) lsum = __builtin_nanf("");
-  if (!stored) return;
+  // A sequence that goes through all of its keys by itself has its own splits where these would be.
+  if (col >= rows || steps == 0 || shared_keys(A, prefix, keys) == 0) return;
   const int64_t at = ((int64_t)b * A.HK * A.G + h) * A.smax + split;
 #pragma unroll
   for (int j = 0; j < DT; ++j)
@@ -652,7 +704,10 @@ __host__ __device__ __forceinline__ int prefix_waves(int rows) { return rows <= 
 template <int D, int BITS>
 __device__ __forceinline__ void prefix_tile(const PagedArgs& A, int total, int index, char* lds) {
   const int g = index % A.HK;
-  const int* T = A.tiles + (int64_t)(index / A.HK) * kTileInts;
+  int T[kTileInts];
+  __builtin_memcpy(T, A.tiles + (int64_t)(index / A.HK) * kTileInts, sizeof T);
+#pragma unroll
+  for (int i = 0; i < kTileInts; ++i) T[i] = __builtin_amdgcn_readfirstlane(T[i]);
   const int b0 = T[0], rows = T[1], row0 = T[2], split0 = T[3], splits = T[4], P = T[5];
   if (b0 < 0 || b0 >= total || rows < 1 || rows > kPrefixRows || row0 < 0 || row0 >= (int64_t)(total - b0) * A.G) return;
   if (P < kKeys || P % kKeys || P > A.longest || P > ((int64_t)A.width << A.shift)) return;
@@ -699,7 +754,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
   for (int i = 0; i < R; ++i) ml[i] = lane + 64 * i < A.smax ? A.pml[p + lane + 64 * i] : f32x2{kNone, 0.f};   // beside the length
   const int n = A.lens[b];
   if (n <= 0 || n > ((int64_t)A.width << A.shift)) return;
-  const int from = shared_keys<SHARED>(A, b, n);
+  const int from = SHARED ? shared_keys(A, A.prefix[b], n) : 0;
   const int splits = (from > 0 ? prefix_splits(from) : 0) + split_count<BITS>(n - from);
   if (splits == 1 && from == 0) return;
   const int c = threadIdx.x % L, part = threadIdx.x / L;
