@@ -432,29 +432,11 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
     load_q(nxt);              // on its way while this item's waves are joined
     if (cur.splits == 0) {    // no keys: zeros; a length that does not fit: NaN
       for (int i = threadIdx.x; i < A.G * D; i += 256) orow[(i / D) * A.soh + i % D] = cur.n == 0 ? 0 : 0x7fc0;
-    } else if (cur.heads > 1) {   // this wave's own
-      if (__builtin_amdgcn_ballot_w64(bad) != 0) lsum = __builtin_nanf("");
-      lsum = sum4(lsum);
-      const int64_t p = (((int64_t)cur.b * A.HK + cur.g) * A.G + c16) * A.smax + (SHARED ? prefix_splits(cur.from) : 0);
-      if (cur.tend > 0 && c16 < A.G) {
-#pragma unroll
-        for (int j = 0; j < DT; ++j) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] + 0.f;   // as joined: no -0
-          if (cur.from == 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) orow[c16 * A.soh + 16 * j + 4 * r4 + e] = f32_to_bf16_rne(acc[j][e] / lsum);
-          } else {
-            *reinterpret_cast<f32x4*>(A.po + p * D + 16 * j + 4 * r4) = acc[j];
-          }
-        }
-        if (cur.from != 0 && r4 == 0) A.pml[p] = f32x2{mref, lsum};
-      }
     } else {
       if (__builtin_amdgcn_ballot_w64(bad) != 0) lsum = __builtin_nanf("");
       lsum = sum4(lsum);
-      // The four waves' results, joined in wave order.  A wave's stage holds its [16][D] sums
-      // (the tile's V has been read by this wave).
+      // The four waves' results, joined in wave order, or this wave's own.  A wave's stage holds its
+      // [16][D] sums (the tile's V has been read by this wave).
       float* so = reinterpret_cast<float*>(&stage[0][0]);
 #pragma unroll
       for (int j = 0; j < DT; ++j) *reinterpret_cast<f32x4*>(so + (w * 16 + c16) * D + (16 * j + 4 * r4)) = acc[j];
@@ -462,18 +444,25 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
         sm[w][c16] = mref;
         sl[w][c16] = lsum;
       }
-      lds_barrier();
-      for (int i = threadIdx.x; i < A.G * D; i += 256) {
+      const bool joined = cur.heads == 1;
+      if (joined) lds_barrier();
+      else asm volatile("" ::: "memory");   // a wave's LDS operations keep their order
+      const int count = joined || cur.tend > 0 ? A.G * D : 0, stride = joined ? 256 : 64;
+      for (int i = joined ? (int)threadIdx.x : lane; i < count; i += stride) {
         const int h = i / D, d = i % D;
-        float m = sm[0][h];
+        float m, o = 0.f, l = 0.f;
+        if (joined) {
+          m = sm[0][h];
 #pragma unroll
-        for (int k = 1; k < kWaves; ++k) m = fmaxf(m, sm[k][h]);
-        float o = 0.f, l = 0.f;
+          for (int k = 1; k < kWaves; ++k) m = fmaxf(m, sm[k][h]);
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-          const float a = fexp2(sm[k][h] - m);
-          l = __builtin_fmaf(sl[k][h], a, l);
-          o = __builtin_fmaf(so[(k * 16 + h) * D + d], a, o);
+          for (int k = 0; k < kWaves; ++k) {
+            const float a = fexp2(sm[k][h] - m);
+            l = __builtin_fmaf(sl[k][h], a, l);
+            o = __builtin_fmaf(so[(k * 16 + h) * D + d], a, o);
+          }
+        } else {
+          m = sm[w][h], l = sl[w][h], o = o + so[(w * 16 + h) * D + d];   // as joined: no -0
         }
         if (cur.splits == 1 && cur.from == 0) {
           orow[h * A.soh + d] = f32_to_bf16_rne(o / l);
@@ -483,7 +472,7 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
           if (d == 0) A.pml[p] = f32x2{m, l};
         }
       }
-      lds_barrier();   // the stages and the waves' m and l have been read
+      if (joined) lds_barrier();   // the stages and the waves' m and l have been read
     }
     if (after >= items) break;
     item = after;
