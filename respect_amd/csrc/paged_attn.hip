@@ -498,7 +498,10 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   constexpr int W = kShare >= 16 ? 16 : kShare > BITS ? kShare : BITS;
   constexpr int UR = RB / W, N = kTile * UR, UL = N > kTeam ? N / kTeam : 1;
   constexpr int E = W * 8 / BITS, EU = E / 8;
-  constexpr int kRoom = (D >= 128 ? (WR == 1 ? 64 : 48) : 32) / (UL * W / 2), PF = kRoom < 1 ? 1 : kRoom > 4 ? 4 : kRoom;   // registers in flight
+  // Steps in flight: as many as 64 registers hold (48 beside K operands read ahead; fewer where
+  // more waves than two share a SIMD's).
+  constexpr int kSet = UL * (W / 2 + (BITS < 16 ? 2 : 0)), kRoom = (D < 128 ? 32 : WR == 1 ? 64 : 48) / kSet;
+  constexpr int PF = kRoom < 1 ? 1 : kRoom > 4 ? 4 : kRoom;
   constexpr int NB = WR == 1 ? 1 : 2, kBytes = kTile * D * 2;                    // K or V of a step in LDS
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5, tid = threadIdx.x % kTeam, team = w / WR;
