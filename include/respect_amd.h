@@ -532,8 +532,7 @@ int rspx_kv_read(const void* k_codes, int64_t skch, int64_t skcn, const void* k_
                  int HK, int D, int format, void* stream);
 
 /* ---------------------------------------------------------------- paged attention, other caches
- * rspx_paged_attn_mx: rspx_paged_attn over pools of codes and scales (not RSPX_BF16), with the
- * same workspace.
+ * rspx_paged_attn_mx: rspx_paged_attn over pools of codes and scales (not RSPX_BF16).
  * rspx_paged_attn_shared: the same over pools of any format for a batch with groups of
  * consecutive sequences that begin with the same keys, which are read once for the group.
  * rspx_shared_plan: for n groups of members[i] sequences (all of the batch, in order), whose first
@@ -546,7 +545,9 @@ int rspx_kv_read(const void* k_codes, int64_t skch, int64_t skcn, const void* k_
  * pages and refusals as for rspx_paged_attn (a bad page among the shared ones: NaN for all who
  * read it).  The shared part rounds probabilities to bf16, half a step each, and sums them as
  * rounded.  A sequence's bits depend on its own keys and length and on its prefix alone.
- * workspace: rspx_paged_attn_shared_workspace_bytes, as for rspx_paged_attn.
+ * Slot strides of both calls are below 2 GB (RSPX_EUNSUPPORTED).
+ * workspace: rspx_paged_attn_shared_workspace_bytes (rspx_paged_attn_mx: with longest 0), as for
+ * rspx_paged_attn.
  */
 int rspx_paged_attn_mx(const void* q, int64_t sqb, int64_t sqh, const void* k_codes, int64_t skch, int64_t skcn,
                        const void* k_scales, int64_t sksh, int64_t sksn, const void* v_codes, int64_t svch, int64_t svcn,

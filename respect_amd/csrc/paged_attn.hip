@@ -9,11 +9,11 @@
 // A sequence of n keys is cut into splits of split_keys(n) keys, a function of n alone, so
 // a sequence's result does not depend on the rest of the batch nor on where its pages lie.
 // The lengths are known on the device only: as many workgroups as are resident at once list
-// the splits there are and take them in turn, (split, kv head) by (split, kv head), each
-// requesting the first tile of its next one before it joins the waves of the present one.
-// (A grid over every split that the table has room for, most of which end at once: 218 us
-// instead of 60 for 64 sequences of up to 8000 keys.)  A second launch joins a sequence's
-// splits, where the table has room for more than one.
+// the items there are and take them in turn, each requesting the first tile of its next one
+// before it joins the waves of the present one.  (A grid over every split that the table has room
+// for, most of which end at once: 218 us instead of 60 for 64 sequences of up to 8000 keys.)  An
+// item is a split for one kv head, or a sequence of at most a tile's keys for four, one a wave.
+// A second launch joins a sequence's splits, where the table has room for more than one.
 //
 // The four waves of a workgroup take the split's 32-key tiles in turn.  Scores are
 // S^T = K Q^T by v_mfma_f32_16x16x32_bf16 with the G heads of the group in the 16 columns
@@ -22,15 +22,22 @@
 // place as the B operand of O^T += V^T P^T, as two bf16 terms: p cut to bf16 and the rest
 // rounded to it (2^-15 of p is lost at most; the second product costs nothing next to the
 // memory traffic).  Both terms are positive, so that an infinite v gives no inf - inf.  V
-// goes from registers through a wave-private LDS stage to be read transposed.
+// goes from registers through a wave-private LDS stage to be read transposed.  Codes become
+// bf16 in registers, exactly.  (The products that take codes and their scales as they are would
+// save the conversions of K, but lose up to 2^-12 of the sum of their terms' sizes.)
 //
 // What bounds it: the K/V bytes, read once, where there are enough of them (one sequence of
-// 131072 keys and five shorter ones, 32 / 8 heads of 128: 822 MB in 149 us, 5.5 TB/s; 64
-// sequences of up to 8000: 260 MB in 64 us); below that the chain of dependent reads --
-// lengths, table, K/V, the second launch's partial sums (13 us for one sequence of 4097, whose
-// 17 MB take 3.3 of them).  Splits of 128 keys: 67 us instead of 64 for the batch, of 512: 17
-// instead of 13 for the one; at most 64 splits, or two tiles per wave requested at once: no
-// difference.
+// 131072 keys and five shorter ones, 32 / 8 heads of 128: 822 MB of bf16 in 146 us, 5.6 TB/s; 64
+// sequences of up to 8000: 260 MB in 48 us, 115 MB of mxfp8 in 31), and over 4-bit rows the
+// instructions that a wave spends on a tile (the 131072 keys in mxfp4: 152 MB in 36 us, 4.2 TB/s; one
+// wave per SIMD, with splits as long as bf16's, 46); below that the chain of dependent reads --
+// lengths, table, K/V, the second launch's partial sums (10 + 4 us for one sequence of 4097, whose
+// 17 MB of bf16 take 3.3 of them).  Splits of 128 keys: 67 us instead of 64 for bf16's batch, of
+// 512: 17 instead of 13 for the one; at most 64 splits for bf16, or two tiles per wave requested at
+// once: no difference.
+//
+// Keys that sequences of a batch share (prefix_rows, below) are split by their number alone, so that
+// who shares them does not matter either; their splits are joined with the sequence's own.
 #include <algorithm>
 
 #include "keys64.h"
@@ -45,7 +52,7 @@ constexpr int kTile = 32;            // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kSplitKeys = 256;      // the shortest split
 // A longer cache gets longer splits.  Rows of few bits are bound by the waves that take them
-// before they are by their bytes: twice the splits (131072 keys in 4 bits: SPLIT64).
+// before they are by their bytes: twice the splits (131072 keys in mxfp4: 36 us for 46).
 constexpr int most_splits(int bits) { return bits < 16 ? 64 : 32; }
 constexpr int kSeqs = 1024;          // sequences of a launch
 constexpr int kCUs = 256;
@@ -480,6 +487,15 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
   }
 }
 
+// What bounds shared keys: for few rows the serial chain of a launch and a split's steps (4
+// sequences behind 2496 keys: 11 us, 6 of them without any step); for many the partial sums, 520 bytes
+// per row and split, and the steps (64 behind 8000 keys of bf16, 54 MB: 30 us, 8 of them the sums'
+// 20 MB, where every sequence by itself would read 2.1 GB); for long ones the issue of a step's
+// instructions and its chain LDS -> scores -> exponentials -> products (24 behind 100032 keys of
+// mxfp4: 74 us, 0.53 PFLOP/s; without the products, staging alone 33).  20 splits up to 10240 keys:
+// with 32, 34 us for the 64 and 8.4 instead of 7.1 to join them; with 16, 13 for the 4.  Steps of 64
+// keys, one in flight: 168 us for the 24.
+//
 // What a tile says of shared keys: up to kPrefixRows rows (sequence b0 + r / G, head r % G of kv
 // head g) and up to 4 / WR splits of the keys they share.  A wave takes 32 rows through one split,
 // 32 keys a step; WR waves of different rows take the same split, and fetch its K and V together.

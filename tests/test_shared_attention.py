@@ -393,6 +393,25 @@ def test_bits_do_not_depend_on_who_shares(fmt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("k", [64, 320, 832])
+def test_any_number_of_members_gives_the_same_bits(fmt, D, k):
+    """One to 136 rows a kv head, blocks of 32, 64 and 128 and what is left of them, splits that do
+    not divide evenly among a workgroup's waves; own keys from none to more than a wave takes."""
+    from respect_amd.kernels.paged_attention import paged_attn
+    H, HK, page, B = 24, 3, 32, 17
+    lens = [k + (0, 1, 32, 33, 7)[i % 5] for i in range(B)]
+    kc, vc, table, rows = _cache(lens, page, HK, D, fmt, [B], [k], seed=D + k)
+    q, table = _q(B, H, D).cuda(), table.cuda()
+    all_ = paged_attn(q, kc, vc, table, _i32(lens), page, shared=_plan([B], [k], 8))
+    _check(all_, *_exact(q.cpu(), rows, shared=True))
+    for m in (2, 4, 5, 8, 9, 12, 16):
+        got = paged_attn(q[-m:], kc, vc, table[-m:], _i32(lens[-m:]), page, shared=_plan([m], [k], 8))
+        assert torch.equal(got, all_[-m:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_bad_pages_among_the_shared(fmt):
     """A page that is none: NaN for all who read it, through the group or alone; bad lengths; the
     others keep their bits."""
