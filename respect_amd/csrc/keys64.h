@@ -1,5 +1,6 @@
-// What the attention kernels that take 64 keys a step share: the layout of a step's K and V in
-// LDS, its reads, and the constants of the lazily moved reference maximum.
+// What prompt attention (64 keys a step) and attention over keys that sequences share (32 a step)
+// have in common: the layout of a step's K and V in LDS, its reads, and the constants of the lazily
+// moved reference maximum.
 #pragma once
 
 #include "common.h"
@@ -10,7 +11,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) char lds_char;
 
-constexpr int kKeys = 64;            // keys of a step
+constexpr int kKeys = 64;            // keys of a step of prompt attention; shared keys come in multiples of it
 constexpr float kTau = 8.0f;         // log2 headroom before the reference maximum moves
 constexpr float kNone = -1e30f;      // reference maximum before the first key
 

@@ -24,7 +24,7 @@ class MXRows:
     """A pool of rows [HK, slots, D]: ``codes`` uint8 [HK, slots, D * bits / 8] (16-byte aligned
     rows) and ``scales`` uint8 [HK, slots, D / 32], of ``format`` "mxfp8" or "mxfp4"."""
 
-    __slots__ = ("codes", "scales", "format", "bits", "shape", "device", "_args")
+    __slots__ = ("codes", "scales", "format", "bits", "shape", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, format: str):
         if format not in BITS:
@@ -43,7 +43,6 @@ class MXRows:
         self.codes, self.scales, self.format, self.bits = codes, scales, format, bits
         self.shape = (*codes.shape[:2], codes.shape[2] * 8 // bits)
         self.device = codes.device
-        self._args = (codes.data_ptr(), codes.stride(0), codes.stride(1), scales.data_ptr(), scales.stride(0), scales.stride(1))
 
     @classmethod
     def empty(cls, HK: int, slots: int, D: int, format: str, device="cuda") -> "MXRows":
@@ -55,7 +54,11 @@ class MXRows:
 
 
 def _pool_args(pool) -> tuple:
-    return pool._args if isinstance(pool, MXRows) else (pool.data_ptr(), pool.stride(0), pool.stride(1), None, 0, 0)
+    """A pool's part of a C call: rows and scales, each with its head and slot strides."""
+    if isinstance(pool, MXRows):
+        c, s = pool.codes, pool.scales
+        return c.data_ptr(), c.stride(0), c.stride(1), s.data_ptr(), s.stride(0), s.stride(1)
+    return pool.data_ptr(), pool.stride(0), pool.stride(1), None, 0, 0
 
 
 def _pools(what: str, kc, vc, slots: torch.Tensor) -> tuple[int, int, int, int]:
@@ -90,7 +93,7 @@ def write_rows(k: torch.Tensor, v: torch.Tensor, kc: MXRows, vc: MXRows, slots: 
     with torch.cuda.device(kc.device):
         rc = _lib.lib().rspx_kv_write_mx(
             k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), T, n,
-            *kc._args, *vc._args, HK, D, bits, _lib.stream_ptr(kc.device))
+            *_pool_args(kc), *_pool_args(vc), HK, D, bits, _lib.stream_ptr(kc.device))
     _lib.check("rspx_kv_write_mx", rc)
 
 
