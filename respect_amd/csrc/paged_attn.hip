@@ -134,21 +134,22 @@ __device__ __forceinline__ int list_items(const PagedArgs& A, int64_t cap, int* 
   const int B = A.B;
   __shared__ int waves[4];
   constexpr int kPer = kSeqs / 256;
-  int cnt[kPer], sum = 0;
+  // All loads before the first use: one after the other, 64 sequences in groups took 1.4 us longer.
+  int cnt[kPer], lens_of[kPer], prefix_of[kPer], sum = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int b = threadIdx.x * kPer + i;
-    cnt[i] = 0;
-    if (b < B) {
-      const int n = lens[b];
-      length[b] = n;
-      cnt[i] = n <= 0 || n > cap ? A.HK : item_count<BITS>(n, A.HK);
-      if constexpr (SHARED) {
-        const int p = from[b] = shared_keys(A, A.prefix[b], n);
-        if (p > 0) cnt[i] = item_count<BITS>(n - p, A.HK);
-      }
-    }
+    const int b = min((int)threadIdx.x * kPer + i, B - 1);
+    lens_of[i] = lens[b];
+    prefix_of[i] = SHARED ? A.prefix[b] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = threadIdx.x * kPer + i, n = lens_of[i];
+    const int p = SHARED ? shared_keys(A, prefix_of[i], n) : 0;
+    cnt[i] = b >= B ? 0 : n <= 0 || n > cap ? A.HK : item_count<BITS>(n - p, A.HK);
     sum += cnt[i];
+    length[b] = n;
+    if constexpr (SHARED) from[b] = p;
   }
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int run = sum;
@@ -760,9 +761,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs A) {
   f32x2 ml[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) ml[i] = lane + 64 * i < A.smax ? A.pml[p + lane + 64 * i] : f32x2{kNone, 0.f};   // beside the length
-  const int n = A.lens[b];
+  const int n = A.lens[b], prefix = SHARED ? A.prefix[b] : 0;
   if (n <= 0 || n > ((int64_t)A.width << A.shift)) return;
-  const int from = SHARED ? shared_keys(A, A.prefix[b], n) : 0;
+  const int from = SHARED ? shared_keys(A, prefix, n) : 0;
   const int splits = (from > 0 ? prefix_splits(from) : 0) + split_count<BITS>(n - from);
   if (splits == 1 && from == 0) return;
   const int c = threadIdx.x % L, part = threadIdx.x / L;
