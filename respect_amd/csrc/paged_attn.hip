@@ -493,7 +493,7 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 // per row and split, and the steps (64 behind 8000 keys of bf16, 54 MB: 30 us, 8 of them the sums'
 // 20 MB, where every sequence by itself would read 2.1 GB); for long ones the issue of a step's
 // instructions and its chain LDS -> scores -> exponentials -> products (24 behind 100032 keys of
-// mxfp4: 74 us, 0.53 PFLOP/s; without the products, staging alone 33).  20 splits up to 10240 keys:
+// mxfp4: 73 us, 0.54 PFLOP/s; without the products, staging alone 33).  20 splits up to 10240 keys:
 // with 32, 34 us for the 64 and 8.4 instead of 7.1 to join them; with 16, 13 for the 4.  Steps of 64
 // keys, one in flight: 168 us for the 24.
 //

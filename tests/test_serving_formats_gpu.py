@@ -175,3 +175,37 @@ def test_questions_about_a_document(model):
         _close(logits, other)
     cache.free([doc, *seqs, *plain])
     assert cache.free_pages == 400
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_two_streams_at_once(model, fmt):
+    """Appended tokens and shared steps of two groups, enqueued on two streams behind work that holds
+    both back: the bits of the same calls one after the other."""
+    def start():
+        cache = _cache(pages=600, dtype=fmt)
+        docs, _ = model.prefill_batch(_prompts([300, 700]), cache)
+        seqs = [cache.fork([d], 3) for d in docs]
+        return cache, seqs, [cache.shared(s, CFG["heads"]) for s in seqs]
+
+    def calls(cache, seqs, plans, which, step):
+        if step == 0:
+            return model.append_batch(_prompts([20, 3, 70], which), cache, seqs[which])
+        return model.step_batch(_tok(step, which, 7), cache, seqs[which], shared=plans[which])
+    state = start()
+    want = [[calls(*state, w, i) for w in (0, 1)] for i in range(5)]
+    state = start()
+    a = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            for _ in range(8):
+                torch.mm(a, a)
+    got = []
+    for i in range(5):
+        got.append([])
+        for w in (0, 1):
+            with torch.cuda.stream(streams[w]):
+                got[-1].append(calls(*state, w, i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for g, v in zip(got, want) for x, y in zip(g, v))
