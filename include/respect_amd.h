@@ -540,10 +540,11 @@ int rspx_kv_read(const void* k_codes, int64_t skch, int64_t skcn, const void* k_
  * each sequence that are taken together (keys[i] rounded down to whole steps of 64; 0 for a
  * group of one), and tiles [count][8] int32; returns count (prefix and tiles, host memory, may be
  * NULL).  Both go to the device as they are; longest: the largest of prefix.
- * Which pages a group's shared keys lie in is read from the table row of its first sequence.
- * A sequence of fewer keys than its prefix goes through all of its own by itself.  Lengths,
- * pages and refusals as for rspx_paged_attn (a bad page among the shared ones: NaN for all who
- * read it).  The shared part rounds probabilities to bf16, half a step each, and sums them as
+ * Which pages a group's shared keys lie in is read from the table rows of sequences of it that
+ * have so many keys, whose first ones have to be the same rows.
+ * A sequence of fewer keys than its prefix, be it the first of its group, goes through all of its
+ * own by itself.  Lengths, pages and refusals as for rspx_paged_attn (a bad page among the shared
+ * ones: NaN for all who read it).  The shared part rounds probabilities to bf16, half a step each, and sums them as
  * rounded.  A sequence's bits depend on its own keys and length and on its prefix alone.
  * Slot strides of both calls are below 2 GB (RSPX_EUNSUPPORTED).
  * workspace: rspx_paged_attn_shared_workspace_bytes (rspx_paged_attn_mx: with longest 0), as for

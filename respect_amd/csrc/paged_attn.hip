@@ -500,7 +500,8 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 // What a tile says of shared keys: up to kPrefixRows rows (sequence b0 + r / G, head r % G of kv
 // head g) and up to 4 / WR splits of the keys they share.  A wave takes 32 rows through one split,
 // 32 keys a step; WR waves of different rows take the same split, and fetch its K and V together.
-// What a wave computes of a row does not depend on WR, nor on the rows beside it.
+// What a wave computes of a row does not depend on WR, nor on the rows beside it.  The pages are those
+// of the tile's first sequence that has all the shared keys.
 //
 // K and V come through registers, PF steps ahead, where they become bf16, into LDS: where waves
 // share a split, into one of two slots while the other one is read, with one barrier a step.
@@ -529,6 +530,12 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   const int n = WR == 1 ? steps : (min(P - T[3] * per, per)) / kTile;            // the workgroup's longest
   if (WR == 1 && steps == 0) return;
   const bool active = rows > 0;
+  // The first sequence of the tile that has all P keys names their pages: a shorter one's row may hold
+  // anything behind its end.  Those of the tile's first one are requested beside the lengths.
+  int lead = b0 + row0 / A.G;
+  const int many = rows + 32 * (w % WR);
+  auto has = [&](int r) { return shared_keys(A, P, A.lens[b0 + (row0 + min(r, many - 1)) / A.G]) > 0 && r < many; };
+  const bool has_lo = has(lane), has_hi = WR == 4 && has(lane + 64);
   const int row = row0 + 32 * (w % WR) + min(col, max(rows - 1, 0));
   const int b = b0 + (active ? row / A.G : 0), h = g * A.G + (active ? row % A.G : 0);
   const int keys = A.lens[b], prefix = A.prefix[b];
@@ -541,7 +548,7 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
 
   // The page of key 32 t + lane % 32 of the split (of a step there is not: of the last one's), and
   // its slot, once that has come (0 where there is none).
-  const int* table = A.table + b0 * A.stb;
+  const int* table = A.table + (int64_t)lead * A.stb;
   bool bad = false;
   auto key_of = [&](int t) { return (steps > 0 ? key0 + kTile * min(t, steps - 1) : 0) + (lane & 31); };
   auto page_of = [&](int t) { return table[key_of(t) >> A.shift]; };
@@ -663,6 +670,16 @@ __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const
   int page[PF];
 #pragma unroll
   for (int i = 0; i < PF; ++i) page[i] = page_of(i);
+  {
+    const uint64_t lo = __builtin_amdgcn_ballot_w64(has_lo), hi = __builtin_amdgcn_ballot_w64(has_hi);
+    if ((lo | hi) == 0) return;                            // no row of the tile takes part
+    const int other = b0 + (row0 + (lo ? __builtin_ctzll(lo) : 64 + __builtin_ctzll(hi))) / A.G;
+    if (other != lead) {
+      table = A.table + (int64_t)(lead = other) * A.stb;
+#pragma unroll
+      for (int i = 0; i < PF; ++i) page[i] = page_of(i);
+    }
+  }
   auto next = [&](int set, int t) {
     const RowsOf x = rows_of(slot_of(t, page[set]));
     page[set] = page_of(t + PF);

@@ -24,7 +24,8 @@ class SharedPrefix:
     ``keys[0]`` keys, the next ``members[1]`` with the same ``keys[1]``, and so on over the whole
     batch (0 keys, or one member: nothing is shared).  ``group``: query heads per kv head, up to 16.
     Made once for a batch and used by every layer and step, as long as the rows stay shared:
-    sequences may grow, and one that has become shorter than its ``keys`` is taken by itself.
+    sequences may grow, and any that has become shorter than its ``keys`` is taken by itself.  One
+    that is as long again, but holds rows of its own there, needs a new plan.
     Whole steps of 64 keys are shared, the rest is left to the sequences (``prefix``)."""
 
     def __init__(self, members, keys, group: int, device="cuda"):
@@ -59,8 +60,8 @@ def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None, share
     that reads a page outside the pool, gets NaN.  ``page``: a power of two.  ``out``: written
     in place if given; no memory of the other tensors.  Scores as for ``prompt_attn``.
 
-    ``shared``: which sequences begin alike.  The table row of a group's first sequence names
-    the pages of the keys that it shares.  Probabilities of these keys are rounded to bf16, so
+    ``shared``: which sequences begin alike.  The pages of the keys that a group shares are read
+    from the table rows of sequences that have them all.  Probabilities of these keys are rounded to bf16, so
     the result is not that without ``shared`` bit for bit; it depends on a sequence's own keys,
     length and shared keys, and not on who shares them."""
     mx = isinstance(kc, MXRows)
