@@ -621,6 +621,8 @@ int rspx_kv_write(const void* k, int64_t skt, int64_t skh, const void* v, int64_
  *   shared   the batch ids cut into groups of consecutive sequences that begin with the same full
  *            pages, so that most keys are shared: writes members and keys (of each group; n of
  *            room) and returns their number.  Fewer than `least` keys count as none
+ *   alike    of groups of members[i] consecutive ones of ids (`groups` of them, all of ids): 1 if
+ *            in each all sequences of keys[i] rows or more hold those in the same pages, else 0
  */
 typedef struct rspx_pages rspx_pages;
 rspx_pages* rspx_pages_new(int pages, int page, int sequences); /* NULL: bad sizes or no memory */
@@ -641,6 +643,7 @@ int rspx_pages_width(rspx_pages* p, const int32_t* ids, int n);
 int rspx_pages_table(rspx_pages* p, const int32_t* ids, int n, int width, int32_t* table, int32_t* lens);
 int rspx_pages_slots(rspx_pages* p, const int32_t* ids, int n, const int64_t* first, const int64_t* counts, int32_t* out);
 int rspx_pages_shared(rspx_pages* p, const int32_t* ids, int n, int64_t least, int64_t* members, int64_t* keys);
+int rspx_pages_alike(rspx_pages* p, const int32_t* ids, int n, const int64_t* members, const int64_t* keys, int groups);
 
 /* ---------------------------------------------------------------- scores of given tokens
  * Per row of logits [M, V] (fp32, row stride sl, any 4-byte alignment), with columns

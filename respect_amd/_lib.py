@@ -134,6 +134,7 @@ SIGNATURES: dict[str, tuple] = {
     "rspx_pages_table": (_i32, [_c_p, _c_p, _i32, _i32, _c_p, _c_p]),
     "rspx_pages_slots": (_i32, [_c_p, _c_p, _i32, _c_p, _c_p, _c_p]),
     "rspx_pages_shared": (_i32, [_c_p, _c_p, _i32, _i64, _c_p, _c_p]),
+    "rspx_pages_alike": (_i32, [_c_p, _c_p, _i32, _c_p, _c_p, _i32]),
     "rspx_token_logprobs_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "rspx_token_logprobs": (_i32, [_c_p, _i64, _i32, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _c_p, _i64,
                                    _c_p]),

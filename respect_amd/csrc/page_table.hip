@@ -457,3 +457,24 @@ extern "C" int rspx_pages_shared(rspx_pages* p, const int32_t* ids, int n, int64
     return groups;
   });
 }
+
+extern "C" int rspx_pages_alike(rspx_pages* p, const int32_t* ids, int n, const int64_t* members, const int64_t* keys, int groups) {
+  if (!p || groups < 0 || (groups > 0 && (!members || !keys))) return RSPX_EINVAL;
+  if (const int rc = check_ids(*p, ids, n, false)) return rc;
+  int64_t at = 0;
+  for (int i = 0; i < groups; ++i) {
+    if (members[i] < 0 || keys[i] < 0 || members[i] > n - at) return RSPX_EINVAL;
+    at += members[i];
+  }
+  if (at != n) return RSPX_EINVAL;
+  for (int i = 0; i < groups; ids += members[i++]) {
+    const int32_t* first = nullptr;   // the pages of the first one that is long enough
+    for (int64_t k = 0; k < members[i]; ++k) {
+      if (p->len[ids[k]] < keys[i]) continue;
+      const int32_t* held = p->held[ids[k]].data();
+      if (!first) first = held;
+      else if (!std::equal(first, first + pages_for(*p, keys[i]), held)) return 0;
+    }
+  }
+  return 1;
+}

@@ -438,8 +438,9 @@ class Decoder:
         ``cache``, appended to them.  Returns fp32 logits [B, V].  A sequence's results do not
         depend on the others.  ``shared``: ``cache.shared(seqs, heads)``, made once for these
         sequences in this order and used for all their steps: rows that they begin with alike are
-        then read once.  A step that fails leaves the sequences and the free pages as they
-        were."""
+        then read once.  A plan that is not right for them (``cache.holds``: another batch's, or one
+        of them was freed, or compacted and grown again) is refused (``ValueError``).  A step that
+        fails leaves the sequences and the free pages as they were."""
         self._check_paged(cache)
         seqs = list(seqs)
         if tuple(ids.shape) != (len(seqs),) or not seqs:
@@ -455,6 +456,8 @@ class Decoder:
     def _step_batch(self, ids, cache, seqs, n: list[int], shared) -> torch.Tensor:
         """step_batch for sequences that have been extended to ``n`` rows."""
         cfg, B = self.cfg, len(seqs)
+        if shared is not None and not cache.holds(seqs, shared):
+            raise ValueError("step_batch: the sequences do not share the rows that the plan says")
         slots = cache.slots(seqs, [m - 1 for m in n], 1)
         table, lens = cache.tables(seqs)
         att = torch.empty((B, cfg.heads, cfg.head_dim), dtype=torch.bfloat16, device=self.device)

@@ -159,6 +159,17 @@ class PageTable:
             self.refuse("shared", n)
         return members[:n].tolist(), keys[:n].tolist()
 
+    def alike(self, seqs, members: np.ndarray, keys: np.ndarray) -> bool:
+        """Whether in each group of members[i] consecutive ones of ``seqs`` all that have keys[i] rows
+        hold those in the same pages."""
+        ids = self._ids(seqs)
+        if members.sum() != len(ids):
+            return False
+        y = self._lib.rspx_pages_alike(self.handle, _p(ids), len(ids), _p(members), _p(keys), len(members))
+        if y < 0:
+            self.refuse("alike", y)
+        return y == 1
+
     def slots(self, seqs, first, count) -> np.ndarray:
         ids = self._ids(seqs)
         lo, n = self._counts(first, len(ids)), self._counts(count, len(ids))
@@ -341,12 +352,19 @@ class PagedKVCache:
     def shared(self, seqs, heads: int, least: int = 256) -> SharedPrefix:
         """The plan by which ``paged_attn`` and ``Decoder.step_batch`` take the pages that
         consecutive ones of ``seqs`` begin with in common once, for ``heads`` query heads: forks
-        stand side by side.  Groups that share fewer than ``least`` keys are none.  It holds while
-        the sequences grow, and until one of them is compacted into those pages or freed."""
+        stand side by side.  Groups that share fewer than ``least`` keys are none.  It holds (``holds``)
+        while the sequences grow, and until one of them is freed, or compacted into those pages and
+        then extended past them."""
         heads = operator.index(heads)
         if heads < 1 or heads % self.HK:
             raise ValueError(f"PagedKVCache.shared: {heads} heads over {self.HK} kv heads")
         return SharedPrefix(*self._t.shared(seqs, least), heads // self.HK, device=self.device)
+
+    def holds(self, seqs, shared: SharedPrefix) -> bool:
+        """Whether the plan ``shared`` is right for ``seqs`` as they are now: all of a group that have the
+        keys it shares hold them in the same pages (a shorter one is taken by itself).  Books on the
+        host alone; ``paged_attn`` does not look."""
+        return self._t.alike(seqs, *shared.groups)
 
     def read(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(k, v) [T, HK, D] bf16: the pool rows ``slots`` [T] (device int32) of one layer, as

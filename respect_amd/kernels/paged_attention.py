@@ -45,7 +45,10 @@ class SharedPrefix:
         host = torch.empty(8 * count + self.B, dtype=torch.int32, pin_memory=on_gpu)
         at = host.data_ptr()
         L.rspx_shared_plan(*args, at + 32 * count, at)
-        self.longest = int(host[8 * count:].max()) if self.B else 0
+        prefix = host[8 * count:].numpy()
+        self.longest = int(prefix.max()) if self.B else 0
+        first = np.minimum(m.cumsum() - m, max(self.B - 1, 0))
+        self.groups = m, np.where(m > 0, prefix[first], 0).astype(np.int64) if self.B else 0 * k   # members, keys taken together
         flat = host.to(self.device)                # waited for: any stream may use the plan
         self.tiles, self.prefix = flat[:8 * count].view(count, 8), flat[8 * count:]
 
