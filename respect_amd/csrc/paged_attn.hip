@@ -978,12 +978,12 @@ extern "C" int64_t rspx_shared_plan(const int64_t* members, const int64_t* keys,
     const int rows = (int)members[i] * group, splits = p ? prefix_splits(p) : 0;
     // The row blocks of a split beside one another: they read the same keys.
     for (int split = 0; split < splits; split += 4)
-      for (int r = 0; r < rows; r += kPrefixRows) {
-        const int part = std::min(rows - r, kPrefixRows), each = 4 / prefix_waves(part);
+      for (int64_t r = 0; r < rows; r += kPrefixRows) {    // past the last of 2^31 - 16 rows it is 2^31
+        const int part = (int)std::min<int64_t>(rows - r, kPrefixRows), each = 4 / prefix_waves(part);
         for (int k = split; k < std::min(split + 4, splits); k += each, ++count)
           if (tiles) {
             int32_t* t = tiles + count * kTileInts;
-            t[0] = (int32_t)b, t[1] = part, t[2] = r, t[3] = k, t[4] = std::min({each, splits - k, split + 4 - k});
+            t[0] = (int32_t)b, t[1] = part, t[2] = (int32_t)r, t[3] = k, t[4] = std::min({each, splits - k, split + 4 - k});
             t[5] = p, t[6] = t[7] = 0;
           }
       }

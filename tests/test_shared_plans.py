@@ -116,6 +116,18 @@ def test_alike_against_tables():
         assert y == -1
 
 
+def test_the_largest_group():
+    """2^27 - 1 sequences of 16 heads: the plan's tiles are counted to the end."""
+    from respect_amd import _lib
+    _forks()
+    most = 2 ** 27 - 1
+    for members, tiles in (([most], 2 ** 24), ([most - 1], 2 ** 24), ([5, most - 5], 2 ** 24), ([most - 8], 2 ** 24 - 1),
+                           ([most + 1], -1), ([most, 1], -1)):
+        m, k = np.array(members, np.int64), np.full(len(members), 100, np.int64)
+        want = tiles if len(members) == 1 or tiles < 0 else 1 + 2 ** 24
+        assert _lib.lib().rspx_shared_plan(m.ctypes.data, k.ctypes.data, len(m), 16, None, None) == want, members
+
+
 # ------------------------------------------------------------------ on the GPU
 
 CFG = dict(layers=2, hidden=512, heads=4, kv_heads=2, head_dim=128, ffn=1024, vocab=4096)
