@@ -153,6 +153,7 @@ class PageTable:
         """(members, keys): ``seqs`` cut into groups of consecutive sequences that begin with the
         same full pages, so that most keys are shared; fewer than ``least`` keys count as none."""
         ids = self._ids(seqs)
+        least = max(-1, min(operator.index(least), (1 << 63) - 1))   # any number, in 64 bits
         members, keys = np.empty(len(ids), np.int64), np.empty(len(ids), np.int64)
         n = self._lib.rspx_pages_shared(self.handle, _p(ids), len(ids), least, _p(members), _p(keys))
         if n < 0:

@@ -116,6 +116,18 @@ def test_alike_against_tables():
         assert y == -1
 
 
+def test_least_is_a_whole_number_of_any_size():
+    cache, seqs, _ = _forks()
+    for least, longest in ((0, 640), (256, 640), (641, 0), (1 << 31, 0), (1 << 63, 0), (1 << 64, 0), ((1 << 64) + 5, 0)):
+        assert cache.shared(seqs, 8, least=least).longest == longest
+    for least in (-1, -(1 << 63) - 1, -(1 << 64)):
+        with pytest.raises(ValueError):
+            cache.shared(seqs, 8, least=least)
+    for least in (2.5, None, "3"):
+        with pytest.raises(TypeError):
+            cache.shared(seqs, 8, least=least)
+
+
 def test_the_largest_group():
     """2^27 - 1 sequences of 16 heads: the plan's tiles are counted to the end."""
     from respect_amd import _lib
