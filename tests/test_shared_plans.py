@@ -118,7 +118,7 @@ def test_alike_against_tables():
 
 def test_least_is_a_whole_number_of_any_size():
     cache, seqs, _ = _forks()
-    for least, longest in ((0, 640), (256, 640), (641, 0), (1 << 31, 0), (1 << 63, 0), (1 << 64, 0), ((1 << 64) + 5, 0)):
+    for least, longest in ((0, 640), (256, 640), (688, 640), (689, 0), (1 << 31, 0), (1 << 63, 0), (1 << 64, 0), ((1 << 64) + 5, 0)):
         assert cache.shared(seqs, 8, least=least).longest == longest
     for least in (-1, -(1 << 63) - 1, -(1 << 64)):
         with pytest.raises(ValueError):
