@@ -26,15 +26,16 @@
 // bf16 in registers, exactly.  (The products that take codes and their scales as they are would
 // save the conversions of K, but lose up to 2^-12 of the sum of their terms' sizes.)
 //
-// What bounds it: the K/V bytes, read once, where there are enough of them (one sequence of
-// 131072 keys and five shorter ones, 32 / 8 heads of 128: 822 MB of bf16 in 146 us, 5.6 TB/s; 64
-// sequences of up to 8000: 260 MB in 48 us, 115 MB of mxfp8 in 31), and over 4-bit rows the
-// instructions that a wave spends on a tile (the 131072 keys in mxfp4: 152 MB in 36 us, 4.2 TB/s; one
-// wave per SIMD, with splits as long as bf16's, 46); below that the chain of dependent reads --
-// lengths, table, K/V, the second launch's partial sums (10 + 4 us for one sequence of 4097, whose
-// 17 MB of bf16 take 3.3 of them).  Splits of 128 keys: 67 us instead of 64 for bf16's batch, of
-// 512: 17 instead of 13 for the one; at most 64 splits for bf16, or two tiles per wave requested at
-// once: no difference.
+// What bounds it: the K/V bytes, read once, where there are enough of them, and over 4-bit rows the
+// instructions that a wave spends on a tile.  32 / 8 heads of 128, the same lengths in each format:
+//   140161 keys, 131072 of them in one of six sequences: 574 MB of bf16 in 106 us (5.4 TB/s), 296 MB
+//   of mxfp8 in 51 (5.8), 152 MB of mxfp4 in 36 (4.2; one wave per SIMD, splits as long as bf16's: 46)
+//   54237 keys of 64 sequences of up to 8000: 222 MB in 43 us, 115 MB in 31, 59 MB in 27
+// Below that the chain of dependent reads -- lengths, table, K/V, the second launch's partial sums
+// (10 + 4 us for one sequence of 4097, whose 17 MB of bf16 take 3.3 of them).  With an earlier form
+// over bf16: splits of 128 keys, 67 us instead of 64 for 64 sequences of up to 8000; of 512, 17
+// instead of 13 for the one of 4097; at most 64 splits, or two tiles per wave requested at once: no
+// difference.
 //
 // Keys that sequences of a batch share (prefix_rows, below) are split by their number alone, so that
 // who shares them does not matter either; their splits are joined with the sequence's own.

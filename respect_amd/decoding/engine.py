@@ -397,8 +397,13 @@ class Decoder:
         ``seqs`` of ``cache``, all in one pass: the next turn of conversations, the questions about a
         document that was forked.  Returns logits [B, V] of each one's last token.  Attention reads
         the sequences' rows back from the cache (``cache.read``), the new ones among them, and runs
-        as in ``prefill_batch``.  A sequence's results do not depend on the others.  A pass that
-        fails leaves the sequences and the free pages as they were."""
+        as in ``prefill_batch``: over a bf16 cache with the bits of one prompt in one piece.  A
+        sequence's results do not depend on the others.  The pass takes scratch for all rows that the
+        sequences hold, beside that of ``prefill_batch`` for the new ones: 2 kv_heads head_dim bf16
+        each (4 KB at the 8B sizes), in which rows that forks share count once for each fork, and every layer
+        reads and writes them (24 forks of 100000 rows: 9.8 GB, 4.4 ms a layer): for many
+        questions to one long document, append to a few forks at a time.  A pass that fails leaves
+        the sequences and the free pages as they were."""
         self._check_paged(cache)
         prompts, seqs = list(prompts), list(seqs)
         rows = [int(p.shape[0]) for p in prompts]
@@ -438,7 +443,8 @@ class Decoder:
         ``cache``, appended to them.  Returns fp32 logits [B, V].  A sequence's results do not
         depend on the others.  ``shared``: ``cache.shared(seqs, heads)``, made once for these
         sequences in this order and used for all their steps: rows that they begin with alike are
-        then read once.  A plan that is not right for them (``cache.holds``: another batch's, or one
+        then read once.  Their probabilities are rounded to bf16 then (``paged_attn``), so that results
+        also depend on how many rows the plan says a sequence shares, still not on with whom.  A plan that is not right for them (``cache.holds``: another batch's, or one
         of them was freed, or compacted and grown again) is refused (``ValueError``).  A step that
         fails leaves the sequences and the free pages as they were."""
         self._check_paged(cache)

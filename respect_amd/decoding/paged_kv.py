@@ -355,7 +355,12 @@ class PagedKVCache:
         consecutive ones of ``seqs`` begin with in common once, for ``heads`` query heads: forks
         stand side by side.  Groups that share fewer than ``least`` keys are none.  It holds (``holds``)
         while the sequences grow, and until one of them is freed, or compacted into those pages and
-        then extended past them."""
+        then extended past them.
+
+        Attention with a plan rounds the shared keys' probabilities to bf16 (``paged_attn``).  It is
+        faster where many share much: with 32 / 8 heads of 128 from 4 sequences of bf16 or 8 of few
+        bits behind 4096 keys on.  Few sequences over few kv heads lose by it (two behind 100000
+        keys of mxfp4 with 2 kv heads: 75 us a layer instead of 26)."""
         heads = operator.index(heads)
         if heads < 1 or heads % self.HK:
             raise ValueError(f"PagedKVCache.shared: {heads} heads over {self.HK} kv heads")

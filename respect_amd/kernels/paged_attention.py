@@ -64,9 +64,11 @@ def paged_attn(q, kc, vc, table, lens, page: int, sm_scale=None, out=None, share
     in place if given; no memory of the other tensors.  Scores as for ``prompt_attn``.
 
     ``shared``: which sequences begin alike.  The pages of the keys that a group shares are read
-    from the table rows of sequences that have them all.  Probabilities of these keys are rounded to bf16, so
-    the result is not that without ``shared`` bit for bit; it depends on a sequence's own keys,
-    length and shared keys, and not on who shares them."""
+    from the table rows of sequences that have them all.  Probabilities of these keys are rounded to
+    bf16, each by at most 2^-8 of itself (without ``shared`` by 2^-15), as in ``prompt_attn``, and an
+    infinite value makes NaN where its probability is 0: the result is not that without ``shared`` bit
+    for bit.  It depends on a sequence's own keys, length and shared keys, and not on who shares
+    them.  The plan has to be kept as long as a graph that captured the call."""
     mx = isinstance(kc, MXRows)
     if out is None:
         if not mx and shared is None:
