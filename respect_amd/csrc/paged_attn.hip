@@ -508,7 +508,10 @@ __device__ __forceinline__ void paged_items(const PagedArgs& A, int block, int b
 // share a split, into one of two slots while the other one is read, with one barrier a step.
 // S^T = K Q^T by v_mfma_f32_32x32x16_bf16 leaves a row's scores in one lane and its neighbour of
 // the other half; the probabilities, rounded to bf16 (half a step each) and summed as rounded, are
-// used in place.  Every row sees all keys: there is no mask.
+// used in place.  Every row sees all keys: there is no mask.  One term of p, as prompt attention has,
+// and not the two of the sequences' own keys, since here products bound: with two, errors are those of
+// a call without shared keys (0.0017 of the result's norm instead of 0.0023), and the 24 rows' 73 us become 94,
+// the 64's 30 become 35, the 4's 10.5 become 11.6.
 template <int D, int BITS, int WR>
 __device__ __forceinline__ void prefix_rows(const PagedArgs& A, int total, const int (&T)[kTileInts], int g, char* lds) {
   constexpr int U = D / 8, NS = D / 16, DT = D / 32;
